@@ -455,6 +455,64 @@ int specdec_linear_silu(const void *x, int64_t x_stride, const void *w, int64_t 
                         int64_t hidden_stride, int64_t hidden_dim, float eps, void *out,
                         int64_t out_stride, void *stream);
 
+/* ------------------------------------------------------- 8-bit projections --- */
+
+/* Rows in 8 bits, with a scale for each group of 128 values along the row
+ * (the last group may be shorter).  A group's scale is the least power of two
+ * s = 2^e, e >= -126, with max |y| <= 448 s over the group's finite values; a
+ * code is y / s rounded once, to nearest even, to e4m3 (OCP, largest value
+ * 448); an infinity or NaN becomes a NaN code and leaves its group's scale to
+ * the others.  A row of K values is stored as
+ *   codes   128 ceil(K / 128) bytes, zeros past K
+ *   scales  4 ceil(K / 512) bytes, e8m0 (e + 127), ones (127) past the groups
+ * rows one behind the other, codes 16-byte and scales 4-byte aligned.
+ *
+ * The three entries below write it from bf16 or fp32 rows (dtype), the values
+ * kept in fp32 up to the one rounding.  Input rows need no alignment beyond
+ * their element's.  A row's codes do not depend on the other rows.  No
+ * counterpart in the reference, whose projections run in the model's type. */
+
+/* y = x: rows [rows, dim], row_stride apart. */
+int specdec_quantize_fp8(const void *x, int dtype, int64_t rows, int64_t dim, int64_t row_stride,
+                         void *codes, void *scales, void *stream);
+
+/* y = SiLU(gate) * up, SiLU(g) = g / (1 + e^-g): gate_up [rows, 2*inter] holds
+ * gate then up per row (row_stride apart), as specdec_silu_mul reads it. */
+int specdec_silu_mul_fp8(const void *gate_up, int dtype, int64_t rows, int64_t inter,
+                         int64_t row_stride, void *codes, void *scales, void *stream);
+
+/* Residual addition and RMSNorm: with delta not null, h = hidden + delta
+ * rounded to the element type, written to `summed` (which may be hidden
+ * itself); else h = hidden and `summed` is not used.  Then
+ * y = h * rsqrt(mean(h^2) + eps) * weight.  hidden, delta and summed
+ * [rows, dim] contiguous, weight [dim]; dim <= 16384 (else
+ * SPECDEC_EUNSUPPORTED). */
+int specdec_add_rmsnorm_fp8(const void *hidden, const void *delta, const void *weight, void *summed,
+                            int dtype, int64_t rows, int64_t dim, float eps, void *codes,
+                            void *scales, void *stream);
+
+/* out [rows, out_features] bf16 (out_stride apart) = x w^T, or x w^T + add,
+ * rounded once to bf16 (nearest even), with x [rows, in_codes] and w
+ * [out_features, in_codes] in the format above: in_codes % 128 == 0 counts a
+ * row's codes with their padding.  Products are accumulated in fp32 by the
+ * scaled fp8 MFMA, which drops what lies more than 13 bits below the largest of
+ * eight products before it adds them (measured: 1.3e-5 of a result's size for
+ * normal data at any in_codes, against 2e-3 for the rounding to bf16).
+ * x codes x_stride apart (16-byte aligned, stride % 16 == 0), x_scales
+ * x_scale_stride apart (4-byte aligned, stride % 4 == 0).  w is tiled: the
+ * 2 KB block of feature tile t and group s at (t * in_codes / 128 + s) * 2048,
+ * element (n, k) of it at
+ *   (k % 128 / 64) * 1024 + ((k % 64 / 16) * 16 + n % 16) * 16 + k % 16,
+ * features past out_features zero; 16-byte aligned.  w_scales
+ * [out_features, 4 ceil(in_codes / 512)].  add (null for none) bf16, rows
+ * add_stride apart; it may be out itself and may not overlap it otherwise.
+ * Calls of at most 64 rows give a row the same bits whatever rows come with
+ * it. */
+int specdec_linear_fp8(const void *x, int64_t x_stride, const void *x_scales, int64_t x_scale_stride,
+                       const void *w, const void *w_scales, int64_t rows, int64_t in_codes,
+                       int64_t out_features, const void *add, int64_t add_stride, void *out,
+                       int64_t out_stride, void *stream);
+
 /* ------------------------------------------------------------------ head --- */
 
 /* Output head: logits [rows, vocab] fp32 (logits_stride apart) = x [rows,

@@ -408,6 +408,185 @@ def linear_silu(x: torch.Tensor, w: torch.Tensor, hidden: torch.Tensor, out: tor
     return out
 
 
+# ------------------------------------------------------- 8-bit projections --
+FP8_GROUP = 128  # values that share a scale
+FP8_CODE, FP8_SCALE = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
+def fp8_code_cols(k: int) -> int:
+    """Codes of a row of k values: whole groups, zeros past k."""
+    return -(-k // FP8_GROUP) * FP8_GROUP
+
+
+def fp8_scale_cols(k: int) -> int:
+    """Scales of a row of k values: a multiple of four, ones past the groups."""
+    return -(-k // (4 * FP8_GROUP)) * 4
+
+
+def _launch(dev: torch.device, entry, *args) -> int:
+    """`entry` on the current stream of `dev`, which need not be the current device."""
+    if _device_index is None or _device_index() == dev.index:
+        return entry(*args, stream())
+    with torch.cuda.device(dev):
+        return entry(*args, stream())
+
+
+def _fp8_rows(dev: torch.device, lead, k: int, codes: torch.Tensor | None, scales: torch.Tensor | None):
+    """codes [*lead, Kp] and scales [*lead, Gp] of rows of k values: given and checked, or new."""
+    cshape, sshape = (*lead, fp8_code_cols(k)), (*lead, fp8_scale_cols(k))
+    for t, shape, dtype, align, name in ((codes, cshape, FP8_CODE, 16, "codes"), (scales, sshape, FP8_SCALE, 4, "scales")):
+        if t is not None:
+            _on(dev, t, name, dtype, True)
+            if tuple(t.shape) != shape:
+                raise ValueError(f"{name} must be {list(shape)} (got {list(t.shape)})")
+            if t.data_ptr() % align:
+                raise ValueError(f"{name} must be {align}-byte aligned")
+    if codes is None:
+        codes = torch.empty(cshape, dtype=FP8_CODE, device=dev)
+    if scales is None:
+        scales = torch.empty(sshape, dtype=FP8_SCALE, device=dev)
+    return codes, scales
+
+
+def _fp8_input(x: torch.Tensor, name: str) -> tuple[torch.Tensor, int]:
+    """x as rows [R, K] of unit inner stride, bf16 or fp32."""
+    gpu(x, name)
+    if x.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"{name} must be bf16 or fp32 (got {x.dtype})")
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError(f"{name} needs rows of at least one value (got {list(x.shape)})")
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    if x2.stride(1) != 1 or x2.shape[0] > 1 and x2.stride(0) < x2.shape[1]:  # transposed, or overlapping rows
+        x2 = x2.contiguous()
+    return x2, _DTYPES[x.dtype]
+
+
+def quantize_fp8(x: torch.Tensor, codes: torch.Tensor | None = None, scales: torch.Tensor | None = None):
+    """Rows of x [..., K] (bf16 or fp32) in 8 bits: codes float8_e4m3fn
+    [..., 128 ceil(K / 128)] and scales float8_e8m0fnu [..., 4 ceil(K / 512)].
+
+    Each group of 128 values along a row (the last may be shorter) has the
+    least power of two s >= 2^-126 with max |y| <= 448 s over its finite
+    values as its scale, and y / s rounded to nearest even as its codes; an
+    infinity or NaN becomes a NaN code.  Codes past K are zeros, scales past
+    the groups ones.  `codes` and `scales` take the results where given."""
+    x2, dt = _fp8_input(x, "x")
+    codes, scales = _fp8_rows(x.device, x.shape[:-1], x2.shape[1], codes, scales)
+    st = _launch(x.device, lib().specdec_quantize_fp8, x2.data_ptr(), dt, x2.shape[0], x2.shape[1], x2.stride(0),
+                 codes.data_ptr(), scales.data_ptr())
+    _check(st, "quantize_fp8")
+    return codes, scales
+
+
+def silu_mul_fp8(gate_up: torch.Tensor, codes: torch.Tensor | None = None, scales: torch.Tensor | None = None):
+    """quantize_fp8(SiLU(gate) * up) of gate_up [..., 2 I] (gate then up, bf16
+    or fp32), computed in fp32 with the one rounding to 8 bits."""
+    x2, dt = _fp8_input(gate_up, "gate_up")
+    if x2.shape[1] % 2:
+        raise ValueError(f"gate_up rows hold gate then up, an even number of values (got {x2.shape[1]})")
+    inter = x2.shape[1] // 2
+    codes, scales = _fp8_rows(gate_up.device, gate_up.shape[:-1], inter, codes, scales)
+    st = _launch(gate_up.device, lib().specdec_silu_mul_fp8, x2.data_ptr(), dt, x2.shape[0], inter, x2.stride(0),
+                 codes.data_ptr(), scales.data_ptr())
+    _check(st, "silu_mul_fp8")
+    return codes, scales
+
+
+def add_rmsnorm_fp8(hidden: torch.Tensor, delta: torch.Tensor | None, weight: torch.Tensor, eps: float,
+                    codes: torch.Tensor | None = None, scales: torch.Tensor | None = None,
+                    summed: torch.Tensor | None = None):
+    """h = hidden + delta (if given, rounded to hidden's type and written to
+    `summed`, else back to hidden), then quantize_fp8(h * rsqrt(mean(h^2) +
+    eps) * weight), the norm in fp32 with the one rounding to 8 bits.  hidden,
+    delta and summed [..., D] contiguous, bf16 or fp32, D <= 16384."""
+    dev = gpu(hidden, "hidden").device
+    if hidden.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"hidden must be bf16 or fp32 (got {hidden.dtype})")
+    if hidden.dim() < 1 or hidden.shape[-1] == 0:
+        raise ValueError(f"hidden needs rows of at least one value (got {list(hidden.shape)})")
+    dim = hidden.shape[-1]
+    _on(dev, hidden, "hidden", contiguous=True)
+    _on(dev, weight, "weight", hidden.dtype, True, dim)
+    if delta is not None:
+        _on(dev, delta, "delta", hidden.dtype, True, hidden.numel())
+        summed = hidden if summed is None else _on(dev, summed, "summed", hidden.dtype, True, hidden.numel())
+    elif summed is not None:
+        raise ValueError("summed is written where there is a delta only")
+    codes, scales = _fp8_rows(dev, hidden.shape[:-1], dim, codes, scales)
+    st = _launch(dev, lib().specdec_add_rmsnorm_fp8, hidden.data_ptr(), ptr(delta), weight.data_ptr(), ptr(summed),
+                 _DTYPES[hidden.dtype], hidden.numel() // dim, dim, float(eps), codes.data_ptr(), scales.data_ptr())
+    _check(st, "add_rmsnorm_fp8")
+    return codes, scales
+
+
+def tile_weight_fp8(codes: torch.Tensor) -> torch.Tensor:
+    """Weight codes [N, Kp] (quantize_fp8 of W [N, K]) in the layout that
+    linear_fp8 reads, [ceil(N / 16), Kp / 128, 2, 64, 16]: 16 features by 128
+    inputs are 2 KB, lane 16 g + c of half h holding feature c's inputs
+    64 h + 16 g .. 64 h + 16 g + 15, so each load instruction reads one
+    contiguous KB.  Features past N are zeros.  Made once per weight."""
+    if codes.dim() != 2 or codes.dtype != FP8_CODE or codes.shape[0] == 0 or codes.shape[1] == 0 \
+            or codes.shape[1] % FP8_GROUP:
+        raise ValueError(f"a tiled weight is made of float8_e4m3fn codes [N, Kp], Kp % {FP8_GROUP} == 0 "
+                         f"(got {codes.dtype} {list(codes.shape)})")
+    n, kp = codes.shape
+    tiles = -(-n // 16)
+    raw = codes.view(torch.uint8)
+    if tiles * 16 > n:
+        raw = torch.cat([raw, raw.new_zeros(tiles * 16 - n, kp)])
+    t = raw.reshape(tiles, 16, kp // 128, 2, 4, 16).permute(0, 2, 3, 4, 1, 5)
+    return t.reshape(tiles, kp // 128, 2, 64, 16).contiguous().view(FP8_CODE)
+
+
+def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor,
+               out: torch.Tensor | None = None, add: torch.Tensor | None = None) -> torch.Tensor:
+    """The product of 8-bit rows (codes x [..., Kp], scales x_scales [..., Gp],
+    as quantize_fp8, add_rmsnorm_fp8 and silu_mul_fp8 give them) and an 8-bit
+    weight (w = tile_weight_fp8 of its codes, w_scales [N, Gp]) transposed,
+    accumulated in fp32 and rounded once: bf16 [..., N].  With `add` (bf16,
+    [..., N]; it may be `out`) out = x @ w.T + add inside that rounding.  Calls
+    of at most 64 rows give a row the same bits whatever rows come with it."""
+    dev = gpu(w, "w").device
+    if w.dtype != FP8_CODE or w.dim() != 5 or tuple(w.shape[2:]) != (2, 64, 16) or not w.is_contiguous():
+        raise ValueError("w must be a tile_weight_fp8() result")
+    kp = w.shape[1] * FP8_GROUP
+    gp = -(-w.shape[1] // 4) * 4
+    _on(dev, w_scales, "w_scales", FP8_SCALE, True)
+    n = w_scales.shape[0]
+    if w_scales.dim() != 2 or w_scales.shape[1] != gp or -(-n // 16) != w.shape[0]:
+        raise ValueError(f"w_scales must be [N, {gp}] with N in {16 * w.shape[0]} - 15 .. {16 * w.shape[0]} "
+                         f"(got {list(w_scales.shape)})")
+    _on(dev, x, "x", FP8_CODE)
+    _on(dev, x_scales, "x_scales", FP8_SCALE)
+    if x.shape[-1:] != (kp,) or x_scales.shape != (*x.shape[:-1], gp):
+        raise ValueError(f"x must be [..., {kp}] and x_scales [..., {gp}] "
+                         f"(got {list(x.shape)} and {list(x_scales.shape)})")
+    x2 = x if x.dim() == 2 else x.reshape(-1, kp)
+    s2 = x_scales if x_scales.dim() == 2 else x_scales.reshape(-1, gp)
+    rows = x2.shape[0]
+    if x2.stride(1) != 1 or rows > 1 and (x2.stride(0) < kp or x2.stride(0) % 16) or x2.data_ptr() % 16:
+        x2 = x2.clone(memory_format=torch.contiguous_format)
+    if s2.stride(1) != 1 or rows > 1 and (s2.stride(0) < gp or s2.stride(0) % 4) or s2.data_ptr() % 4:
+        s2 = s2.clone(memory_format=torch.contiguous_format)
+
+    def flat(t: torch.Tensor, name: str) -> torch.Tensor:
+        _on(dev, t, name, torch.bfloat16)
+        t2 = t if t.dim() == 2 else t.view(-1, t.shape[-1])
+        if tuple(t2.shape) != (rows, n) or t2.stride(1) != 1 or (rows > 1 and t2.stride(0) < n):
+            raise ValueError(f"{name} must be bf16 [rows, N] = [{rows}, {n}] with unit inner stride and rows apart")
+        return t2
+
+    a2 = None if add is None else flat(add, "add")
+    fresh = out is None
+    o2 = torch.empty(rows, n, dtype=torch.bfloat16, device=dev) if fresh else flat(out, "out")
+    one = rows <= 1  # a single row's strides mean nothing
+    st = _launch(dev, lib().specdec_linear_fp8, x2.data_ptr(), kp if one else x2.stride(0), s2.data_ptr(),
+                 gp if one else s2.stride(0), w.data_ptr(), w_scales.data_ptr(), rows, kp, n, ptr(a2),
+                 n if one or a2 is None else a2.stride(0), o2.data_ptr(), n if one else o2.stride(0))
+    _check(st, "linear_fp8")
+    return o2.view(*x.shape[:-1], n) if fresh else out
+
+
 def head_logits(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
     """x [..., H] bf16 times the head w [V, H] bf16, accumulated in fp32:
     fp32 logits [..., V].  A row's logits do not depend on the other rows
