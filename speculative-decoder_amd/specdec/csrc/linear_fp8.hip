@@ -113,14 +113,20 @@ template <int RT> __global__ __launch_bounds__(kLin8MaxWaves * 64) void linear_f
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
 
-// LDS bytes of the tile kernel: the ring of operand pieces, later the waves'
-// output rows (32 of each, padded by 16 bytes so that neither the 8-byte
-// writes down a column of rows nor the 16-byte reads along a row meet in a bank)
-template <int WR, int WF> constexpr int tile8_piece() { return 4 * (WR + WF) * 1024; }
-template <int WR, int WF, int RING> constexpr int tile8_lds() {
-  const int ring = RING * tile8_piece<WR, WF>(), outs = 4 * 32 * (64 * WF + 16);
-  return ring > outs ? ring : outs;
-}
+// LDS of the tile kernel, for 64 WR rows and 64 WF features: three slots of 64
+// inputs of the features, three of 128 inputs of the rows, two of 16 groups'
+// scales; the waves' output rows (32 of each at a time, padded by 16 bytes so
+// that neither the 8-byte writes down a column of rows nor the 16-byte reads
+// along a row meet in a bank) take the rings' place at the end.
+constexpr int kTileSlots = 3;
+template <int WR, int WF> struct Tile8 {
+  static constexpr int kW = 4 * WF * 1024, kX = 8 * WR * 1024, kScales = (WR + WF) * 1024;
+  static constexpr int kXAt = kTileSlots * kW, kScalesAt = kXAt + kTileSlots * kX;
+  static constexpr int kPitch = 64 * WF + 16;
+  static constexpr int kRings = kScalesAt + 2 * kScales, kOut = 4 * 32 * kPitch;
+  static constexpr int kLds = kRings > kOut ? kRings : kOut;
+  static_assert((WR + WF) % 4 == 0, "a thread loads whole rows of scales");
+};
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t from_corner(const uint8_t *base) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base), 0, 0x7FFFFFFF, 0x00020000);
@@ -132,8 +138,8 @@ __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t from, uint8_t
   __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void *)dst, 16, lane_off, off, 0, 0);
 }
 
-// At most N of this wave's loads still on their way and none of its LDS reads,
-// and every wave of the workgroup here; no memory access moves across.
+// At most N of this wave's loads still on their way and none of its LDS
+// accesses, and every wave of the workgroup here; no memory access moves across.
 template <int N> __device__ __forceinline__ void wait_meet() {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x70);
@@ -142,30 +148,27 @@ template <int N> __device__ __forceinline__ void wait_meet() {
 }
 
 // Four waves, two by two, of 32 WR rows x 32 WF features each, on
-// v_mfma_scale_f32_32x32x64_f8f6f4.  Operands pass through LDS in pieces of 64
-// inputs, loaded straight from memory into a ring of RING pieces: blocks of
-// 16 rows (or features) x 64 inputs, 1 KB in the order [16 bytes of inputs]
-// [row], which is how the weight is stored and what a wave's 16-byte LDS reads
-// take without a bank met twice.  While a piece is multiplied from registers,
-// the next one's operands are read from LDS and the piece RING ahead is asked
-// for, so one barrier a piece is the only wait.
-template <int WR, int WF, int RING>
+// v_mfma_scale_f32_32x32x64_f8f6f4.  Operands go from memory straight to LDS,
+// in instructions of 1 KB that touch eight whole cache lines (what bounds them
+// is the lines they look up, so rows come 128 inputs at a time): features in
+// the order in which they are stored, rows with the 16-byte chunk c of row r at
+// place c ^ (r / 2 % 8) of its 128 bytes, so that the 16-byte LDS reads of
+// either meet in no bank.  A turn multiplies 64 inputs from registers while the
+// next turn's are read from LDS and later ones asked for, so one barrier a turn
+// is the only wait.
+template <int WR, int WF, bool ADD>
 __global__ __launch_bounds__(256, 1) void linear_fp8_tile_kernel(Lin8Args a, int tiles_m, int tiles_n) {
   extern __shared__ __align__(1024) uint8_t s_ring[];
-  constexpr int kPiece = tile8_piece<WR, WF>();
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  using L = Tile8<WR, WF>;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, kh = lane >> 5;
   // the tile: 8 XCDs take turns in the launch order, so each gets a contiguous
   // run of tiles; a run walks eight row tiles of one feature tile, then the next
-  const int total = tiles_m * tiles_n;
-  int t = blockIdx.x;
-  {
-    const int per = total / 8, rest = total % 8, x = t % 8, i = t / 8;
-    t = x * per + min(x, rest) + i;
-  }
   int tm, tn;
   {
     constexpr int kBand = 8;
+    const int total = tiles_m * tiles_n, x = blockIdx.x % 8;
+    const int t = x * (total / 8) + min(x, total % 8) + (int)blockIdx.x / 8;
     const int band = t / (kBand * tiles_n), in = t % (kBand * tiles_n);
     const int rows = min(kBand, tiles_m - band * kBand);
     tm = band * kBand + in % rows;
@@ -174,46 +177,74 @@ __global__ __launch_bounds__(256, 1) void linear_fp8_tile_kernel(Lin8Args a, int
   const int64_t m0 = (int64_t)tm * (64 * WR);
   const int n0 = tn * (64 * WF);
   const int wm = wave >> 1, wn = wave & 1;
+  const int m_last = (int)min(a.M - 1 - m0, (int64_t)64 * WR), n_last = a.N - 1 - n0;
   const int pieces = a.steps * 2;
 
-  // this lane's share of a piece: WF blocks of features, WR blocks of rows,
-  // addressed by 32-bit offsets from the tile's corner (features and rows past
-  // the ends read the last ones; they are never stored)
-  const int ftiles = (a.N + 15) / 16;
+  // this wave's share: WF 1 KB blocks of 16 features x 64 inputs a turn, 2 WR
+  // blocks of 8 rows x 128 inputs every two turns, by 32-bit offsets from the
+  // tile's corner (features and rows past the ends read the last ones; they are
+  // never stored)
   const int tile_bytes = a.steps * 2048;
   const __amdgpu_buffer_rsrc_t wb = from_corner(a.w + (int64_t)(n0 / 16) * tile_bytes);
   const __amdgpu_buffer_rsrc_t xb = from_corner(a.x + m0 * a.x_stride);
-  int woff[WF], xoff[WR];  // woff: the same in all lanes
+  int woff[WF], xoff[2 * WR];  // woff: the same in all lanes
 #pragma unroll
-  for (int i = 0; i < WF; ++i) woff[i] = min(wave + 4 * i, ftiles - 1 - n0 / 16) * tile_bytes;
+  for (int i = 0; i < WF; ++i) woff[i] = min(wave + 4 * i, n_last / 16) * tile_bytes;
 #pragma unroll
-  for (int i = 0; i < WR; ++i)
-    xoff[i] = (int)(min((int64_t)(16 * (wave + 4 * i) + (lane & 15)), a.M - 1 - m0) * a.x_stride) + (lane >> 4) * 16;
-  // piece p (past the end: the last one again, never multiplied) to a slot
-  auto fetch = [&](int slot, int piece) {
-    const int p = min(piece, pieces - 1);
-    uint8_t *dst = s_ring + slot * kPiece;
+  for (int i = 0; i < 2 * WR; ++i) {
+    const int row = 8 * (wave + 4 * i) + (lane >> 3);
+    xoff[i] = min(row, m_last) * (int)a.x_stride + ((lane & 7) ^ ((row >> 1) & 7)) * 16;
+  }
+  // inputs past the end: the last ones again, never multiplied
+  auto fetch_w = [&](int slot, int piece) {
+    const int off = min(piece, pieces - 1) * 1024;
 #pragma unroll
-    for (int i = 0; i < WF; ++i) load_to_lds(wb, dst + (wave + 4 * i) * 1024, lane * 16, woff[i] + p * 1024);
-#pragma unroll
-    for (int i = 0; i < WR; ++i) load_to_lds(xb, dst + (4 * WF + wave + 4 * i) * 1024, xoff[i], p * 64);
+    for (int i = 0; i < WF; ++i)
+      load_to_lds(wb, s_ring + slot * L::kW + (wave + 4 * i) * 1024, lane * 16, woff[i] + off);
   };
-  // scales: four groups a word
-  const int ws_stride = (a.steps + 3) / 4 * 4;
-  const __amdgpu_buffer_rsrc_t wsb = from_corner(a.ws + (int64_t)n0 * ws_stride);
-  const __amdgpu_buffer_rsrc_t xsb = from_corner(a.xs + m0 * a.xs_stride);
-  int wsoff[WF], xsoff[WR];
+  auto fetch_x = [&](int slot, int step, auto part) {  // half of this wave's rows
+    const int off = min(step, a.steps - 1) * 128;
 #pragma unroll
-  for (int i = 0; i < WF; ++i) wsoff[i] = min((wn * WF + i) * 32 + r, a.N - 1 - n0) * ws_stride;
+    for (int i = decltype(part)::value * WR; i < (decltype(part)::value + 1) * WR; ++i)
+      load_to_lds(xb, s_ring + L::kXAt + slot * L::kX + (wave + 4 * i) * 1024, xoff[i], off);
+  };
+  // scales: 16 groups of 64 WF features, then of 64 WR rows, 16 bytes each
+  constexpr int kScaleRows = (WR + WF) / 4;  // a thread's
+  const int words = (a.steps + 3) / 4;
+  const unsigned *sp[kScaleRows];
 #pragma unroll
-  for (int i = 0; i < WR; ++i)
-    xsoff[i] = (int)(min((int64_t)((wm * WR + i) * 32 + r), a.M - 1 - m0) * a.xs_stride);
+  for (int i = 0; i < kScaleRows; ++i) {
+    const int row = tid + 256 * i;
+    sp[i] = reinterpret_cast<const unsigned *>(
+        row < 64 * WF ? a.ws + (int64_t)(n0 + min(row, n_last)) * (4 * words)
+                      : a.xs + (m0 + min(row - 64 * WF, m_last)) * a.xs_stride);
+  }
+  u32x4 sv[kScaleRows];
+  auto load_scales = [&](int chunk) {
+#pragma unroll
+    for (int i = 0; i < kScaleRows; ++i) {
+      if (4 * chunk + 4 <= words) {
+        __builtin_memcpy(&sv[i], sp[i] + 4 * chunk, 16);
+      } else {  // the row's last words
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sv[i][k] = sp[i][min(4 * chunk + k, words - 1)];
+      }
+    }
+  };
+  auto store_scales = [&](int chunk) {
+#pragma unroll
+    for (int i = 0; i < kScaleRows; ++i)
+      *reinterpret_cast<u32x4 *>(s_ring + L::kScalesAt + (chunk & 1) * L::kScales + (tid + 256 * i) * 16) = sv[i];
+  };
   unsigned sw[WF], sx[WR], sw_next[WF], sx_next[WR];
-  auto load_scales = [&](int q) {
+  auto read_scales = [&](int q) {  // the word of groups 4 q .. 4 q + 3
+    const uint8_t *src = s_ring + L::kScalesAt + (q >> 2 & 1) * L::kScales + (q & 3) * 4;
 #pragma unroll
-    for (int i = 0; i < WF; ++i) sw_next[i] = __builtin_amdgcn_raw_buffer_load_b32(wsb, wsoff[i], 4 * q, 0);
+    for (int i = 0; i < WF; ++i)
+      sw_next[i] = *reinterpret_cast<const unsigned *>(src + ((wn * WF + i) * 32 + r) * 16);
 #pragma unroll
-    for (int i = 0; i < WR; ++i) sx_next[i] = __builtin_amdgcn_raw_buffer_load_b32(xsb, xsoff[i], 4 * q, 0);
+    for (int i = 0; i < WR; ++i)
+      sx_next[i] = *reinterpret_cast<const unsigned *>(src + (64 * WF + (wm * WR + i) * 32 + r) * 16);
   };
 
   f32x16 acc[WR][WF];
@@ -225,71 +256,111 @@ __global__ __launch_bounds__(256, 1) void linear_fp8_tile_kernel(Lin8Args a, int
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
 
   i32x8 fw[2][WF], fx[2][WR];
-  const int at = (r >> 4) * 1024 + kh * 512 + (r & 15) * 16;
-  auto read = [&](int slot, int b) {
-    const uint8_t *src = s_ring + slot * kPiece + at;
+  const int w_at = (r >> 4) * 1024 + kh * 512 + (r & 15) * 16 + wn * WF * 2048;
+  const int x_at = L::kXAt + (wm * WR * 32 + r) * 128;
+  const int x_swz = (r >> 1) & 7;
+  auto read = [&](int w_slot, int x_slot, auto half) {
+    constexpr int H = decltype(half)::value;
+    const uint8_t *src = s_ring + w_slot * L::kW + w_at;
 #pragma unroll
     for (int i = 0; i < WF; ++i) {
-      const u32x4 *v = reinterpret_cast<const u32x4 *>(src + (wn * WF + i) * 2048);
-      fw[b][i] = join8(v[0], v[16]);
+      const u32x4 *v = reinterpret_cast<const u32x4 *>(src + i * 2048);
+      fw[H][i] = join8(v[0], v[16]);
     }
+    const uint8_t *xsrc = s_ring + x_slot * L::kX + x_at;
+    const uint8_t *c0 = xsrc + ((4 * H + 2 * kh) ^ x_swz) * 16, *c1 = xsrc + ((4 * H + 2 * kh + 1) ^ x_swz) * 16;
 #pragma unroll
-    for (int i = 0; i < WR; ++i) {
-      const u32x4 *v = reinterpret_cast<const u32x4 *>(src + 4 * WF * 1024 + (wm * WR + i) * 2048);
-      fx[b][i] = join8(v[0], v[16]);
-    }
+    for (int i = 0; i < WR; ++i)
+      fx[H][i] = join8(*reinterpret_cast<const u32x4 *>(c0 + i * 4096), *reinterpret_cast<const u32x4 *>(c1 + i * 4096));
   };
-  constexpr int kLoads = WR + WF;  // a wave's loads of a piece
-  // Piece q is in registers (half B of the group whose scales are byte K of
-  // the words).  The wait and barrier: this wave's loads of piece q + 1 have
-  // landed and its reads of piece q are done; behind the barrier every wave's
-  // are.  So q + 1 may be read, and q's slot loaded again.
+  auto after = [](int slot) { return slot == kTileSlots - 1 ? 0 : slot + 1; };
+  int ws = 0, xs = 0;  // slots of the current turn's features and step's rows
+  // Turn q multiplies the half H of step q / 2, whose scales are byte K of the
+  // words, from registers.  The wait and barrier before it: this wave's loads
+  // for turn q + 1 have landed and its reads for turn q are done, and behind
+  // the barrier every wave's are.  So turn q + 1's operands may be read, and
+  // the features' slot of turn q and, once both halves of a step are read, its
+  // rows' slot loaded again: half the rows in this turn, half in the next.
   auto turn = [&](int q, auto k, auto half) {
-    constexpr int K = decltype(k)::value, B = decltype(half)::value;
-    wait_meet<kLoads *(RING - 2)>();
-    fetch(q & (RING - 1), q + RING);
-    read((q + 1) & (RING - 1), 1 - B);
+    constexpr int K = decltype(k)::value, H = decltype(half)::value;
+    wait_meet<WR + WF>();
+    read(after(ws), H == 1 ? after(xs) : xs, std::integral_constant<int, 1 - H>());
+    if constexpr (H == 1)
+      fetch_x(xs, (q >> 1) + kTileSlots, std::integral_constant<int, 0>());
+    else
+      fetch_x(xs == 0 ? kTileSlots - 1 : xs - 1, (q >> 1) - 1 + kTileSlots, std::integral_constant<int, 1>());
+    fetch_w(ws, q + kTileSlots);
 #pragma unroll
     for (int i = 0; i < WR; ++i)
 #pragma unroll
       for (int j = 0; j < WF; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fw[B][j], fx[B][i], acc[i][j], 0, 0, K, (int)sw[j],
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fw[H][j], fx[H][i], acc[i][j], 0, 0, K, (int)sw[j],
                                                                     K, (int)sx[i]);
-    // the memory path's instructions between the products, not before them
+    // between the products: the LDS reads in the first half, then the loads
+    constexpr int kHalf = WR * WF / 2, kEach = WR + WF;
 #pragma unroll
-    for (int i = 0; i < WR * WF; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a product
-      __builtin_amdgcn_sched_group_barrier(0x100, (2 * kLoads + WR * WF - 1) / (WR * WF), 0);  // LDS reads
-      __builtin_amdgcn_sched_group_barrier(0x010, (kLoads + WR * WF - 1) / (WR * WF), 0);      // loads
+    for (int i = 0; i < kHalf; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                            // a product
+      __builtin_amdgcn_sched_group_barrier(0x100, (2 * kEach + kHalf - 1) / kHalf, 0);  // LDS reads
+    }
+#pragma unroll
+    for (int i = 0; i < kHalf; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x010, (kEach + kHalf - 1) / kHalf, 0);  // loads
     }
     __builtin_amdgcn_sched_barrier(0);
+    ws = after(ws);
+    if constexpr (H == 1) xs = after(xs);
   };
-  auto group = [&](int s, auto k) {
+  auto step = [&](int s, auto k) {
     turn(2 * s, k, std::integral_constant<int, 0>());
     turn(2 * s + 1, k, std::integral_constant<int, 1>());
   };
   load_scales(0);
 #pragma unroll
-  for (int p = 0; p < RING; ++p) fetch(p, p);
-  wait_meet<kLoads *(RING - 1)>();
-  read(0, 0);
-  for (int s = 0; s < a.steps; s += 4) {
+  for (int i = 0; i < kTileSlots; ++i) {
+    fetch_x(i, i, std::integral_constant<int, 0>());
+    // the second half of the third step's rows is asked for in turn 0
+    if (i + 1 < kTileSlots) fetch_x(i, i, std::integral_constant<int, 1>());
+    fetch_w(i, i);
+  }
+  store_scales(0);
+  wait_meet<0>();
+  read(0, 0, std::integral_constant<int, 0>());
+  read_scales(0);
+  auto next_scales = [&]() {
 #pragma unroll
     for (int i = 0; i < WF; ++i) sw[i] = sw_next[i];
 #pragma unroll
     for (int i = 0; i < WR; ++i) sx[i] = sx_next[i];
-    load_scales(min(s / 4 + 1, (a.steps - 1) / 4));
-    group(s, std::integral_constant<int, 0>());
-    if (s + 1 < a.steps) group(s + 1, std::integral_constant<int, 1>());
-    if (s + 2 < a.steps) group(s + 2, std::integral_constant<int, 2>());
-    if (s + 3 < a.steps) group(s + 3, std::integral_constant<int, 3>());
+  };
+  const int fours = a.steps / 4;
+  for (int q = 0; q < fours; ++q) {
+    next_scales();
+    // the next 16 groups' scales: asked for at the start of these, stored in
+    // the last word's turns, where two barriers follow before they are read
+    if ((q & 3) == 0 && 4 * (q + 4) < a.steps) load_scales((q >> 2) + 1);
+    step(4 * q, std::integral_constant<int, 0>());
+    step(4 * q + 1, std::integral_constant<int, 1>());
+    if ((q & 3) == 3) store_scales((q >> 2) + 1);
+    step(4 * q + 2, std::integral_constant<int, 2>());
+    read_scales(q + 1);
+    step(4 * q + 3, std::integral_constant<int, 3>());
   }
-  // every load has landed and every wave is through with the ring
+  if (4 * fours < a.steps) {
+    next_scales();
+    step(4 * fours, std::integral_constant<int, 0>());
+    if (4 * fours + 1 < a.steps) step(4 * fours + 1, std::integral_constant<int, 1>());
+    if (4 * fours + 2 < a.steps) step(4 * fours + 2, std::integral_constant<int, 2>());
+  }
+  // every load has landed and every wave is through with the rings
   wait_meet<0>();
   // 32 rows at a time: this lane's features of its row to LDS, whole rows back
-  constexpr int kPitch = 64 * WF + 16;
-  uint8_t *mine = s_ring + wave * 32 * kPitch;
+  uint8_t *mine = s_ring + wave * 32 * L::kPitch;
   const int fbase = n0 + wn * WF * 32;
+  constexpr int kLanes = 4 * WF;  // lanes of a row
+  const int rr0 = lane / kLanes, f0 = (lane % kLanes) * 8;
+  const bool whole = m_last >= 64 * WR - 1 && n_last >= 64 * WF - 1;  // nothing of the tile past the ends
 #pragma unroll
   for (int i = 0; i < WR; ++i) {
     const int64_t row0 = m0 + (wm * WR + i) * 32;
@@ -301,50 +372,57 @@ __global__ __launch_bounds__(256, 1) void linear_fp8_tile_kernel(Lin8Args a, int
         float v[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] = acc[i][j][4 * e + k];
-        if (a.add) {
-          const int64_t row = min(row0 + r, a.M - 1);
+        if constexpr (ADD) {
+          const uint16_t *src = a.add + min(row0 + r, a.M - 1) * a.add_stride;
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            v[k] += __uint_as_float((unsigned)a.add[row * a.add_stride + min(fbase + f + k, a.N - 1)] << 16);
+          for (int k = 0; k < 4; ++k) v[k] += __uint_as_float((unsigned)src[min(fbase + f + k, a.N - 1)] << 16);
         }
         const bf16x2 lo{(__bf16)v[0], (__bf16)v[1]}, hi{(__bf16)v[2], (__bf16)v[3]};
-        *reinterpret_cast<u32x2 *>(mine + r * kPitch + f * 2) =
+        *reinterpret_cast<u32x2 *>(mine + r * L::kPitch + f * 2) =
             u32x2{__builtin_bit_cast(unsigned, lo), __builtin_bit_cast(unsigned, hi)};
       }
     __builtin_amdgcn_sched_barrier(0);
-    constexpr int kLanes = 4 * WF;  // lanes of a row
+    uint16_t *dst = a.out + (row0 + rr0) * a.out_stride + fbase + f0;
 #pragma unroll
-    for (int v = 0; v < 32 * kLanes / 64; ++v) {
-      const int rr = v * (64 / kLanes) + lane / kLanes, f = (lane % kLanes) * 8;
-      const u32x4 o = *reinterpret_cast<const u32x4 *>(mine + rr * kPitch + f * 2);
-      if (row0 + rr >= a.M) continue;
-      uint16_t *dst = a.out + (row0 + rr) * a.out_stride + fbase + f;
-      if (fbase + f + 8 <= a.N) {
+    for (int v = 0; v < kLanes / 2; ++v) {
+      const int rr = v * (64 / kLanes) + rr0;
+      const u32x4 o = *reinterpret_cast<const u32x4 *>(mine + rr * L::kPitch + f0 * 2);
+      if (whole || (row0 + rr < a.M && fbase + f0 + 8 <= a.N)) {
         __builtin_memcpy(dst, &o, 16);
-      } else {
+      } else if (row0 + rr < a.M) {
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          if (fbase + f + k < a.N) dst[k] = (uint16_t)(o[k >> 1] >> (16 * (k & 1)));
+          if (fbase + f0 + k < a.N) dst[k] = (uint16_t)(o[k >> 1] >> (16 * (k & 1)));
       }
+      dst += (64 / kLanes) * a.out_stride;
     }
     __builtin_amdgcn_sched_barrier(0);
   }
 }
 
-template <int WR, int WF, int RING> int launch_tile8(const Lin8Args &a, hipStream_t s) {
-  constexpr int lds = tile8_lds<WR, WF, RING>();
+// The tile kernel addresses a tile's operands by 32-bit offsets.
+template <int WR, int WF> bool tile8_fits(const Lin8Args &a) {
+  return a.x_stride <= 0x7FFFFFFF / (64 * WR + 1) && (int64_t)a.steps * 2048 <= 0x7FFFFFFF / (4 * WF + 1);
+}
+
+template <int WR, int WF, bool ADD> int launch_tile8_as(const Lin8Args &a, hipStream_t s) {
+  constexpr int lds = Tile8<WR, WF>::kLds;
   static bool ready[64];
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return SPECDEC_EHIP;
   if (!ready[dev]) {
-    if (hipFuncSetAttribute((const void *)linear_fp8_tile_kernel<WR, WF, RING>,
+    if (hipFuncSetAttribute((const void *)linear_fp8_tile_kernel<WR, WF, ADD>,
                             hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
       return SPECDEC_EHIP;
     ready[dev] = true;
   }
   const int tm = (int)((a.M + 64 * WR - 1) / (64 * WR)), tn = (a.N + 64 * WF - 1) / (64 * WF);
-  linear_fp8_tile_kernel<WR, WF, RING><<<tm * tn, 256, lds, s>>>(a, tm, tn);
+  linear_fp8_tile_kernel<WR, WF, ADD><<<tm * tn, 256, lds, s>>>(a, tm, tn);
   return launch_status();
+}
+
+template <int WR, int WF> int launch_tile8(const Lin8Args &a, hipStream_t s) {
+  return a.add ? launch_tile8_as<WR, WF, true>(a, s) : launch_tile8_as<WR, WF, false>(a, s);
 }
 
 }  // namespace specdec
@@ -374,8 +452,8 @@ SPECDEC_API int specdec_linear_fp8(const void *x, int64_t x_stride, const void *
   a.per_wave = (a.steps + waves - 1) / waves;
   const unsigned tiles = (unsigned)((out_features + 15) / 16);
   hipStream_t s = as_stream(stream);
-  if (rows > 512) return launch_tile8<4, 4, 4>(a, s);
-  if (rows > 64) return launch_tile8<2, 2, 4>(a, s);
+  if (rows > 512 && tile8_fits<4, 4>(a)) return launch_tile8<4, 4>(a, s);
+  if (rows > 64 && tile8_fits<2, 2>(a)) return launch_tile8<2, 2>(a, s);
   if (rows <= 16)
     linear_fp8_kernel<1><<<dim3(tiles, 1), waves * 64, 0, s>>>(a);
   else
