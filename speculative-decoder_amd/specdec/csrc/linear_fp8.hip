@@ -110,22 +110,24 @@ template <int RT> __global__ __launch_bounds__(kLin8MaxWaves * 64) void linear_f
 }
 
 // ---------------------------------------------------------------- many rows --
-typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
 
-// LDS of the tile kernel, for 64 WR rows and 64 WF features: three slots of 64
-// inputs of the features, three of 128 inputs of the rows, two of 16 groups'
-// scales; the waves' output rows (32 of each at a time, padded by 16 bytes so
-// that neither the 8-byte writes down a column of rows nor the 16-byte reads
-// along a row meet in a bank) take the rings' place at the end.
+// The tile kernel's shape: WM x WN waves of 16 TR rows x 16 TF features, and
+// its LDS: three slots of half of the features x 128 inputs, three of the rows
+// x 128 inputs, two of 16 groups' scales; the waves' output rows (padded by 16
+// bytes so that neither the 8-byte writes down a column of rows nor the 16-byte
+// reads along a row meet in a bank) take their place at the end.
 constexpr int kTileSlots = 3;
-template <int WR, int WF> struct Tile8 {
-  static constexpr int kW = 4 * WF * 1024, kX = 8 * WR * 1024, kScales = (WR + WF) * 1024;
+template <int TR, int TF, int WM, int WN> struct Tile8 {
+  static_assert(WM * WN == 4 && TF % TR == 0 && TF >= 4 && TR % 2 == 0, "");
+  static constexpr int kRows = 16 * TR * WM, kFeatures = 16 * TF * WN;
+  static constexpr int kW = kFeatures * 64, kX = kRows * 128, kScales = (kRows + kFeatures) * 16;
   static constexpr int kXAt = kTileSlots * kW, kScalesAt = kXAt + kTileSlots * kX;
-  static constexpr int kPitch = 64 * WF + 16;
-  static constexpr int kRings = kScalesAt + 2 * kScales, kOut = 4 * 32 * kPitch;
+  static constexpr int kPitch = 32 * TF + 16;
+  static constexpr int kRings = kScalesAt + 2 * kScales, kOut = 4 * 16 * TR * kPitch;
   static constexpr int kLds = kRings > kOut ? kRings : kOut;
-  static_assert((WR + WF) % 4 == 0, "a thread loads whole rows of scales");
+  static constexpr int kLoadsW = kW / 4096, kLoadsX = kX / 8192;  // a wave's loads of a turn
+  static_assert(kLds <= 160 * 1024, "");
 };
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t from_corner(const uint8_t *base) {
@@ -147,21 +149,53 @@ template <int N> __device__ __forceinline__ void wait_meet() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// Four waves, two by two, of 32 WR rows x 32 WF features each, on
-// v_mfma_scale_f32_32x32x64_f8f6f4.  Operands go from memory straight to LDS,
-// in instructions of 1 KB that touch eight whole cache lines (what bounds them
-// is the lines they look up, so rows come 128 inputs at a time): features in
-// the order in which they are stored, rows with the 16-byte chunk c of row r at
-// place c ^ (r / 2 % 8) of its 128 bytes, so that the 16-byte LDS reads of
-// either meet in no bank.  A turn multiplies 64 inputs from registers while the
-// next turn's are read from LDS and later ones asked for, so one barrier a turn
-// is the only wait.
-template <int WR, int WF, bool ADD>
+// acc += w x, the operands scaled by byte K of sw and sx.  In assembly so that
+// the sum stays in its registers: given the choice the compiler moves sums from
+// one set to another, and a tile's take half of the register file.  Nothing in
+// a turn reads a sum, so none of the hazards that the compiler would have to
+// pad arises before settle().
+template <int K>
+__device__ __forceinline__ void product(f32x4 &acc, const i32x8 &w, const i32x8 &x, unsigned sw, unsigned sx) {
+  if constexpr (K == 0)
+    asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0]"
+                 : "+a"(acc) : "v"(w), "v"(x), "v"(sw), "v"(sx));
+  else if constexpr (K == 1)
+    asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[1,1,0] op_sel_hi:[0,0,0]"
+                 : "+a"(acc) : "v"(w), "v"(x), "v"(sw), "v"(sx));
+  else if constexpr (K == 2)
+    asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[1,1,0]"
+                 : "+a"(acc) : "v"(w), "v"(x), "v"(sw), "v"(sx));
+  else
+    asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[1,1,0] op_sel_hi:[1,1,0]"
+                 : "+a"(acc) : "v"(w), "v"(x), "v"(sw), "v"(sx));
+}
+// Between writes to sums or operands by other instructions and the first
+// product, and between the last product and what reads a sum: the products that
+// are still in the unit end first (at most 18 cycles' wait is asked for).
+template <int TF> __device__ __forceinline__ void settle(f32x4 (&acc)[TF]) {
+#pragma unroll
+  for (int j = 0; j < TF; j += 4)
+    asm volatile("s_nop 15\n\ts_nop 15" : "+a"(acc[j]), "+a"(acc[j + 1]), "+a"(acc[j + 2]), "+a"(acc[j + 3]));
+}
+
+// A tile of kRows x kFeatures a workgroup, on v_mfma_scale_f32_16x16x128_f8f6f4
+// (at this size the card's power bounds the matrix unit, and of its two shapes
+// this one does more per watt: with random operands in registers 3765 TFLOP/s,
+// 32x32x64 3113).  Operands go from memory straight to LDS, in instructions of
+// 1 KB that touch eight whole cache lines (the memory path looks up a line at a
+// time): features in the order in which they are stored, rows with the 16-byte
+// chunk c of row r at place c ^ (r / 2 % 8) of its 128 bytes, so that the
+// 16-byte LDS reads of either meet in no bank.  A turn multiplies 128 inputs of
+// half of a wave's features with all its rows; its operands are in registers
+// when it starts, the next turn's are read from LDS and later ones asked for
+// between its products, so one barrier a turn is the only wait.
+template <int TR, int TF, int WM, int WN, bool ADD>
 __global__ __launch_bounds__(256, 1) void linear_fp8_tile_kernel(Lin8Args a, int tiles_m, int tiles_n) {
   extern __shared__ __align__(1024) uint8_t s_ring[];
-  using L = Tile8<WR, WF>;
+  using L = Tile8<TR, TF, WM, WN>;
+  constexpr int kHalf = TF / 2;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int r = lane & 31, kh = lane >> 5;
+  const int c = lane & 15, g = lane >> 4;
   // the tile: 8 XCDs take turns in the launch order, so each gets a contiguous
   // run of tiles; a run walks eight row tiles of one feature tile, then the next
   int tm, tn;
@@ -174,50 +208,47 @@ __global__ __launch_bounds__(256, 1) void linear_fp8_tile_kernel(Lin8Args a, int
     tm = band * kBand + in % rows;
     tn = in / rows;
   }
-  const int64_t m0 = (int64_t)tm * (64 * WR);
-  const int n0 = tn * (64 * WF);
-  const int wm = wave >> 1, wn = wave & 1;
-  const int m_last = (int)min(a.M - 1 - m0, (int64_t)64 * WR), n_last = a.N - 1 - n0;
-  const int pieces = a.steps * 2;
+  const int64_t m0 = (int64_t)tm * L::kRows;
+  const int n0 = tn * L::kFeatures;
+  const int wm = wave / WN, wn = wave % WN;
+  const int m_last = (int)min(a.M - 1 - m0, (int64_t)L::kRows), n_last = a.N - 1 - n0;
 
-  // this wave's share: WF 1 KB blocks of 16 features x 64 inputs a turn, 2 WR
-  // blocks of 8 rows x 128 inputs every two turns, by 32-bit offsets from the
-  // tile's corner (features and rows past the ends read the last ones; they are
-  // never stored)
+  // this wave's share of the loads, by 32-bit offsets from the tile's corner
+  // (features and rows past the ends read the last ones; they are never stored).
+  // Block b of a turn's features is half b % 2 of the b / 2-th of their 16s.
   const int tile_bytes = a.steps * 2048;
   const __amdgpu_buffer_rsrc_t wb = from_corner(a.w + (int64_t)(n0 / 16) * tile_bytes);
   const __amdgpu_buffer_rsrc_t xb = from_corner(a.x + m0 * a.x_stride);
-  int woff[WF], xoff[2 * WR];  // woff: the same in all lanes
+  int woff[2][L::kLoadsW], xoff[2 * L::kLoadsX];  // woff: the same in all lanes
 #pragma unroll
-  for (int i = 0; i < WF; ++i) woff[i] = min(wave + 4 * i, n_last / 16) * tile_bytes;
+  for (int i = 0; i < L::kLoadsW; ++i) {
+    const int b = wave + 4 * i, t = b >> 1;
 #pragma unroll
-  for (int i = 0; i < 2 * WR; ++i) {
+    for (int h = 0; h < 2; ++h)
+      woff[h][i] = min(t / kHalf * TF + h * kHalf + t % kHalf, n_last / 16) * tile_bytes + (b & 1) * 1024;
+  }
+#pragma unroll
+  for (int i = 0; i < 2 * L::kLoadsX; ++i) {
     const int row = 8 * (wave + 4 * i) + (lane >> 3);
     xoff[i] = min(row, m_last) * (int)a.x_stride + ((lane & 7) ^ ((row >> 1) & 7)) * 16;
   }
-  // inputs past the end: the last ones again, never multiplied
-  auto fetch_w = [&](int slot, int piece) {
-    const int off = min(piece, pieces - 1) * 1024;
-#pragma unroll
-    for (int i = 0; i < WF; ++i)
-      load_to_lds(wb, s_ring + slot * L::kW + (wave + 4 * i) * 1024, lane * 16, woff[i] + off);
+  const auto last = [&](int s) { return min(s, a.steps - 1); };  // past the end: never multiplied
+  auto fetch_w = [&](int slot, int s, int h, int i) {
+    load_to_lds(wb, s_ring + slot * L::kW + (wave + 4 * i) * 1024, lane * 16, woff[h][i] + last(s) * 2048);
   };
-  auto fetch_x = [&](int slot, int step, auto part) {  // half of this wave's rows
-    const int off = min(step, a.steps - 1) * 128;
-#pragma unroll
-    for (int i = decltype(part)::value * WR; i < (decltype(part)::value + 1) * WR; ++i)
-      load_to_lds(xb, s_ring + L::kXAt + slot * L::kX + (wave + 4 * i) * 1024, xoff[i], off);
+  auto fetch_x = [&](int slot, int s, int i) {
+    load_to_lds(xb, s_ring + L::kXAt + slot * L::kX + (wave + 4 * i) * 1024, xoff[i], last(s) * 128);
   };
-  // scales: 16 groups of 64 WF features, then of 64 WR rows, 16 bytes each
-  constexpr int kScaleRows = (WR + WF) / 4;  // a thread's
+  // scales: 16 groups of the features, then of the rows, 16 bytes each
+  constexpr int kScaleRows = (L::kRows + L::kFeatures + 255) / 256;  // a thread's
   const int words = (a.steps + 3) / 4;
   const unsigned *sp[kScaleRows];
 #pragma unroll
   for (int i = 0; i < kScaleRows; ++i) {
     const int row = tid + 256 * i;
     sp[i] = reinterpret_cast<const unsigned *>(
-        row < 64 * WF ? a.ws + (int64_t)(n0 + min(row, n_last)) * (4 * words)
-                      : a.xs + (m0 + min(row - 64 * WF, m_last)) * a.xs_stride);
+        row < L::kFeatures ? a.ws + (int64_t)(n0 + min(row, n_last)) * (4 * words)
+                           : a.xs + (m0 + min(row - L::kFeatures, m_last)) * a.xs_stride);
   }
   u32x4 sv[kScaleRows];
   auto load_scales = [&](int chunk) {
@@ -234,106 +265,116 @@ __global__ __launch_bounds__(256, 1) void linear_fp8_tile_kernel(Lin8Args a, int
   auto store_scales = [&](int chunk) {
 #pragma unroll
     for (int i = 0; i < kScaleRows; ++i)
-      *reinterpret_cast<u32x4 *>(s_ring + L::kScalesAt + (chunk & 1) * L::kScales + (tid + 256 * i) * 16) = sv[i];
+      if (tid + 256 * i < L::kRows + L::kFeatures)
+        *reinterpret_cast<u32x4 *>(s_ring + L::kScalesAt + (chunk & 1) * L::kScales + (tid + 256 * i) * 16) = sv[i];
   };
-  unsigned sw[WF], sx[WR], sw_next[WF], sx_next[WR];
+  unsigned sw[TF], sx[TR], sw_next[TF], sx_next[TR];
   auto read_scales = [&](int q) {  // the word of groups 4 q .. 4 q + 3
     const uint8_t *src = s_ring + L::kScalesAt + (q >> 2 & 1) * L::kScales + (q & 3) * 4;
 #pragma unroll
-    for (int i = 0; i < WF; ++i)
-      sw_next[i] = *reinterpret_cast<const unsigned *>(src + ((wn * WF + i) * 32 + r) * 16);
+    for (int i = 0; i < TF; ++i)
+      sw_next[i] = *reinterpret_cast<const unsigned *>(src + ((wn * TF + i) * 16 + c) * 16);
 #pragma unroll
-    for (int i = 0; i < WR; ++i)
-      sx_next[i] = *reinterpret_cast<const unsigned *>(src + (64 * WF + (wm * WR + i) * 32 + r) * 16);
+    for (int i = 0; i < TR; ++i)
+      sx_next[i] = *reinterpret_cast<const unsigned *>(src + (L::kFeatures + (wm * TR + i) * 16 + c) * 16);
   };
-
-  f32x16 acc[WR][WF];
-#pragma unroll
-  for (int i = 0; i < WR; ++i)
-#pragma unroll
-    for (int j = 0; j < WF; ++j)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
-
-  i32x8 fw[2][WF], fx[2][WR];
-  const int w_at = (r >> 4) * 1024 + kh * 512 + (r & 15) * 16 + wn * WF * 2048;
-  const int x_at = L::kXAt + (wm * WR * 32 + r) * 128;
-  const int x_swz = (r >> 1) & 7;
-  auto read = [&](int w_slot, int x_slot, auto half) {
-    constexpr int H = decltype(half)::value;
-    const uint8_t *src = s_ring + w_slot * L::kW + w_at;
-#pragma unroll
-    for (int i = 0; i < WF; ++i) {
-      const u32x4 *v = reinterpret_cast<const u32x4 *>(src + i * 2048);
-      fw[H][i] = join8(v[0], v[16]);
-    }
-    const uint8_t *xsrc = s_ring + x_slot * L::kX + x_at;
-    const uint8_t *c0 = xsrc + ((4 * H + 2 * kh) ^ x_swz) * 16, *c1 = xsrc + ((4 * H + 2 * kh + 1) ^ x_swz) * 16;
-#pragma unroll
-    for (int i = 0; i < WR; ++i)
-      fx[H][i] = join8(*reinterpret_cast<const u32x4 *>(c0 + i * 4096), *reinterpret_cast<const u32x4 *>(c1 + i * 4096));
-  };
-  auto after = [](int slot) { return slot == kTileSlots - 1 ? 0 : slot + 1; };
-  int ws = 0, xs = 0;  // slots of the current turn's features and step's rows
-  // Turn q multiplies the half H of step q / 2, whose scales are byte K of the
-  // words, from registers.  The wait and barrier before it: this wave's loads
-  // for turn q + 1 have landed and its reads for turn q are done, and behind
-  // the barrier every wave's are.  So turn q + 1's operands may be read, and
-  // the features' slot of turn q and, once both halves of a step are read, its
-  // rows' slot loaded again: half the rows in this turn, half in the next.
-  auto turn = [&](int q, auto k, auto half) {
-    constexpr int K = decltype(k)::value, H = decltype(half)::value;
-    wait_meet<WR + WF>();
-    read(after(ws), H == 1 ? after(xs) : xs, std::integral_constant<int, 1 - H>());
-    if constexpr (H == 1)
-      fetch_x(xs, (q >> 1) + kTileSlots, std::integral_constant<int, 0>());
-    else
-      fetch_x(xs == 0 ? kTileSlots - 1 : xs - 1, (q >> 1) - 1 + kTileSlots, std::integral_constant<int, 1>());
-    fetch_w(ws, q + kTileSlots);
-#pragma unroll
-    for (int i = 0; i < WR; ++i)
-#pragma unroll
-      for (int j = 0; j < WF; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fw[H][j], fx[H][i], acc[i][j], 0, 0, K, (int)sw[j],
-                                                                    K, (int)sx[i]);
-    // between the products: the LDS reads in the first half, then the loads
-    constexpr int kHalf = WR * WF / 2, kEach = WR + WF;
-#pragma unroll
-    for (int i = 0; i < kHalf; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                            // a product
-      __builtin_amdgcn_sched_group_barrier(0x100, (2 * kEach + kHalf - 1) / kHalf, 0);  // LDS reads
-    }
-#pragma unroll
-    for (int i = 0; i < kHalf; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x010, (kEach + kHalf - 1) / kHalf, 0);  // loads
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    ws = after(ws);
-    if constexpr (H == 1) xs = after(xs);
-  };
-  auto step = [&](int s, auto k) {
-    turn(2 * s, k, std::integral_constant<int, 0>());
-    turn(2 * s + 1, k, std::integral_constant<int, 1>());
-  };
-  load_scales(0);
-#pragma unroll
-  for (int i = 0; i < kTileSlots; ++i) {
-    fetch_x(i, i, std::integral_constant<int, 0>());
-    // the second half of the third step's rows is asked for in turn 0
-    if (i + 1 < kTileSlots) fetch_x(i, i, std::integral_constant<int, 1>());
-    fetch_w(i, i);
-  }
-  store_scales(0);
-  wait_meet<0>();
-  read(0, 0, std::integral_constant<int, 0>());
-  read_scales(0);
   auto next_scales = [&]() {
 #pragma unroll
-    for (int i = 0; i < WF; ++i) sw[i] = sw_next[i];
+    for (int i = 0; i < TF; ++i) sw[i] = sw_next[i];
 #pragma unroll
-    for (int i = 0; i < WR; ++i) sx[i] = sx_next[i];
+    for (int i = 0; i < TR; ++i) sx[i] = sx_next[i];
   };
+
+  f32x4 acc[TR][TF];
+#pragma unroll
+  for (int i = 0; i < TR; ++i)
+#pragma unroll
+    for (int j = 0; j < TF; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  i32x8 fw[2][kHalf], fx[TR];
+  auto read_w = [&](int slot, int h, int t) {
+    const u32x4 *v = reinterpret_cast<const u32x4 *>(s_ring + slot * L::kW + (wn * kHalf + t) * 2048 + lane * 16);
+    fw[h][t] = join8(v[0], v[64]);
+  };
+  const int x_at = L::kXAt + (wm * TR * 16 + c) * 128, x_c0 = (g ^ (c >> 1)) * 16, x_c1 = ((4 + g) ^ (c >> 1)) * 16;
+  auto read_x = [&](int slot, int i) {
+    const uint8_t *src = s_ring + slot * L::kX + x_at + i * 2048;
+    fx[i] = join8(*reinterpret_cast<const u32x4 *>(src + x_c0), *reinterpret_cast<const u32x4 *>(src + x_c1));
+  };
+  auto after = [](int slot) { return slot == kTileSlots - 1 ? 0 : slot + 1; };
+  auto before = [](int slot) { return slot == 0 ? kTileSlots - 1 : slot - 1; };
+  int ws = 0, xs = 0;  // slots of the current turn's features and step's rows
+  // Turn (s, H): half H of the features in step s, whose scales are byte K of
+  // the words.  The wait and barrier before it: this wave's loads for the reads
+  // below have landed and its earlier reads are done, and behind the barrier
+  // every wave's are.  So the next turn's features may be read and the slot of
+  // this turn's loaded again, for three turns later.  The next step's rows are
+  // read in turn (s, 1), each 16 behind the last product that takes the old
+  // ones, the last 16 in turn (s + 1, 0), whose last products take them; their
+  // slot is loaded again in turns (s + 1, 1) and (s + 2, 0), half in each.
+  auto turn = [&](int s, auto k, auto half) {
+    constexpr int K = decltype(k)::value, H = decltype(half)::value;
+    constexpr int kLoads = L::kLoadsW + L::kLoadsX;
+    wait_meet<kLoads>();
+    const int ws_next = after(ws), xs_next = after(xs);
+#pragma unroll
+    for (int i = 0; i < TR; ++i) {
+#pragma unroll
+      for (int t = 0; t < kHalf; ++t) {
+        product<K>(acc[i][H * kHalf + t], fw[H][t], fx[i], sw[H * kHalf + t], sx[i]);
+        if (H == 0 && i == 0 && t == 0) read_x(xs, TR - 1);
+        if (i < TR / 2 && t == (kHalf > 2 ? 1 : 0)) {
+#pragma unroll
+          for (int n = i * (TF / TR); n < (i + 1) * (TF / TR); ++n) read_w(ws_next, 1 - H, n);
+        }
+        if (t == kHalf - 2) {  // this turn's loads, spread over its products
+#pragma unroll
+          for (int l = i * kLoads / TR; l < (i + 1) * kLoads / TR; ++l) {
+            if (l < L::kLoadsX) {
+              if (H == 1)
+                fetch_x(xs, s + kTileSlots, l);
+              else
+                fetch_x(before(xs), s - 1 + kTileSlots, L::kLoadsX + l);
+            } else {
+              fetch_w(ws, s + 1 + (H == 1), 1 - H, l - L::kLoadsX);
+            }
+          }
+        }
+        if (H == 1 && i < TR - 1 && t == kHalf - 1) read_x(xs_next, i);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    ws = ws_next;
+    if constexpr (H == 1) xs = xs_next;
+  };
+  auto step = [&](int s, auto k) {
+    turn(s, k, std::integral_constant<int, 0>());
+    turn(s, k, std::integral_constant<int, 1>());
+  };
+  // The first loads, in the order in which the turns need them: turns (0, 0) and
+  // (0, 1) find all but the last kLoadsW + kLoadsX of them landed, and the
+  // second half of step 2's rows is asked for in turn (0, 0).
+  load_scales(0);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int i = 0; i < 2 * L::kLoadsX; ++i) fetch_x(0, 0, i);
+#pragma unroll
+  for (int q = 0; q < 2; ++q)
+#pragma unroll
+    for (int i = 0; i < L::kLoadsW; ++i) fetch_w(q, 0, q, i);
+#pragma unroll
+  for (int i = 0; i < 2 * L::kLoadsX; ++i) fetch_x(1, 1, i);
+#pragma unroll
+  for (int i = 0; i < L::kLoadsW; ++i) fetch_w(2, 1, 0, i);
+#pragma unroll
+  for (int i = 0; i < L::kLoadsX; ++i) fetch_x(2, 2, i);
+  store_scales(0);
+  wait_meet<2 * L::kLoadsW + 3 * L::kLoadsX>();
+#pragma unroll
+  for (int t = 0; t < kHalf; ++t) read_w(0, 0, t);
+#pragma unroll
+  for (int i = 0; i < TR - 1; ++i) read_x(0, i);
+  read_scales(0);
   const int fours = a.steps / 4;
   for (int q = 0; q < fours; ++q) {
     next_scales();
@@ -355,74 +396,85 @@ __global__ __launch_bounds__(256, 1) void linear_fp8_tile_kernel(Lin8Args a, int
   }
   // every load has landed and every wave is through with the rings
   wait_meet<0>();
-  // 32 rows at a time: this lane's features of its row to LDS, whole rows back
-  uint8_t *mine = s_ring + wave * 32 * L::kPitch;
-  const int fbase = n0 + wn * WF * 32;
-  constexpr int kLanes = 4 * WF;  // lanes of a row
-  const int rr0 = lane / kLanes, f0 = (lane % kLanes) * 8;
-  const bool whole = m_last >= 64 * WR - 1 && n_last >= 64 * WF - 1;  // nothing of the tile past the ends
 #pragma unroll
-  for (int i = 0; i < WR; ++i) {
-    const int64_t row0 = m0 + (wm * WR + i) * 32;
+  for (int i = 0; i < TR; ++i) settle(acc[i]);
+  // this lane's features of its rows to LDS, whole rows back
+  uint8_t *mine = s_ring + wave * 16 * TR * L::kPitch;
+  const int fbase = n0 + wn * TF * 16;
+  const int64_t row0 = m0 + wm * TR * 16;
+  const bool whole = m_last >= L::kRows - 1 && n_last >= L::kFeatures - 1;  // nothing of the tile past the ends
 #pragma unroll
-    for (int j = 0; j < WF; ++j)
+  for (int i = 0; i < TR; ++i) {
+    const uint16_t *src = ADD ? a.add + min(row0 + 16 * i + c, a.M - 1) * a.add_stride : nullptr;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int f = j * 32 + 8 * e + 4 * kh;
-        float v[4];
+    for (int j = 0; j < TF; ++j) {
+      const int f = 16 * j + 4 * g;
+      f32x4 v = acc[i][j];
+      if constexpr (ADD) {
+        uint16_t r[4];
+        if (whole) {
+          __builtin_memcpy(r, src + fbase + f, 8);
+        } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = acc[i][j][4 * e + k];
-        if constexpr (ADD) {
-          const uint16_t *src = a.add + min(row0 + r, a.M - 1) * a.add_stride;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) v[k] += __uint_as_float((unsigned)src[min(fbase + f + k, a.N - 1)] << 16);
+          for (int k = 0; k < 4; ++k) r[k] = src[min(fbase + f + k, a.N - 1)];
         }
-        const bf16x2 lo{(__bf16)v[0], (__bf16)v[1]}, hi{(__bf16)v[2], (__bf16)v[3]};
-        *reinterpret_cast<u32x2 *>(mine + r * L::kPitch + f * 2) =
-            u32x2{__builtin_bit_cast(unsigned, lo), __builtin_bit_cast(unsigned, hi)};
-      }
-    __builtin_amdgcn_sched_barrier(0);
-    uint16_t *dst = a.out + (row0 + rr0) * a.out_stride + fbase + f0;
 #pragma unroll
-    for (int v = 0; v < kLanes / 2; ++v) {
-      const int rr = v * (64 / kLanes) + rr0;
-      const u32x4 o = *reinterpret_cast<const u32x4 *>(mine + rr * L::kPitch + f0 * 2);
-      if (whole || (row0 + rr < a.M && fbase + f0 + 8 <= a.N)) {
-        __builtin_memcpy(dst, &o, 16);
-      } else if (row0 + rr < a.M) {
+        for (int k = 0; k < 4; ++k) v[k] += __uint_as_float((unsigned)r[k] << 16);
+      }
+      const bf16x2 lo{(__bf16)v[0], (__bf16)v[1]}, hi{(__bf16)v[2], (__bf16)v[3]};
+      *reinterpret_cast<u32x2 *>(mine + (16 * i + c) * L::kPitch + f * 2) =
+          u32x2{__builtin_bit_cast(unsigned, lo), __builtin_bit_cast(unsigned, hi)};
+    }
+  }
+  constexpr int kLanes = 2 * TF, kAtOnce = 64 / kLanes;  // lanes of a row, rows of an instruction
+  const int rr0 = lane / kLanes, f0 = (lane % kLanes) * 8;
+  const uint8_t *back = mine + rr0 * L::kPitch + f0 * 2;
+  uint16_t *dst = a.out + (row0 + rr0) * a.out_stride + fbase + f0;
+  if (whole) {
+#pragma unroll
+    for (int v = 0; v < 16 * TR / kAtOnce; ++v) {
+      const u32x4 o = *reinterpret_cast<const u32x4 *>(back + v * kAtOnce * L::kPitch);
+      __builtin_memcpy(dst + (int64_t)v * kAtOnce * a.out_stride, &o, 16);
+    }
+  } else {
+    for (int v = 0; v < 16 * TR / kAtOnce; ++v) {
+      const u32x4 o = *reinterpret_cast<const u32x4 *>(back + v * kAtOnce * L::kPitch);
+      if (row0 + rr0 + v * kAtOnce >= a.M) break;
+      uint16_t *to = dst + (int64_t)v * kAtOnce * a.out_stride;
+      if (fbase + f0 + 8 <= a.N) {
+        __builtin_memcpy(to, &o, 16);
+      } else {
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          if (fbase + f0 + k < a.N) dst[k] = (uint16_t)(o[k >> 1] >> (16 * (k & 1)));
+          if (fbase + f0 + k < a.N) to[k] = (uint16_t)(o[k >> 1] >> (16 * (k & 1)));
       }
-      dst += (64 / kLanes) * a.out_stride;
     }
-    __builtin_amdgcn_sched_barrier(0);
   }
 }
 
 // The tile kernel addresses a tile's operands by 32-bit offsets.
-template <int WR, int WF> bool tile8_fits(const Lin8Args &a) {
-  return a.x_stride <= 0x7FFFFFFF / (64 * WR + 1) && (int64_t)a.steps * 2048 <= 0x7FFFFFFF / (4 * WF + 1);
+template <typename L> bool tile8_fits(const Lin8Args &a) {
+  return a.x_stride <= 0x7FFFFFFF / (L::kRows + 1) && (int64_t)a.steps * 2048 <= 0x7FFFFFFF / (L::kFeatures / 16 + 1);
 }
 
-template <int WR, int WF, bool ADD> int launch_tile8_as(const Lin8Args &a, hipStream_t s) {
-  constexpr int lds = Tile8<WR, WF>::kLds;
+template <int TR, int TF, int WM, int WN, bool ADD> int launch_tile8_as(const Lin8Args &a, hipStream_t s) {
+  using L = Tile8<TR, TF, WM, WN>;
   static bool ready[64];
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return SPECDEC_EHIP;
   if (!ready[dev]) {
-    if (hipFuncSetAttribute((const void *)linear_fp8_tile_kernel<WR, WF, ADD>,
-                            hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
+    if (hipFuncSetAttribute((const void *)linear_fp8_tile_kernel<TR, TF, WM, WN, ADD>,
+                            hipFuncAttributeMaxDynamicSharedMemorySize, L::kLds) != hipSuccess)
       return SPECDEC_EHIP;
     ready[dev] = true;
   }
-  const int tm = (int)((a.M + 64 * WR - 1) / (64 * WR)), tn = (a.N + 64 * WF - 1) / (64 * WF);
-  linear_fp8_tile_kernel<WR, WF, ADD><<<tm * tn, 256, lds, s>>>(a, tm, tn);
+  const int tm = (int)((a.M + L::kRows - 1) / L::kRows), tn = (a.N + L::kFeatures - 1) / L::kFeatures;
+  linear_fp8_tile_kernel<TR, TF, WM, WN, ADD><<<tm * tn, 256, L::kLds, s>>>(a, tm, tn);
   return launch_status();
 }
 
-template <int WR, int WF> int launch_tile8(const Lin8Args &a, hipStream_t s) {
-  return a.add ? launch_tile8_as<WR, WF, true>(a, s) : launch_tile8_as<WR, WF, false>(a, s);
+template <int TR, int TF, int WM, int WN> int launch_tile8(const Lin8Args &a, hipStream_t s) {
+  return a.add ? launch_tile8_as<TR, TF, WM, WN, true>(a, s) : launch_tile8_as<TR, TF, WM, WN, false>(a, s);
 }
 
 }  // namespace specdec
@@ -452,8 +504,8 @@ SPECDEC_API int specdec_linear_fp8(const void *x, int64_t x_stride, const void *
   a.per_wave = (a.steps + waves - 1) / waves;
   const unsigned tiles = (unsigned)((out_features + 15) / 16);
   hipStream_t s = as_stream(stream);
-  if (rows > 512 && tile8_fits<4, 4>(a)) return launch_tile8<4, 4>(a, s);
-  if (rows > 64 && tile8_fits<2, 2>(a)) return launch_tile8<2, 2>(a, s);
+  if (rows > 512 && tile8_fits<Tile8<8, 8, 2, 2>>(a)) return launch_tile8<8, 8, 2, 2>(a, s);
+  if (rows > 64 && tile8_fits<Tile8<4, 4, 2, 2>>(a)) return launch_tile8<4, 4, 2, 2>(a, s);
   if (rows <= 16)
     linear_fp8_kernel<1><<<dim3(tiles, 1), waves * 64, 0, s>>>(a);
   else
