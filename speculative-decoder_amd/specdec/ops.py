@@ -433,32 +433,45 @@ def _launch(dev: torch.device, entry, *args) -> int:
 
 def _fp8_rows(dev: torch.device, lead, k: int, codes: torch.Tensor | None, scales: torch.Tensor | None):
     """codes [*lead, Kp] and scales [*lead, Gp] of rows of k values: given and checked, or new."""
-    cshape, sshape = (*lead, fp8_code_cols(k)), (*lead, fp8_scale_cols(k))
-    for t, shape, dtype, align, name in ((codes, cshape, FP8_CODE, 16, "codes"), (scales, sshape, FP8_SCALE, 4, "scales")):
-        if t is not None:
-            _on(dev, t, name, dtype, True)
-            if tuple(t.shape) != shape:
-                raise ValueError(f"{name} must be {list(shape)} (got {list(t.shape)})")
-            if t.data_ptr() % align:
-                raise ValueError(f"{name} must be {align}-byte aligned")
+    cshape, sshape = (*lead, -(-k // 128) * 128), (*lead, -(-k // 512) * 4)
     if codes is None:
         codes = torch.empty(cshape, dtype=FP8_CODE, device=dev)
+    else:
+        _fp8_given(dev, codes, cshape, FP8_CODE, 16, "codes")
     if scales is None:
         scales = torch.empty(sshape, dtype=FP8_SCALE, device=dev)
+    else:
+        _fp8_given(dev, scales, sshape, FP8_SCALE, 4, "scales")
     return codes, scales
 
 
-def _fp8_input(x: torch.Tensor, name: str) -> tuple[torch.Tensor, int]:
-    """x as rows [R, K] of unit inner stride, bf16 or fp32."""
-    gpu(x, name)
-    if x.dtype not in (torch.bfloat16, torch.float32):
+def _fp8_given(dev: torch.device, t: torch.Tensor, shape, dtype: torch.dtype, align: int, name: str) -> None:
+    _on(dev, t, name, dtype, True)
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must be {list(shape)} (got {list(t.shape)})")
+    if t.data_ptr() % align:
+        raise ValueError(f"{name} must be {align}-byte aligned")
+
+
+_FP8_INPUTS = {torch.bfloat16: BF16, torch.float32: F32}
+
+
+def _fp8_input(x: torch.Tensor, name: str) -> tuple[torch.Tensor, int, int, int, int]:
+    """x as rows of unit inner stride, bf16 or fp32: the tensor that holds
+    them, their type's code, number, width and stride."""
+    if not x.is_cuda:
+        gpu(x, name)
+    dt = _FP8_INPUTS.get(x.dtype)
+    if dt is None:
         raise TypeError(f"{name} must be bf16 or fp32 (got {x.dtype})")
     if x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError(f"{name} needs rows of at least one value (got {list(x.shape)})")
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    if x2.stride(1) != 1 or x2.shape[0] > 1 and x2.stride(0) < x2.shape[1]:  # transposed, or overlapping rows
-        x2 = x2.contiguous()
-    return x2, _DTYPES[x.dtype]
+    rows, k = x2.shape
+    stride, inner = x2.stride()
+    if inner != 1 and k > 1 or rows > 1 and stride < k:  # transposed, or overlapping rows
+        x2, stride = x2.contiguous(), k
+    return x2, dt, rows, k, stride
 
 
 def quantize_fp8(x: torch.Tensor, codes: torch.Tensor | None = None, scales: torch.Tensor | None = None):
@@ -470,25 +483,28 @@ def quantize_fp8(x: torch.Tensor, codes: torch.Tensor | None = None, scales: tor
     values as its scale, and y / s rounded to nearest even as its codes; an
     infinity or NaN becomes a NaN code.  Codes past K are zeros, scales past
     the groups ones.  `codes` and `scales` take the results where given."""
-    x2, dt = _fp8_input(x, "x")
-    codes, scales = _fp8_rows(x.device, x.shape[:-1], x2.shape[1], codes, scales)
-    st = _launch(x.device, lib().specdec_quantize_fp8, x2.data_ptr(), dt, x2.shape[0], x2.shape[1], x2.stride(0),
-                 codes.data_ptr(), scales.data_ptr())
-    _check(st, "quantize_fp8")
+    x2, dt, rows, k, stride = _fp8_input(x, "x")
+    dev = x.device
+    codes, scales = _fp8_rows(dev, x.shape[:-1], k, codes, scales)
+    st = _launch(dev, lib().specdec_quantize_fp8, x2.data_ptr(), dt, rows, k, stride, codes.data_ptr(),
+                 scales.data_ptr())
+    if st:
+        _check(st, "quantize_fp8")
     return codes, scales
 
 
 def silu_mul_fp8(gate_up: torch.Tensor, codes: torch.Tensor | None = None, scales: torch.Tensor | None = None):
     """quantize_fp8(SiLU(gate) * up) of gate_up [..., 2 I] (gate then up, bf16
     or fp32), computed in fp32 with the one rounding to 8 bits."""
-    x2, dt = _fp8_input(gate_up, "gate_up")
-    if x2.shape[1] % 2:
-        raise ValueError(f"gate_up rows hold gate then up, an even number of values (got {x2.shape[1]})")
-    inter = x2.shape[1] // 2
-    codes, scales = _fp8_rows(gate_up.device, gate_up.shape[:-1], inter, codes, scales)
-    st = _launch(gate_up.device, lib().specdec_silu_mul_fp8, x2.data_ptr(), dt, x2.shape[0], inter, x2.stride(0),
-                 codes.data_ptr(), scales.data_ptr())
-    _check(st, "silu_mul_fp8")
+    x2, dt, rows, two, stride = _fp8_input(gate_up, "gate_up")
+    if two % 2:
+        raise ValueError(f"gate_up rows hold gate then up, an even number of values (got {two})")
+    dev = gate_up.device
+    codes, scales = _fp8_rows(dev, gate_up.shape[:-1], two // 2, codes, scales)
+    st = _launch(dev, lib().specdec_silu_mul_fp8, x2.data_ptr(), dt, rows, two // 2, stride, codes.data_ptr(),
+                 scales.data_ptr())
+    if st:
+        _check(st, "silu_mul_fp8")
     return codes, scales
 
 
@@ -499,23 +515,30 @@ def add_rmsnorm_fp8(hidden: torch.Tensor, delta: torch.Tensor | None, weight: to
     `summed`, else back to hidden), then quantize_fp8(h * rsqrt(mean(h^2) +
     eps) * weight), the norm in fp32 with the one rounding to 8 bits.  hidden,
     delta and summed [..., D] contiguous, bf16 or fp32, D <= 16384."""
-    dev = gpu(hidden, "hidden").device
-    if hidden.dtype not in (torch.bfloat16, torch.float32):
-        raise TypeError(f"hidden must be bf16 or fp32 (got {hidden.dtype})")
-    if hidden.dim() < 1 or hidden.shape[-1] == 0:
-        raise ValueError(f"hidden needs rows of at least one value (got {list(hidden.shape)})")
-    dim = hidden.shape[-1]
-    _on(dev, hidden, "hidden", contiguous=True)
-    _on(dev, weight, "weight", hidden.dtype, True, dim)
+    if not hidden.is_cuda:
+        gpu(hidden, "hidden")
+    dev, dtype = hidden.device, hidden.dtype
+    dt = _FP8_INPUTS.get(dtype)
+    if dt is None:
+        raise TypeError(f"hidden must be bf16 or fp32 (got {dtype})")
+    shape = hidden.shape
+    if not shape or shape[-1] == 0:
+        raise ValueError(f"hidden needs rows of at least one value (got {list(shape)})")
+    dim, count = shape[-1], hidden.numel()
+    _on(dev, hidden, "hidden", None, True)
+    _on(dev, weight, "weight", dtype, True, dim)
+    delta_ptr = summed_ptr = None
     if delta is not None:
-        _on(dev, delta, "delta", hidden.dtype, True, hidden.numel())
-        summed = hidden if summed is None else _on(dev, summed, "summed", hidden.dtype, True, hidden.numel())
+        _on(dev, delta, "delta", dtype, True, count)
+        delta_ptr = delta.data_ptr()
+        summed_ptr = (hidden if summed is None else _on(dev, summed, "summed", dtype, True, count)).data_ptr()
     elif summed is not None:
         raise ValueError("summed is written where there is a delta only")
-    codes, scales = _fp8_rows(dev, hidden.shape[:-1], dim, codes, scales)
-    st = _launch(dev, lib().specdec_add_rmsnorm_fp8, hidden.data_ptr(), ptr(delta), weight.data_ptr(), ptr(summed),
-                 _DTYPES[hidden.dtype], hidden.numel() // dim, dim, float(eps), codes.data_ptr(), scales.data_ptr())
-    _check(st, "add_rmsnorm_fp8")
+    codes, scales = _fp8_rows(dev, shape[:-1], dim, codes, scales)
+    st = _launch(dev, lib().specdec_add_rmsnorm_fp8, hidden.data_ptr(), delta_ptr, weight.data_ptr(), summed_ptr, dt,
+                 count // dim, dim, eps, codes.data_ptr(), scales.data_ptr())
+    if st:
+        _check(st, "add_rmsnorm_fp8")
     return codes, scales
 
 
@@ -546,45 +569,65 @@ def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scale
     accumulated in fp32 and rounded once: bf16 [..., N].  With `add` (bf16,
     [..., N]; it may be `out`) out = x @ w.T + add inside that rounding.  Calls
     of at most 64 rows give a row the same bits whatever rows come with it."""
-    dev = gpu(w, "w").device
-    if w.dtype != FP8_CODE or w.dim() != 5 or tuple(w.shape[2:]) != (2, 64, 16) or not w.is_contiguous():
+    if not w.is_cuda:
+        gpu(w, "w")
+    dev, wshape = w.device, w.shape
+    if w.dtype != FP8_CODE or len(wshape) != 5 or wshape[2:] != (2, 64, 16) or not w.is_contiguous():
         raise ValueError("w must be a tile_weight_fp8() result")
-    kp = w.shape[1] * FP8_GROUP
-    gp = -(-w.shape[1] // 4) * 4
+    kp, gp = wshape[1] * 128, -(-wshape[1] // 4) * 4
     _on(dev, w_scales, "w_scales", FP8_SCALE, True)
     n = w_scales.shape[0]
-    if w_scales.dim() != 2 or w_scales.shape[1] != gp or -(-n // 16) != w.shape[0]:
-        raise ValueError(f"w_scales must be [N, {gp}] with N in {16 * w.shape[0]} - 15 .. {16 * w.shape[0]} "
+    if w_scales.dim() != 2 or w_scales.shape[1] != gp or -(-n // 16) != wshape[0]:
+        raise ValueError(f"w_scales must be [N, {gp}] with N in {16 * wshape[0] - 15} .. {16 * wshape[0]} "
                          f"(got {list(w_scales.shape)})")
     _on(dev, x, "x", FP8_CODE)
     _on(dev, x_scales, "x_scales", FP8_SCALE)
-    if x.shape[-1:] != (kp,) or x_scales.shape != (*x.shape[:-1], gp):
+    lead = x.shape[:-1]
+    if x.shape[-1:] != (kp,) or x_scales.shape != (*lead, gp):
         raise ValueError(f"x must be [..., {kp}] and x_scales [..., {gp}] "
                          f"(got {list(x.shape)} and {list(x_scales.shape)})")
-    x2 = x if x.dim() == 2 else x.reshape(-1, kp)
-    s2 = x_scales if x_scales.dim() == 2 else x_scales.reshape(-1, gp)
+    x2, x_ptr, x_stride = _fp8_operand(x, kp, 16)
     rows = x2.shape[0]
-    if x2.stride(1) != 1 or rows > 1 and (x2.stride(0) < kp or x2.stride(0) % 16) or x2.data_ptr() % 16:
-        x2 = x2.clone(memory_format=torch.contiguous_format)
-    if s2.stride(1) != 1 or rows > 1 and (s2.stride(0) < gp or s2.stride(0) % 4) or s2.data_ptr() % 4:
-        s2 = s2.clone(memory_format=torch.contiguous_format)
+    s2, s_ptr, s_stride = _fp8_operand(x_scales, gp, 4)
+    if add is None:
+        add_ptr, add_stride = None, 0
+    else:
+        add_ptr, add_stride = _fp8_output(dev, add, rows, n, "add")
+    if out is None:
+        result = torch.empty((*lead, n), dtype=torch.bfloat16, device=dev)
+        out_ptr, out_stride = result.data_ptr(), n
+    else:
+        result = out
+        out_ptr, out_stride = _fp8_output(dev, out, rows, n, "out")
+    st = _launch(dev, lib().specdec_linear_fp8, x_ptr, x_stride, s_ptr, s_stride, w.data_ptr(), w_scales.data_ptr(),
+                 rows, kp, n, add_ptr, add_stride, out_ptr, out_stride)
+    if st:
+        _check(st, "linear_fp8")
+    return result
 
-    def flat(t: torch.Tensor, name: str) -> torch.Tensor:
-        _on(dev, t, name, torch.bfloat16)
-        t2 = t if t.dim() == 2 else t.view(-1, t.shape[-1])
-        if tuple(t2.shape) != (rows, n) or t2.stride(1) != 1 or (rows > 1 and t2.stride(0) < n):
-            raise ValueError(f"{name} must be bf16 [rows, N] = [{rows}, {n}] with unit inner stride and rows apart")
-        return t2
 
-    a2 = None if add is None else flat(add, "add")
-    fresh = out is None
-    o2 = torch.empty(rows, n, dtype=torch.bfloat16, device=dev) if fresh else flat(out, "out")
-    one = rows <= 1  # a single row's strides mean nothing
-    st = _launch(dev, lib().specdec_linear_fp8, x2.data_ptr(), kp if one else x2.stride(0), s2.data_ptr(),
-                 gp if one else s2.stride(0), w.data_ptr(), w_scales.data_ptr(), rows, kp, n, ptr(a2),
-                 n if one or a2 is None else a2.stride(0), o2.data_ptr(), n if one else o2.stride(0))
-    _check(st, "linear_fp8")
-    return o2.view(*x.shape[:-1], n) if fresh else out
+def _fp8_operand(t: torch.Tensor, cols: int, align: int) -> tuple[torch.Tensor, int, int]:
+    """t [..., cols] of one-byte elements as rows whose starts are aligned: the
+    tensor that holds them, its address and its rows' stride."""
+    t2 = t if t.dim() == 2 else t.reshape(-1, cols)
+    stride, inner = t2.stride()
+    if t2.shape[0] <= 1:  # a single row's stride means nothing
+        stride = cols
+    if inner != 1 or stride < cols or stride % align or t2.data_ptr() % align:
+        t2, stride = t2.clone(memory_format=torch.contiguous_format), cols
+    return t2, t2.data_ptr(), stride
+
+
+def _fp8_output(dev: torch.device, t: torch.Tensor, rows: int, n: int, name: str) -> tuple[int, int]:
+    """Address and row stride of a bf16 [..., N] tensor that a product adds or writes."""
+    _on(dev, t, name, torch.bfloat16)
+    t2 = t if t.dim() == 2 else t.view(-1, t.shape[-1])
+    stride, inner = t2.stride()
+    if rows <= 1:
+        stride = n
+    if t2.shape != (rows, n) or inner != 1 and n > 1 or stride < n:
+        raise ValueError(f"{name} must be bf16 [rows, N] = [{rows}, {n}] with unit inner stride and rows apart")
+    return t2.data_ptr(), stride
 
 
 def head_logits(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
