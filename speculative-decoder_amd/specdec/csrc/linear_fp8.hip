@@ -18,8 +18,6 @@ typedef __attribute__((ext_vector_type(8))) int i32x8;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef __attribute__((ext_vector_type(2))) unsigned int u32x2;
 
-constexpr int kLin8MaxWaves = 8;
-
 struct Lin8Args {
   const uint8_t *x;  // codes [M, x_stride], 128 `steps` of each row used
   int64_t x_stride;
@@ -45,30 +43,28 @@ __device__ __forceinline__ f32x4 mfma8(i32x8 a, i32x8 b, f32x4 c, unsigned sa, u
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, (int)sa, 0, (int)sb);
 }
 
-// out's four features f0 .. f0 + 3 of row `row`
-__device__ __forceinline__ void store4(const Lin8Args &a, int64_t row, int f0, f32x4 v) {
-  uint16_t *dst = a.out + row * a.out_stride + f0;
-  uint16_t o[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float y = v[i];
-    if (a.add && f0 + i < a.N) y += __uint_as_float((unsigned)a.add[row * a.add_stride + f0 + i] << 16);
-    o[i] = __builtin_bit_cast(uint16_t, __float2bfloat16(y));
-  }
-  if (f0 + 3 < a.N && ((uintptr_t)dst & 7) == 0) {
-    *reinterpret_cast<u32x2 *>(dst) =
-        u32x2{(uint32_t)o[0] | ((uint32_t)o[1] << 16), (uint32_t)o[2] | ((uint32_t)o[3] << 16)};
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (f0 + i < a.N) dst[i] = o[i];
-  }
+// ----------------------------------------------------------------- few rows --
+constexpr int kLin8MaxWaves = 16;
+
+// The steps of a wave: a power of two (so that four steps' scales are in one
+// word), at most 16 waves a feature tile and, where that leaves enough of them,
+// 16 waves a compute unit.  Of the weight's sizes alone: the order of a row's
+// sums does not depend on the other rows of the call.
+inline int lin8_steps_per_wave(int tiles, int steps) {
+  int per = 1;
+  while ((steps + per - 1) / per > kLin8MaxWaves ||
+         ((int64_t)tiles * ((steps + per - 1) / per) > 4096 && per < steps && per < 8))
+    per *= 2;
+  return per;
 }
 
 // 16 RT rows and one feature tile a workgroup; the waves split the steps and
-// their sums are added in wave order.
-template <int RT> __global__ __launch_bounds__(kLin8MaxWaves * 64) void linear_fp8_kernel(Lin8Args a) {
-  __shared__ f32x4 s_acc[kLin8MaxWaves][RT][64];
+// their sums are added in wave order.  Bound by how many bytes are on their way
+// (a wave asks for KB steps of W and x at once, and there are up to 16 waves of
+// up to 128 registers), so x, which every workgroup reads, comes from L2 straight
+// to registers.
+template <int RT, int KB> __global__ __launch_bounds__(kLin8MaxWaves * 64) void linear_fp8_kernel(Lin8Args a) {
+  extern __shared__ f32x4 s_acc[];  // [wave][RT][64]
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nw = blockDim.x >> 6;
   const int c = lane & 15, g = lane >> 4;
   const int n0 = blockIdx.x * 16;
@@ -84,29 +80,91 @@ template <int RT> __global__ __launch_bounds__(kLin8MaxWaves * 64) void linear_f
     xp[t] = a.x + row * a.x_stride + 16 * g;
     xsp[t] = a.xs + row * a.xs_stride;
   }
+  // what is added before the rounding, asked for now
+  const int f0 = n0 + 4 * g;
+  const int64_t first = m0 + 16 * wave + c;
+  uint16_t pre[4] = {0, 0, 0, 0};
+  if (a.add && wave < RT && first < a.M) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pre[i] = a.add[first * a.add_stride + min(f0 + i, a.N - 1)];
+  }
   f32x4 acc[RT];
 #pragma unroll
   for (int t = 0; t < RT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int s = s_lo; s < s_hi; ++s) {
-    const u32x4 *wv = reinterpret_cast<const u32x4 *>(wp + (int64_t)s * 2048);
-    const i32x8 av = join8(wv[0], wv[64]);
-    const unsigned sa = wsp[s];
+  for (int s4 = s_lo; s4 < s_hi; s4 += 4) {  // the steps of a word of scales
+    const int word = s4 & ~3;
+    unsigned sa = *reinterpret_cast<const unsigned *>(wsp + word), sb[RT];
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      const u32x4 *xv = reinterpret_cast<const u32x4 *>(xp[t] + (int64_t)s * 128);
-      acc[t] = mfma8(av, join8(xv[0], xv[4]), acc[t], sa, xsp[t][s]);
+    for (int t = 0; t < RT; ++t) sb[t] = *reinterpret_cast<const unsigned *>(xsp[t] + word);
+    const int end = min(s4 + 4, s_hi);
+#pragma unroll
+    for (int h = 0; h < 4; h += KB) {
+      if (s4 + h < end) {
+        u32x4 W[KB][2], X[KB][RT][2];
+#pragma unroll
+        for (int j = 0; j < KB; ++j) {
+          const int s = min(s4 + h + j, end - 1);
+          const u32x4 *wv = reinterpret_cast<const u32x4 *>(wp + (int64_t)s * 2048);
+          W[j][0] = wv[0];
+          W[j][1] = wv[64];
+#pragma unroll
+          for (int t = 0; t < RT; ++t) {
+            const u32x4 *xv = reinterpret_cast<const u32x4 *>(xp[t] + (int64_t)s * 128);
+            X[j][t][0] = xv[0];
+            X[j][t][1] = xv[4];
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);  // all of them before the first product
+#pragma unroll
+        for (int j = 0; j < KB; ++j) {
+          const int s = s4 + h + j;
+          if (s < end) {
+            const int byte = 8 * (s & 3);
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+              acc[t] = mfma8(join8(W[j][0], W[j][1]), join8(X[j][t][0], X[j][t][1]), acc[t], sa >> byte, sb[t] >> byte);
+          }
+        }
+      }
     }
   }
 #pragma unroll
-  for (int t = 0; t < RT; ++t) s_acc[wave][t][lane] = acc[t];
+  for (int t = 0; t < RT; ++t) s_acc[(wave * RT + t) * 64 + lane] = acc[t];
   __syncthreads();
   for (int t = wave; t < RT; t += nw) {
     const int64_t row = m0 + 16 * t + c;
     if (row >= a.M) continue;
-    f32x4 v = s_acc[0][t][lane];
-    for (int w = 1; w < nw; ++w) v += s_acc[w][t][lane];
-    store4(a, row, n0 + 4 * g, v);
+    f32x4 v = s_acc[t * 64 + lane];
+    for (int w = 1; w < nw; ++w) v += s_acc[(w * RT + t) * 64 + lane];
+    if (a.add && t != wave) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pre[i] = a.add[row * a.add_stride + min(f0 + i, a.N - 1)];
+    }
+    uint16_t *dst = a.out + row * a.out_stride + f0;
+    uint16_t o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float y = v[i];
+      if (a.add) y += __uint_as_float((unsigned)pre[i] << 16);
+      o[i] = __builtin_bit_cast(uint16_t, __float2bfloat16(y));
+    }
+    if (f0 + 3 < a.N) {
+      __builtin_memcpy(dst, o, 8);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (f0 + i < a.N) dst[i] = o[i];
+    }
   }
+}
+
+template <int RT, int KB> int launch_lin8(Lin8Args a, hipStream_t s) {
+  const int tiles = (a.N + 15) / 16;
+  a.per_wave = lin8_steps_per_wave(tiles, a.steps);
+  const int waves = (a.steps + a.per_wave - 1) / a.per_wave;
+  const dim3 grid((unsigned)tiles, (unsigned)((a.M + 16 * RT - 1) / (16 * RT)));
+  linear_fp8_kernel<RT, KB><<<grid, waves * 64, waves * RT * 1024, s>>>(a);
+  return launch_status();
 }
 
 // ---------------------------------------------------------------- many rows --
@@ -500,15 +558,11 @@ SPECDEC_API int specdec_linear_fp8(const void *x, int64_t x_stride, const void *
   Lin8Args a{(const uint8_t *)x, x_stride,   (const uint8_t *)x_scales, x_scale_stride, (const uint8_t *)w,
              (const uint8_t *)w_scales, (uint16_t *)out, out_stride, (const uint16_t *)add, add_stride, rows,
              (int)out_features, (int)steps, 0};
-  const int waves = std::min<int>(kLin8MaxWaves, a.steps);
-  a.per_wave = (a.steps + waves - 1) / waves;
-  const unsigned tiles = (unsigned)((out_features + 15) / 16);
   hipStream_t s = as_stream(stream);
   if (rows > 512 && tile8_fits<Tile8<8, 8, 2, 2>>(a)) return launch_tile8<8, 8, 2, 2>(a, s);
   if (rows > 64 && tile8_fits<Tile8<4, 4, 2, 2>>(a)) return launch_tile8<4, 4, 2, 2>(a, s);
-  if (rows <= 16)
-    linear_fp8_kernel<1><<<dim3(tiles, 1), waves * 64, 0, s>>>(a);
-  else
-    linear_fp8_kernel<4><<<dim3(tiles, (unsigned)((rows + 63) / 64)), waves * 64, 0, s>>>(a);
-  return launch_status();
+  if (rows <= 16) return launch_lin8<1, 4>(a, s);
+  if (rows <= 32) return launch_lin8<2, 4>(a, s);
+  if (rows <= 48) return launch_lin8<3, 2>(a, s);
+  return launch_lin8<4, 2>(a, s);
 }
