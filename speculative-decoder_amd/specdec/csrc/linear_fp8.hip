@@ -43,76 +43,110 @@ __device__ __forceinline__ f32x4 mfma8(i32x8 a, i32x8 b, f32x4 c, unsigned sa, u
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, (int)sa, 0, (int)sb);
 }
 
+// More than 64 KB of LDS has to be allowed for, once a kernel and device.
+template <typename K> int allow_lds(K kernel, int bytes) {
+  return hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess
+             ? SPECDEC_OK
+             : SPECDEC_EHIP;
+}
+
 // ----------------------------------------------------------------- few rows --
-constexpr int kLin8MaxWaves = 16;
+constexpr int kLin8MaxWaves = 8;
 
 // The steps of a wave: a power of two (so that four steps' scales are in one
 // word), at most 16 waves a feature tile and, where that leaves enough of them,
 // 16 waves a compute unit.  Of the weight's sizes alone: the order of a row's
 // sums does not depend on the other rows of the call.
-inline int lin8_steps_per_wave(int tiles, int steps) {
+inline int lin8_steps_per_wave(int steps) {
   int per = 1;
-  while ((steps + per - 1) / per > kLin8MaxWaves ||
-         ((int64_t)tiles * ((steps + per - 1) / per) > 4096 && per < steps && per < 8))
-    per *= 2;
+  while (per < 4 ? (steps + per - 1) / per > 4 : (steps + per - 1) / per > kLin8MaxWaves) per *= 2;
   return per;
 }
 
-// 16 RT rows and one feature tile a workgroup; the waves split the steps and
-// their sums are added in wave order.  Bound by how many bytes are on their way
-// (a wave asks for KB steps of W and x at once, and there are up to 16 waves of
-// up to 128 registers), so x, which every workgroup reads, comes from L2 straight
-// to registers.
-template <int RT, int KB> __global__ __launch_bounds__(kLin8MaxWaves * 64) void linear_fp8_kernel(Lin8Args a) {
-  extern __shared__ f32x4 s_acc[];  // [wave][RT][64]
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nw = blockDim.x >> 6;
+// Lane l of 64's partner l ^ 8, as a rotation of each row of 16 lanes by 8.
+__device__ __forceinline__ u32x4 from_partner(u32x4 v) {
+  u32x4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = (unsigned)dpp_move<0x128>((int)v[i]);
+  return r;
+}
+
+// 16 RT rows and F feature tiles a workgroup; the waves split the steps and
+// their sums are added in wave order.  A wave asks for KB steps of W and x at
+// once and there are up to 16 waves of up to 128 registers, so x, which every
+// workgroup reads, comes from L2 straight to registers.  What bounds that is
+// the cache lines the memory path looks up (about three cycles each), so one
+// load takes eight whole lines, 128 inputs of eight rows: lanes c < 8 of each 16
+// take the first halves of rows c, then c + 8, lanes c >= 8 the second halves of
+// rows c - 8, then c, and partners exchange what is not their row's.
+template <int RT, int F, int KB> __global__ __launch_bounds__(kLin8MaxWaves * 64) void linear_fp8_kernel(Lin8Args a) {
+  extern __shared__ f32x4 s_acc[];  // [wave][RT][F][64]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
   const int c = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 16;
+  const bool upper = c >= 8;
+  const int ftiles = (a.N + 15) / 16, n0 = blockIdx.x * (16 * F);
   const int64_t m0 = (int64_t)blockIdx.y * (16 * RT);
+  const int m_last = (int)min(a.M - 1 - m0, (int64_t)16 * RT - 1);
   const int s_lo = wave * a.per_wave, s_hi = min(s_lo + a.per_wave, a.steps);
+  // features past N read the last tile's, rows past M the last row; neither is stored
+  const uint8_t *wp[F];
+  unsigned wsoff[F], xoff[RT][2], xsoff[RT];
   const int ws_stride = (a.steps + 3) / 4 * 4;
-  const uint8_t *wp = a.w + ((int64_t)blockIdx.x * a.steps) * 2048 + lane * 16;
-  const uint8_t *wsp = a.ws + (int64_t)min(n0 + c, a.N - 1) * ws_stride;
-  const uint8_t *xp[RT], *xsp[RT];
 #pragma unroll
-  for (int t = 0; t < RT; ++t) {  // rows past M read the last row, never stored
-    const int64_t row = min(m0 + 16 * t + c, a.M - 1);
-    xp[t] = a.x + row * a.x_stride + 16 * g;
-    xsp[t] = a.xs + row * a.xs_stride;
+  for (int f = 0; f < F; ++f) {
+    wp[f] = a.w + (int64_t)min((int)blockIdx.x * F + f, ftiles - 1) * a.steps * 2048;
+    wsoff[f] = (unsigned)(min(n0 + 16 * f + c, a.N - 1) - n0) * ws_stride;
   }
-  // what is added before the rounding, asked for now
-  const int f0 = n0 + 4 * g;
-  const int64_t first = m0 + 16 * wave + c;
+  const uint8_t *wsb = a.ws + (int64_t)n0 * ws_stride;
+  const uint8_t *xb = a.x + m0 * a.x_stride, *xsb = a.xs + m0 * a.xs_stride;
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      xoff[t][h] = (unsigned)min(16 * t + 8 * h + (c & 7), m_last) * (unsigned)a.x_stride + (upper ? 64 : 0) + 16 * g;
+    xsoff[t] = (unsigned)min(16 * t + c, m_last) * (unsigned)a.xs_stride;
+  }
+  // what is added before the rounding, asked for now: wave w finishes the
+  // (w / F)-th 16 rows of the (w % F)-th tile
   uint16_t pre[4] = {0, 0, 0, 0};
-  if (a.add && wave < RT && first < a.M) {
+  auto load_add = [&](int o) {
+    const int row = 16 * (o / F) + c, f0 = n0 + 16 * (o % F) + 4 * g;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) pre[i] = a.add[first * a.add_stride + min(f0 + i, a.N - 1)];
-  }
-  f32x4 acc[RT];
+    for (int i = 0; i < 4; ++i)
+      pre[i] = a.add[(m0 + min(row, m_last)) * a.add_stride + min(f0 + i, a.N - 1)];
+  };
+  if (a.add && wave < RT * F) load_add(wave);
+  f32x4 acc[RT][F];
 #pragma unroll
-  for (int t = 0; t < RT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int t = 0; t < RT; ++t)
+#pragma unroll
+    for (int f = 0; f < F; ++f) acc[t][f] = f32x4{0.f, 0.f, 0.f, 0.f};
   for (int s4 = s_lo; s4 < s_hi; s4 += 4) {  // the steps of a word of scales
     const int word = s4 & ~3;
-    unsigned sa = *reinterpret_cast<const unsigned *>(wsp + word), sb[RT];
+    unsigned sa[F], sb[RT];
 #pragma unroll
-    for (int t = 0; t < RT; ++t) sb[t] = *reinterpret_cast<const unsigned *>(xsp[t] + word);
+    for (int f = 0; f < F; ++f) sa[f] = *reinterpret_cast<const unsigned *>(wsb + word + wsoff[f]);
+#pragma unroll
+    for (int t = 0; t < RT; ++t) sb[t] = *reinterpret_cast<const unsigned *>(xsb + word + xsoff[t]);
     const int end = min(s4 + 4, s_hi);
 #pragma unroll
     for (int h = 0; h < 4; h += KB) {
       if (s4 + h < end) {
-        u32x4 W[KB][2], X[KB][RT][2];
+        u32x4 W[KB][F][2], X[KB][RT][2];
 #pragma unroll
         for (int j = 0; j < KB; ++j) {
           const int s = min(s4 + h + j, end - 1);
-          const u32x4 *wv = reinterpret_cast<const u32x4 *>(wp + (int64_t)s * 2048);
-          W[j][0] = wv[0];
-          W[j][1] = wv[64];
 #pragma unroll
-          for (int t = 0; t < RT; ++t) {
-            const u32x4 *xv = reinterpret_cast<const u32x4 *>(xp[t] + (int64_t)s * 128);
-            X[j][t][0] = xv[0];
-            X[j][t][1] = xv[4];
+          for (int f = 0; f < F; ++f) {
+            const u32x4 *wv = reinterpret_cast<const u32x4 *>(wp[f] + (int64_t)s * 2048);
+            W[j][f][0] = wv[lane];
+            W[j][f][1] = wv[lane + 64];
           }
+          const uint8_t *xs = xb + s * 128;
+#pragma unroll
+          for (int t = 0; t < RT; ++t)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) X[j][t][e] = *reinterpret_cast<const u32x4 *>(xs + xoff[t][e]);
         }
         __builtin_amdgcn_sched_barrier(0);  // all of them before the first product
 #pragma unroll
@@ -121,50 +155,81 @@ template <int RT, int KB> __global__ __launch_bounds__(kLin8MaxWaves * 64) void 
           if (s < end) {
             const int byte = 8 * (s & 3);
 #pragma unroll
-            for (int t = 0; t < RT; ++t)
-              acc[t] = mfma8(join8(W[j][0], W[j][1]), join8(X[j][t][0], X[j][t][1]), acc[t], sa >> byte, sb[t] >> byte);
+            for (int t = 0; t < RT; ++t) {
+              const u32x4 got = from_partner(upper ? X[j][t][0] : X[j][t][1]);
+              const i32x8 x = join8(upper ? got : X[j][t][0], upper ? X[j][t][1] : got);
+#pragma unroll
+              for (int f = 0; f < F; ++f)
+                acc[t][f] = mfma8(join8(W[j][f][0], W[j][f][1]), x, acc[t][f], sa[f] >> byte, sb[t] >> byte);
+            }
           }
         }
       }
     }
   }
 #pragma unroll
-  for (int t = 0; t < RT; ++t) s_acc[(wave * RT + t) * 64 + lane] = acc[t];
-  __syncthreads();
-  for (int t = wave; t < RT; t += nw) {
-    const int64_t row = m0 + 16 * t + c;
-    if (row >= a.M) continue;
-    f32x4 v = s_acc[t * 64 + lane];
-    for (int w = 1; w < nw; ++w) v += s_acc[(w * RT + t) * 64 + lane];
-    if (a.add && t != wave) {
+  for (int t = 0; t < RT; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) pre[i] = a.add[row * a.add_stride + min(f0 + i, a.N - 1)];
-    }
-    uint16_t *dst = a.out + row * a.out_stride + f0;
-    uint16_t o[4];
+    for (int f = 0; f < F; ++f) s_acc[((wave * RT + t) * F + f) * 64 + lane] = acc[t][f];
+  __syncthreads();
+  for (int o = wave; o < RT * F; o += nw) {
+    if (a.add && o != wave) load_add(o);
+    const int row = 16 * (o / F) + c, f0 = n0 + 16 * (o % F) + 4 * g;
+    f32x4 v = s_acc[o * 64 + lane];
+    for (int w = 1; w < nw; ++w) v += s_acc[(w * RT * F + o) * 64 + lane];
+    if (row > m_last) continue;
+    uint16_t *dst = a.out + (m0 + row) * a.out_stride + f0;
+    uint16_t out[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float y = v[i];
       if (a.add) y += __uint_as_float((unsigned)pre[i] << 16);
-      o[i] = __builtin_bit_cast(uint16_t, __float2bfloat16(y));
+      out[i] = __builtin_bit_cast(uint16_t, __float2bfloat16(y));
     }
     if (f0 + 3 < a.N) {
-      __builtin_memcpy(dst, o, 8);
+      __builtin_memcpy(dst, out, 8);
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (f0 + i < a.N) dst[i] = o[i];
+        if (f0 + i < a.N) dst[i] = out[i];
     }
   }
 }
 
-template <int RT, int KB> int launch_lin8(Lin8Args a, hipStream_t s) {
+template <int RT, int F, int KB> int launch_lin8(Lin8Args a, hipStream_t s) {
   const int tiles = (a.N + 15) / 16;
-  a.per_wave = lin8_steps_per_wave(tiles, a.steps);
-  const int waves = (a.steps + a.per_wave - 1) / a.per_wave;
-  const dim3 grid((unsigned)tiles, (unsigned)((a.M + 16 * RT - 1) / (16 * RT)));
-  linear_fp8_kernel<RT, KB><<<grid, waves * 64, waves * RT * 1024, s>>>(a);
+  a.per_wave = lin8_steps_per_wave(a.steps);
+  const int waves = (a.steps + a.per_wave - 1) / a.per_wave, lds = waves * RT * F * 1024;
+  const dim3 grid((unsigned)((tiles + F - 1) / F), (unsigned)((a.M + 16 * RT - 1) / (16 * RT)));
+  if (lds > 65536) {
+    const int st = allow_lds((const void *)linear_fp8_kernel<RT, F, KB>, kLin8MaxWaves * RT * F * 1024);
+    if (st != SPECDEC_OK) return st;
+  }
+  linear_fp8_kernel<RT, F, KB><<<grid, waves * 64, lds, s>>>(a);
   return launch_status();
+}
+
+// The largest block of rows and features that leaves three workgroups for every
+// four compute units: a block of RT x F tiles reads x and W 1 / F and 1 / RT as
+// often, but below that the idle compute units cost more.  Measured, block for
+// block: 40 x 2048 x 16384 9.1 us with 3 x 4 (256 workgroups), 10.2 with 3 x 2,
+// 11 with 1 x 2; 40 x 8192 x 2048 9.3 us with 1 x 2 (192), 11.8 with 1 x 1, 20
+// with 3 x 2 (64); 20 x 2048 x 2048 3.7 us with 1 x 1 (256), 4.0 with 1 x 2.
+inline int launch_few_rows(const Lin8Args &a, hipStream_t s) {
+  const int64_t tiles = (a.N + 15) / 16, rt = (a.M + 15) / 16;
+  const int cus = cu_count();
+  if (cus == 0) return SPECDEC_EHIP;
+  const auto enough = [&](int r, int f) { return (tiles + f - 1) / f * ((rt + r - 1) / r) * 4 >= 3 * cus; };
+  if (rt == 3) {
+    if (enough(3, 4)) return launch_lin8<3, 4, 2>(a, s);
+    if (enough(3, 2)) return launch_lin8<3, 2, 2>(a, s);
+  } else if (rt > 1) {
+    if (rt > 2 && enough(4, 4)) return launch_lin8<4, 4, 2>(a, s);
+    if (enough(2, 4)) return launch_lin8<2, 4, 2>(a, s);
+    if (enough(2, 2)) return launch_lin8<2, 2, 4>(a, s);
+  }
+  if (enough(1, 2)) return launch_lin8<1, 2, 4>(a, s);
+  return launch_lin8<1, 1, 4>(a, s);
 }
 
 // ---------------------------------------------------------------- many rows --
@@ -561,8 +626,5 @@ SPECDEC_API int specdec_linear_fp8(const void *x, int64_t x_stride, const void *
   hipStream_t s = as_stream(stream);
   if (rows > 512 && tile8_fits<Tile8<8, 8, 2, 2>>(a)) return launch_tile8<8, 8, 2, 2>(a, s);
   if (rows > 64 && tile8_fits<Tile8<4, 4, 2, 2>>(a)) return launch_tile8<4, 4, 2, 2>(a, s);
-  if (rows <= 16) return launch_lin8<1, 4>(a, s);
-  if (rows <= 32) return launch_lin8<2, 4>(a, s);
-  if (rows <= 48) return launch_lin8<3, 2>(a, s);
-  return launch_lin8<4, 2>(a, s);
+  return launch_few_rows(a, s);
 }
