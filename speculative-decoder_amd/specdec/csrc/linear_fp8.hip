@@ -236,21 +236,28 @@ inline int launch_few_rows(const Lin8Args &a, hipStream_t s) {
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
 
 // The tile kernel's shape: WM x WN waves of 16 TR rows x 16 TF features, and
-// its LDS: three slots of half of the features x 128 inputs, three of the rows
-// x 128 inputs, two of 16 groups' scales; the waves' output rows (padded by 16
+// its LDS: kSlotsW slots of half of the features x 128 inputs, SX of the rows x
+// 128 inputs, two of 16 groups' scales; the waves' output rows (padded by 16
 // bytes so that neither the 8-byte writes down a column of rows nor the 16-byte
 // reads along a row meet in a bank) take their place at the end.
-constexpr int kTileSlots = 3;
-template <int TR, int TF, int WM, int WN> struct Tile8 {
-  static_assert(WM * WN == 4 && TF % TR == 0 && TF >= 4 && TR % 2 == 0, "");
+template <int TR, int TF, int WM, int WN, int SX> struct Tile8 {
+  static_assert(WM * WN == 4 && TF % TR == 0 && TF >= 4 && TR % 2 == 0 && SX >= 3, "");
+  static constexpr int kTR = TR, kTF = TF, kWM = WM, kWN = WN, kSlotsX = SX;
+  // a step's rows are asked for 2 SX - 3 turns before they are read, features as
+  // many at most
+  static constexpr int kAhead = SX == 3 ? 2 : 2 * SX - 3, kSlotsW = kAhead + 1;
   static constexpr int kRows = 16 * TR * WM, kFeatures = 16 * TF * WN;
   static constexpr int kW = kFeatures * 64, kX = kRows * 128, kScales = (kRows + kFeatures) * 16;
-  static constexpr int kXAt = kTileSlots * kW, kScalesAt = kXAt + kTileSlots * kX;
+  static constexpr int kXAt = kSlotsW * kW, kScalesAt = kXAt + SX * kX;
   static constexpr int kPitch = 32 * TF + 16;
   static constexpr int kRings = kScalesAt + 2 * kScales, kOut = 4 * 16 * TR * kPitch;
   static constexpr int kLds = kRings > kOut ? kRings : kOut;
   static constexpr int kLoadsW = kW / 4096, kLoadsX = kX / 8192;  // a wave's loads of a turn
-  static_assert(kLds <= 160 * 1024, "");
+  // behind the first turn's rows and features
+  static constexpr int kFirst = kLoadsW * (kSlotsW - 1) + kLoadsX * (2 * SX - 3);
+  static_assert(kFirst < 64, "");
+  static constexpr int kPerCu = 160 * 1024 / kLds;
+  static_assert(kPerCu >= 1, "");
 };
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t from_corner(const uint8_t *base) {
@@ -312,10 +319,11 @@ template <int TF> __device__ __forceinline__ void settle(f32x4 (&acc)[TF]) {
 // half of a wave's features with all its rows; its operands are in registers
 // when it starts, the next turn's are read from LDS and later ones asked for
 // between its products, so one barrier a turn is the only wait.
-template <int TR, int TF, int WM, int WN, bool ADD>
-__global__ __launch_bounds__(256, 1) void linear_fp8_tile_kernel(Lin8Args a, int tiles_m, int tiles_n) {
+template <typename L, bool ADD>
+__global__ __launch_bounds__(256, L::kPerCu > 2 ? 2 : L::kPerCu) void linear_fp8_tile_kernel(Lin8Args a, int tiles_m,
+                                                                                             int tiles_n) {
   extern __shared__ __align__(1024) uint8_t s_ring[];
-  using L = Tile8<TR, TF, WM, WN>;
+  constexpr int TR = L::kTR, TF = L::kTF, WN = L::kWN;
   constexpr int kHalf = TF / 2;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
@@ -424,8 +432,8 @@ __global__ __launch_bounds__(256, 1) void linear_fp8_tile_kernel(Lin8Args a, int
     const uint8_t *src = s_ring + slot * L::kX + x_at + i * 2048;
     fx[i] = join8(*reinterpret_cast<const u32x4 *>(src + x_c0), *reinterpret_cast<const u32x4 *>(src + x_c1));
   };
-  auto after = [](int slot) { return slot == kTileSlots - 1 ? 0 : slot + 1; };
-  auto before = [](int slot) { return slot == 0 ? kTileSlots - 1 : slot - 1; };
+  const auto after = [](int slot, int slots) { return slot == slots - 1 ? 0 : slot + 1; };
+  const auto before = [](int slot, int slots) { return slot == 0 ? slots - 1 : slot - 1; };
   int ws = 0, xs = 0;  // slots of the current turn's features and step's rows
   // Turn (s, H): half H of the features in step s, whose scales are byte K of
   // the words.  The wait and barrier before it: this wave's loads for the reads
@@ -438,8 +446,8 @@ __global__ __launch_bounds__(256, 1) void linear_fp8_tile_kernel(Lin8Args a, int
   auto turn = [&](int s, auto k, auto half) {
     constexpr int K = decltype(k)::value, H = decltype(half)::value;
     constexpr int kLoads = L::kLoadsW + L::kLoadsX;
-    wait_meet<kLoads>();
-    const int ws_next = after(ws), xs_next = after(xs);
+    wait_meet<kLoads *(L::kAhead - 1)>();
+    const int ws_next = after(ws, L::kSlotsW), xs_next = after(xs, L::kSlotsX);
 #pragma unroll
     for (int i = 0; i < TR; ++i) {
 #pragma unroll
@@ -455,11 +463,12 @@ __global__ __launch_bounds__(256, 1) void linear_fp8_tile_kernel(Lin8Args a, int
           for (int l = i * kLoads / TR; l < (i + 1) * kLoads / TR; ++l) {
             if (l < L::kLoadsX) {
               if (H == 1)
-                fetch_x(xs, s + kTileSlots, l);
+                fetch_x(xs, s + L::kSlotsX, l);
               else
-                fetch_x(before(xs), s - 1 + kTileSlots, L::kLoadsX + l);
+                fetch_x(before(xs, L::kSlotsX), s - 1 + L::kSlotsX, L::kLoadsX + l);
             } else {
-              fetch_w(ws, s + 1 + (H == 1), 1 - H, l - L::kLoadsX);
+              constexpr int A = H + L::kSlotsW;  // halves from the step's first on
+              fetch_w(ws, s + A / 2, A & 1, l - L::kLoadsX);
             }
           }
         }
@@ -474,25 +483,31 @@ __global__ __launch_bounds__(256, 1) void linear_fp8_tile_kernel(Lin8Args a, int
     turn(s, k, std::integral_constant<int, 0>());
     turn(s, k, std::integral_constant<int, 1>());
   };
-  // The first loads, in the order in which the turns need them: turns (0, 0) and
-  // (0, 1) find all but the last kLoadsW + kLoadsX of them landed, and the
-  // second half of step 2's rows is asked for in turn (0, 0).
+  // The first loads, as the turns before the first would have asked for them:
+  // turn -j for features j before slot kSlotsW's, all others before those.
   load_scales(0);
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (int i = 0; i < 2 * L::kLoadsX; ++i) fetch_x(0, 0, i);
 #pragma unroll
-  for (int q = 0; q < 2; ++q)
+  for (int i = 0; i < L::kLoadsW; ++i) fetch_w(0, 0, 0, i);
 #pragma unroll
-    for (int i = 0; i < L::kLoadsW; ++i) fetch_w(q, 0, q, i);
+  for (int i = 0; i < L::kLoadsW; ++i) fetch_w(1, 0, 1, i);
 #pragma unroll
-  for (int i = 0; i < 2 * L::kLoadsX; ++i) fetch_x(1, 1, i);
+  for (int q = 2 - 2 * L::kSlotsX; q < 0; ++q) {  // the turn that would ask for part (q + 1) & 1 of a step's rows
+    const int xstep = (q - ((q & 1) ? 1 : 2)) / 2 + L::kSlotsX, piece = q + L::kSlotsW;
+    if (xstep >= 1) {
 #pragma unroll
-  for (int i = 0; i < L::kLoadsW; ++i) fetch_w(2, 1, 0, i);
+      for (int i = 0; i < L::kLoadsX; ++i) fetch_x(xstep, xstep, (q & 1 ? 0 : L::kLoadsX) + i);
+    }
+    if (piece >= 2) {
 #pragma unroll
-  for (int i = 0; i < L::kLoadsX; ++i) fetch_x(2, 2, i);
+      for (int i = 0; i < L::kLoadsW; ++i) fetch_w(piece, piece / 2, piece & 1, i);
+    }
+  }
   store_scales(0);
-  wait_meet<2 * L::kLoadsW + 3 * L::kLoadsX>();
+  // rows and features of the first turn: everything but what follows W's second half
+  wait_meet<L::kFirst>();
 #pragma unroll
   for (int t = 0; t < kHalf; ++t) read_w(0, 0, t);
 #pragma unroll
@@ -580,24 +595,61 @@ template <typename L> bool tile8_fits(const Lin8Args &a) {
   return a.x_stride <= 0x7FFFFFFF / (L::kRows + 1) && (int64_t)a.steps * 2048 <= 0x7FFFFFFF / (L::kFeatures / 16 + 1);
 }
 
-template <int TR, int TF, int WM, int WN, bool ADD> int launch_tile8_as(const Lin8Args &a, hipStream_t s) {
-  using L = Tile8<TR, TF, WM, WN>;
+template <typename L, bool ADD> int launch_tile8_as(const Lin8Args &a, hipStream_t s) {
   static bool ready[64];
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return SPECDEC_EHIP;
   if (!ready[dev]) {
-    if (hipFuncSetAttribute((const void *)linear_fp8_tile_kernel<TR, TF, WM, WN, ADD>,
-                            hipFuncAttributeMaxDynamicSharedMemorySize, L::kLds) != hipSuccess)
-      return SPECDEC_EHIP;
+    const int st = allow_lds(linear_fp8_tile_kernel<L, ADD>, L::kLds);
+    if (st != SPECDEC_OK) return st;
     ready[dev] = true;
   }
   const int tm = (int)((a.M + L::kRows - 1) / L::kRows), tn = (a.N + L::kFeatures - 1) / L::kFeatures;
-  linear_fp8_tile_kernel<TR, TF, WM, WN, ADD><<<tm * tn, 256, L::kLds, s>>>(a, tm, tn);
+  linear_fp8_tile_kernel<L, ADD><<<tm * tn, 256, L::kLds, s>>>(a, tm, tn);
   return launch_status();
 }
 
-template <int TR, int TF, int WM, int WN> int launch_tile8(const Lin8Args &a, hipStream_t s) {
-  return a.add ? launch_tile8_as<TR, TF, WM, WN, true>(a, s) : launch_tile8_as<TR, TF, WM, WN, false>(a, s);
+template <typename L> int launch_tile8(const Lin8Args &a, hipStream_t s) {
+  return a.add ? launch_tile8_as<L, true>(a, s) : launch_tile8_as<L, false>(a, s);
+}
+
+// More than 64 rows: blocks of the few-row kernel where there are few of them,
+// else the tile that a simple account of its time makes the fastest.
+//   A tile shape takes, for each round of as many workgroups as the card holds,
+//   a start and end and so much a step of 128 inputs (measured, us, 2048 inputs
+//   unless said):
+//                         workgroups          start + end, a step
+//     64 x 128            1 a compute unit    2.4, 0.28   64..256 workgroups 7.5..8.2 (8192 inputs 19.9..22.5), 768 21
+//     128 x 128, 7 slots  1                   2.4, 0.43   128..256 10.2..11.9 (28..31.5)
+//     128 x 128, 3 slots  2                   2.0, 0.95   512 19.5, 4096 136
+//     256 x 256           1                   6.0, 1.43   256 31.7 (98), 1024 117
+//   which gets 65 x 2048 x 16384 (8.5 us, 12 with 128 x 128), 2048 x 8192 x 2048
+//   (31.5, 42 with 64 x 128), 4096 x 2048 x 2048 (19.4, 24.5 and 27 with the
+//   smallest and largest) and 4096 x 2048 x 16384 (117, 136 with 128 x 128) right.
+//   The few-row kernel, with up to one block of 32 x 32 a compute unit: 65 x 2048
+//   x 2048 5.2 us (tiles 7.3), 128 x 8192 x 2048 13.2 (18.8), 200 x 1536 x 576 3.7
+//   (7.0); with more, 288 x 2048 x 2048 9.7 (7.6), 100 x 2048 x 6144 9.6 (7.7).
+inline int launch_many_rows(const Lin8Args &a, hipStream_t s) {
+  using Small = Tile8<2, 4, 2, 2, 4>;
+  using Deep = Tile8<4, 4, 2, 2, 4>;
+  using Pair = Tile8<4, 4, 2, 2, 3>;
+  using Large = Tile8<8, 8, 2, 2, 3>;
+  const int64_t cus = cu_count();
+  if (cus == 0) return SPECDEC_EHIP;
+  const auto blocks = [&](int64_t rows, int64_t features) {
+    return (a.M + rows - 1) / rows * ((a.N + features - 1) / features);
+  };
+  if (!tile8_fits<Large>(a) || blocks(32, 32) * 4 <= 5 * cus) return launch_few_rows(a, s);
+  const auto cost = [&](int64_t tiles, int64_t at_once, float ends, float step) {
+    return (float)((tiles + at_once - 1) / at_once) * (ends + step * (float)a.steps);
+  };
+  const float small = cost(blocks(64, 128), cus, 2.4f, 0.28f), deep = cost(blocks(128, 128), cus, 2.4f, 0.43f);
+  const float pair = cost(blocks(128, 128), 2 * cus, 2.0f, 0.95f), large = cost(blocks(256, 256), cus, 6.0f, 1.43f);
+  const float least = std::min(std::min(small, deep), std::min(pair, large));
+  if (large == least) return launch_tile8<Large>(a, s);
+  if (pair == least) return launch_tile8<Pair>(a, s);
+  if (deep == least) return launch_tile8<Deep>(a, s);
+  return launch_tile8<Small>(a, s);
 }
 
 }  // namespace specdec
@@ -624,7 +676,5 @@ SPECDEC_API int specdec_linear_fp8(const void *x, int64_t x_stride, const void *
              (const uint8_t *)w_scales, (uint16_t *)out, out_stride, (const uint16_t *)add, add_stride, rows,
              (int)out_features, (int)steps, 0};
   hipStream_t s = as_stream(stream);
-  if (rows > 512 && tile8_fits<Tile8<8, 8, 2, 2>>(a)) return launch_tile8<8, 8, 2, 2>(a, s);
-  if (rows > 64 && tile8_fits<Tile8<4, 4, 2, 2>>(a)) return launch_tile8<4, 4, 2, 2>(a, s);
-  return launch_few_rows(a, s);
+  return rows > 64 ? launch_many_rows(a, s) : launch_few_rows(a, s);
 }
