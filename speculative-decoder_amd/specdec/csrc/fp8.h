@@ -23,12 +23,6 @@ inline __host__ __device__ int64_t fp8_scale_cols(int64_t k) { return (k + 4 * k
 
 constexpr unsigned kFp8ScaleOne = 127;  // the padding's scale
 
-// |y|'s bits, 0 for infinities and NaN
-__device__ __forceinline__ unsigned fp8_finite_bits(float y) {
-  const unsigned b = __float_as_uint(y) & 0x7FFFFFFFu;
-  return b < 0x7F800000u ? b : 0u;
-}
-
 // The scale byte of a group whose largest finite |y| has the bits `amax`:
 // with |y| = 1.f 2^E and 448 = 1.75 2^8, the least e is E - 8, or E - 7 where
 // 1.f > 1.75.
@@ -51,12 +45,12 @@ __device__ __forceinline__ unsigned fp8_pack4(float a, float b, float c, float d
   return (unsigned)p;
 }
 
-// The largest of v over each row of 16 lanes, in every lane of the row.
-__device__ __forceinline__ unsigned row16_max(unsigned v) {
-  v = max(v, (unsigned)dpp_move<0xB1>((int)v));
-  v = max(v, (unsigned)dpp_move<0x4E>((int)v));
-  v = max(v, (unsigned)dpp_move<0x141>((int)v));
-  return max(v, (unsigned)dpp_move<0x140>((int)v));
+// The largest of v >= 0 over each row of 16 lanes, in every lane of the row.
+__device__ __forceinline__ float row16_max(float v) {
+  v = dpp_max_step<0xB1>(v);
+  v = dpp_max_step<0x4E>(v);
+  v = dpp_max_step<0x141>(v);
+  return dpp_max_step<0x140>(v);
 }
 
 }  // namespace specdec

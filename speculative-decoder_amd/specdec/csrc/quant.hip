@@ -3,15 +3,18 @@
 // projection, and from the MLP's SiLU(gate) * up.
 //
 // All values stay in fp32 up to the one rounding to 8 bits; the format has
-// nothing to gain from bf16 steps in between.  These kernels move bytes: a
-// thread takes 8 consecutive values, the 16 lanes of a DPP row make a group,
-// so the group's maximum is four lane moves and no memory, and a wave's loads
-// and stores are contiguous.  Rows of any width and stride: the loads need no
-// alignment (bf16 rows of odd width start at odd addresses; the memory path
-// takes a 16-byte load at any), only a row's last values are read one by one.
+// nothing to gain from bf16 steps in between.  These kernels move bytes, at what
+// a large copy does (5.2 TB/s) or near it: quantize 4096 x 2048 in bf16 5.3 us,
+// 4.7 TB/s; SiLU 3001 x 8192 in bf16 26.1 us, 4.7 TB/s.  A thread takes 8
+// consecutive values and the 16 lanes of a DPP row make a group, so a group's
+// maximum is four lane moves and no memory, and a wave's loads and stores are
+// contiguous.  Rows of any width and stride: the loads need no alignment (bf16
+// rows of odd width start at odd addresses; the memory path takes a 16-byte load
+// at any), only a row's last values are read one by one.
 #include "fp8.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace specdec {
 
@@ -35,13 +38,18 @@ template <typename T> __device__ __forceinline__ void load8(const T *row, int64_
 }
 
 // The codes and scale of the group that the calling 16 lanes hold: lane r of
-// them (0 .. 15) has the values 8 r .. 8 r + 7.  `last`: the row's last group,
-// whose lanes also write the padding scales behind it.
+// them (0 .. 15) has the values 8 r .. 8 r + 7.  `pad`: scales behind this one
+// that the row's last group also writes.
 __device__ __forceinline__ void store_group(const float (&y)[kPer], int r, uint8_t *codes, uint8_t *scale, int pad) {
-  unsigned m = 0;
+  float m = 0.0f;  // fmaxf leaves NaN out; infinities, which are rare, are left out by a second look
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) m = max(m, fp8_finite_bits(y[j]));
-  const unsigned byte = fp8_scale_byte(row16_max(m));
+  for (int j = 0; j < kPer; ++j) m = fmaxf(m, fabsf(y[j]));
+  if (__any(m == INFINITY)) {
+    m = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) m = fmaxf(m, fabsf(y[j]) == INFINITY ? 0.0f : fabsf(y[j]));
+  }
+  const unsigned byte = fp8_scale_byte(__float_as_uint(row16_max(m)));
   const float inv = fp8_inverse(byte);
   const uint2 c = make_uint2(fp8_pack4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv),
                              fp8_pack4(y[4] * inv, y[5] * inv, y[6] * inv, y[7] * inv));
@@ -49,10 +57,26 @@ __device__ __forceinline__ void store_group(const float (&y)[kPer], int r, uint8
   if (r <= pad) scale[r] = (uint8_t)(r == 0 ? byte : kFp8ScaleOne);
 }
 
-// SiLU(g) * u in fp32: g / (1 + e^-g) * u, each step rounded on its own.
+// SiLU(g) * u = g / (1 + e^-g) * u in fp32, as exactly as with a library's exp
+// and a division (each about half a unit) and in half of their instructions,
+// which would take longer than the rows' bytes (3001 x 8192 in bf16: 31.2 us
+// with them).  e^-g is 2^t on the hardware's exp2, t = -g log2 e in two parts of
+// which the small one is applied after; the quotient is g times the hardware's
+// reciprocal with one correction by its remainder.  Gates are taken as at least
+// -88.5 (e^-g still finite; the value there is below 4e-37); infinite ones give
+// NaN, as -inf / inf does, through 0 * g.
 __device__ __forceinline__ float silu_mul_f32(float g, float u) {
 #pragma clang fp contract(off)
-  return g / (1.0f + expf(-g)) * u;
+  constexpr float kLog2e = 1.44269502f, kLog2eLow = 1.92596303e-8f, kLn2 = 0.693147182f;
+  const float x = __builtin_amdgcn_fmed3f(g, -88.5f, 88.5f), top = fmaxf(g, -88.5f);
+  const float t = -x * kLog2e;
+  const float low = fmaf(-x, kLog2eLow, fmaf(-x, kLog2e, -t));
+  const float e0 = __builtin_amdgcn_exp2f(t);
+  const float d = 1.0f + fmaf(e0, low * kLn2, e0);
+  const float r = __builtin_amdgcn_rcpf(d);
+  const float s0 = top * r;
+  const float s = fmaf(fmaf(-d, s0, top), r, s0);
+  return fmaf(0.0f, g, s) * u;
 }
 
 // One group for every 16 lanes; SILU: rows hold gate then up, `dim` each.
@@ -79,43 +103,48 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_kernel(const T *__rest
   store_group(y, r, codes + row * cols + (int64_t)grp * kFp8Group, scales + row * gcols + grp, pad);
 }
 
-// One workgroup a row, CH groups of every 16 lanes in registers (dim <= 2048
-// CH).  summed = round(hidden + delta), or hidden alone without delta; then
-// y = summed * rsqrt(mean(summed^2) + eps) * weight in fp32.  The row's sum is
-// taken in an order that dim alone fixes, so a row has the same bits whatever
-// rows come with it.
-constexpr int kNormMaxCh = 8;
+// LANES threads a row (several rows a workgroup below 256), CH groups of every
+// 16 lanes in registers (dim <= 8 CH LANES).  summed = round(hidden + delta), or
+// hidden alone without delta; then y = summed * rsqrt(mean(summed^2) + eps) *
+// weight in fp32.  The row's sum is taken in an order that dim alone fixes, so a
+// row has the same bits whatever rows come with it.
+// One group of 8 values a thread and a whole row at once, as far as a workgroup
+// reaches: a row's time is one round trip to memory and one sum.  4096 x 2048 in
+// bf16 with the sum written 12.1 us (4.8 TB/s, what a large copy does is 5.2;
+// 128 threads with two groups 13.0, 64 with four 13.2), one row 2.8 us (3.5, 4.7).
+constexpr int kNormMaxLanes = 1024, kNormMaxCh = 2;
 
-template <typename T, int CH>
-__global__ __launch_bounds__(kQuantThreads) void add_rmsnorm_quant_kernel(
-    const T *hidden, const T *__restrict__ delta, const T *__restrict__ weight, T *summed, int64_t dim, float eps,
-    unsigned groups, uint8_t *codes, uint8_t *scales) {
+template <typename T, int CH, int LANES>
+__global__ __launch_bounds__(LANES < kQuantThreads ? kQuantThreads : LANES) void add_rmsnorm_quant_kernel(
+    const T *hidden, const T *__restrict__ delta, const T *__restrict__ weight, T *summed, int64_t rows, int64_t dim,
+    float eps, unsigned groups, uint8_t *codes, uint8_t *scales) {
 #pragma clang fp contract(off)
-  __shared__ float red[kQuantThreads / kWave];
-  const int64_t row = blockIdx.x;
-  const int tid = threadIdx.x, r = tid & 15, lanes = blockDim.x;
-  const T *h = hidden + row * dim;
+  constexpr int kThreads = LANES < kQuantThreads ? kQuantThreads : LANES;
+  __shared__ float red[kThreads / kWave];
+  const int64_t row = (int64_t)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
+  const int tid = threadIdx.x % LANES, r = tid & 15;
+  if (LANES <= kWave && row >= rows) return;  // whole waves, and no barrier below
+  const int64_t at = min(row, rows - 1) * dim;
+  const T *h = hidden + at;
   float y[CH][kPer];
-  float ss = 0.0f;
 #pragma unroll
-  for (int k = 0; k < CH; ++k) {
-    const int64_t i = (int64_t)kPer * (tid + k * lanes);
-    load8(h, i, dim, y[k]);
-  }
+  for (int k = 0; k < CH; ++k) load8(h, (int64_t)kPer * (tid + k * LANES), dim, y[k]);
   if (delta) {
-    const T *dl = delta + row * dim;
-    T *out = summed + row * dim;
+    const T *dl = delta + at;
+    T *out = summed + at;
+    float d[CH][kPer];
+#pragma unroll
+    for (int k = 0; k < CH; ++k) load8(dl, (int64_t)kPer * (tid + k * LANES), dim, d[k]);
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
-      const int64_t i = (int64_t)kPer * (tid + k * lanes);
-      float d[kPer];
-      load8(dl, i, dim, d);
+      const int64_t i = (int64_t)kPer * (tid + k * LANES);
       Eight<T> s;
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
-        s.v[j] = from_f32<T>(y[k][j] + d[j]);
+        s.v[j] = from_f32<T>(y[k][j] + d[k][j]);
         y[k][j] = to_f32(s.v[j]);
       }
+      if (row >= rows) continue;
       if (i + kPer <= dim) {
         __builtin_memcpy(out + i, &s, sizeof(s));
       } else {
@@ -123,21 +152,26 @@ __global__ __launch_bounds__(kQuantThreads) void add_rmsnorm_quant_kernel(
       }
     }
   }
+  float ss = 0.0f;
 #pragma unroll
   for (int k = 0; k < CH; ++k)
 #pragma unroll
     for (int j = 0; j < kPer; ++j) ss += y[k][j] * y[k][j];
   ss = wave_sum_dpp(ss);
-  if ((tid & (kWave - 1)) == 0) red[tid / kWave] = ss;
-  __syncthreads();
-  ss = red[0];
-  for (int w = 1; w < lanes / kWave; ++w) ss += red[w];
+  if constexpr (LANES > kWave) {
+    const int first = threadIdx.x / LANES * (LANES / kWave);
+    if ((tid & (kWave - 1)) == 0) red[threadIdx.x / kWave] = ss;
+    __syncthreads();
+    ss = red[first];
+#pragma unroll
+    for (int w = 1; w < LANES / kWave; ++w) ss += red[first + w];
+  }
   const float inv = rsqrtf(ss / (float)dim + eps);
   const int64_t cols = (int64_t)groups * kFp8Group, gcols = fp8_scale_cols(dim);
 #pragma unroll
   for (int k = 0; k < CH; ++k) {
-    const unsigned grp = (unsigned)(tid + k * lanes) >> 4;
-    if (grp >= groups) break;  // whole rows of 16 lanes
+    const unsigned grp = (unsigned)(tid + k * LANES) >> 4;
+    if (grp >= groups || row >= rows) break;  // whole rows of 16 lanes
     const int64_t i = (int64_t)grp * kFp8Group + kPer * r;
     float w[kPer];
     load8(weight, i, dim, w);
@@ -168,23 +202,36 @@ int launch_quantize(const void *x, int64_t rows, int64_t dim, int64_t stride, ui
   return launch_status();
 }
 
+template <typename T, int CH, int LANES>
+void launch_add_rmsnorm_as(const void *hidden, const void *delta, const void *weight, void *summed, int64_t rows,
+                           int64_t dim, float eps, uint8_t *codes, uint8_t *scales, hipStream_t s) {
+  constexpr int threads = LANES < kQuantThreads ? kQuantThreads : LANES, at_once = threads / LANES;
+  add_rmsnorm_quant_kernel<T, CH, LANES><<<(unsigned)((rows + at_once - 1) / at_once), threads, 0, s>>>(
+      (const T *)hidden, (const T *)delta, (const T *)weight, (T *)summed, rows, dim, eps,
+      (unsigned)((dim + kFp8Group - 1) / kFp8Group), codes, scales);
+}
+
 template <typename T>
 int launch_add_rmsnorm_quant(const void *hidden, const void *delta, const void *weight, void *summed, int64_t rows,
                              int64_t dim, float eps, uint8_t *codes, uint8_t *scales, hipStream_t s) {
-  const unsigned groups = (unsigned)((dim + kFp8Group - 1) / kFp8Group);
-  const unsigned chunks = groups * 16;  // threads that hold one chunk each
-  const dim3 grid((unsigned)rows), block(std::min<unsigned>((chunks + kWave - 1) / kWave * kWave, kQuantThreads));
-  const unsigned ch = (chunks + block.x - 1) / block.x;
-  const T *h = (const T *)hidden, *d = (const T *)delta, *w = (const T *)weight;
-  T *o = (T *)summed;
-  if (ch <= 1)
-    add_rmsnorm_quant_kernel<T, 1><<<grid, block, 0, s>>>(h, d, w, o, dim, eps, groups, codes, scales);
-  else if (ch <= 2)
-    add_rmsnorm_quant_kernel<T, 2><<<grid, block, 0, s>>>(h, d, w, o, dim, eps, groups, codes, scales);
-  else if (ch <= 4)
-    add_rmsnorm_quant_kernel<T, 4><<<grid, block, 0, s>>>(h, d, w, o, dim, eps, groups, codes, scales);
+  const auto run = [&](auto ch, auto lanes) {
+    launch_add_rmsnorm_as<T, decltype(ch)::value, decltype(lanes)::value>(hidden, delta, weight, summed, rows, dim, eps,
+                                                                          codes, scales, s);
+  };
+  using std::integral_constant;
+  const integral_constant<int, 1> one;
+  if (dim <= 512)
+    run(one, integral_constant<int, 64>());
+  else if (dim <= 1024)
+    run(one, integral_constant<int, 128>());
+  else if (dim <= 2048)
+    run(one, integral_constant<int, 256>());
+  else if (dim <= 4096)
+    run(one, integral_constant<int, 512>());
+  else if (dim <= 8192)
+    run(one, integral_constant<int, kNormMaxLanes>());
   else
-    add_rmsnorm_quant_kernel<T, kNormMaxCh><<<grid, block, 0, s>>>(h, d, w, o, dim, eps, groups, codes, scales);
+    run(integral_constant<int, kNormMaxCh>(), integral_constant<int, kNormMaxLanes>());
   return launch_status();
 }
 
@@ -225,7 +272,7 @@ SPECDEC_API int specdec_add_rmsnorm_fp8(const void *hidden, const void *delta, c
                                         void *stream) {
   if (rows < 0 || dim <= 0) return SPECDEC_EINVAL;
   if (dtype != SPECDEC_BF16 && dtype != SPECDEC_F32) return SPECDEC_EINVAL;
-  if (dim > (int64_t)kQuantThreads * kPer * kNormMaxCh || rows > INT32_MAX) return SPECDEC_EUNSUPPORTED;
+  if (dim > (int64_t)kNormMaxLanes * kPer * kNormMaxCh || rows > INT32_MAX) return SPECDEC_EUNSUPPORTED;
   if (rows == 0) return SPECDEC_OK;
   if (!hidden || !weight || (delta && !summed) || !quant_out_ok(codes, scales)) return SPECDEC_EINVAL;
   uint8_t *c = (uint8_t *)codes, *sc = (uint8_t *)scales;
