@@ -22,7 +22,8 @@ A forward is split in two:
     then the final norm and the fp32 output projection (lm/forward.py:71-84).
     The norm weights live in the projections' columns (lm/model.py:Layer).
     Prefill (more than 16 new tokens) and fp32 models normalise in a kernel
-    of their own instead, without the weight.
+    of their own instead, without the weight.  A model with 8-bit projections
+    (Llama.fp8) runs its layers in `_fp8_layers`.
 The device part reads everything it needs from device memory, so a fixed
 (batch, width) shape can be captured once in a HIP graph and replayed
 (lm/graphs.py).
@@ -139,6 +140,9 @@ def forward_core(llama: Llama, cache: KVCache, meta: torch.Tensor, ids: torch.Te
     tables = cache.table_tensor
     layers = llama.layers
     hidden = F.embedding(ids, llama.embed)
+    if llama.is_fp8:
+        x = _fp8_layers(llama, cache, meta, hidden, max_kv_len, workspace, split_tokens)
+        return _project_out(llama, x, last, temperature, out, index_out)
     x = torch.empty_like(hidden)
     # the attention finishes the input norm for decode-sized calls; else a
     # weightless norm kernel writes x and the projection reads that
@@ -177,12 +181,49 @@ def forward_core(llama: Llama, cache: KVCache, meta: torch.Tensor, ids: torch.Te
             _project_add(hidden, act, layer.wd, gemv, layer.wd_t)
         else:
             ops.add_rmsnorm(hidden, _project(act, layer.wd, gemv, layer.wd_t), llama.unit_norm, x, eps)
+    return _project_out(llama, x, last, temperature, out, index_out)
+
+
+def _project_out(llama: Llama, x: torch.Tensor, last: torch.Tensor | None, temperature: float | None,
+                 out: torch.Tensor | None, index_out: torch.Tensor | None) -> torch.Tensor:
+    """Logits, or with a temperature probabilities, of the normed rows x [B,
+    T, hidden], or of each entry's row `last`."""
     if last is not None:
+        b, t, _ = x.shape
         # last is in [0, t): with one token per row it selects that token, a view
         x = x[:, 0] if t == 1 else x[torch.arange(b, device=x.device), last]
     if temperature is None:
         return logits(llama, x)
     return probabilities(llama, x, temperature, out, index_out)
+
+
+def _fp8_layers(llama: Llama, cache: KVCache, meta: torch.Tensor, hidden: torch.Tensor, max_kv_len: int,
+                workspace: ops.AttentionWorkspace | None, split_tokens: int) -> torch.Tensor:
+    """The decoder layers of a model with 8-bit projections over hidden [B, T,
+    hidden], and the final norm.  Nine launches a layer: each projection reads
+    rows in 8 bits that the norm before it, the attention's output or the MLP's
+    activation was written as, and o_proj and down add into the residual stream
+    inside their rounding.  With at most 64 rows a row's bits do not depend on
+    the other rows, as in the bf16 path, so a verify decides as plain decoding
+    would."""
+    cfg = llama.config
+    b, t, _ = hidden.shape
+    h, hk, d, eps = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim, cfg.rms_norm_eps
+    tables, ones = cache.table_tensor, llama.unit_norm
+    attn = torch.empty(b, t, h * d, dtype=hidden.dtype, device=hidden.device)
+    x = ops.add_rmsnorm_fp8(hidden, None, ones, eps)
+    for i, layer in enumerate(llama.layers):
+        qkv = ops.linear_fp8(*x, *layer.wqkv)
+        ops.rope_paged_attention(qkv, llama.rope_cos, llama.rope_sin, cache.k[i], cache.v[i], tables, meta, b, t, h, hk,
+                                 d, cache.block_size, llama.scaling, max_kv_len, attn, attn.stride(1), workspace,
+                                 split_tokens)
+        ops.linear_fp8(*ops.quantize_fp8(attn), *layer.wo, out=hidden, add=hidden)
+        gate_up = ops.linear_fp8(*ops.add_rmsnorm_fp8(hidden, None, ones, eps), *layer.wgu)
+        act = ops.silu_mul_fp8(gate_up)
+        if i + 1 == len(llama.layers):
+            return ops.add_rmsnorm(hidden, ops.linear_fp8(*act, *layer.wd), llama.norm, torch.empty_like(hidden), eps)
+        ops.linear_fp8(*act, *layer.wd, out=hidden, add=hidden)
+        x = ops.add_rmsnorm_fp8(hidden, None, ones, eps)
 
 
 @torch.no_grad()

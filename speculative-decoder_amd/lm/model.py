@@ -13,7 +13,7 @@ inv_freq in fp32, then cos and sin), and kept in fp32 on the device.
 """
 from __future__ import annotations
 
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 
 import torch
 
@@ -138,6 +138,25 @@ class Layer:
             self.wqkv_t, self.wo_t, self.wgu_t, self.wd_t = (tiled(w) for w in (self.wqkv, self.wo, self.wgu, self.wd))
 
 
+@dataclass
+class Fp8Layer:
+    """One decoder layer whose projections are held and multiplied in 8 bits:
+    each weight as (codes, scales), the codes tiled (ops.tile_weight_fp8), a
+    scale for each 128 inputs of a feature.  The norm weights are folded into
+    wqkv and wgu as in Layer, so the norms before them run without weights."""
+    wqkv: tuple[torch.Tensor, torch.Tensor]
+    wo: tuple[torch.Tensor, torch.Tensor]
+    wgu: tuple[torch.Tensor, torch.Tensor]
+    wd: tuple[torch.Tensor, torch.Tensor]
+
+    @classmethod
+    def from_layer(cls, layer: Layer) -> "Fp8Layer":
+        def quantized(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+            codes, scales = ops.quantize_fp8(w)
+            return ops.tile_weight_fp8(codes), scales
+        return cls(*(quantized(w) for w in (layer.wqkv, layer.wo, layer.wgu, layer.wd)))
+
+
 def fold_norm(w: torch.Tensor, ln: torch.Tensor) -> torch.Tensor:
     """W diag(ln): the norm weight multiplied into W's columns, in fp32 or
     wider, then rounded once to W's dtype."""
@@ -149,7 +168,7 @@ def fold_norm(w: torch.Tensor, ln: torch.Tensor) -> torch.Tensor:
 class Llama:
     config: LlamaShape
     embed: torch.Tensor
-    layers: list[Layer]
+    layers: list[Layer] | list[Fp8Layer]
     norm: torch.Tensor
     lm_head: torch.Tensor
     # lm_head as the output projection reads it: bf16/fp16 weights on the GPU
@@ -173,6 +192,25 @@ class Llama:
     @property
     def dtype(self) -> torch.dtype:
         return self.embed.dtype
+
+    @property
+    def is_fp8(self) -> bool:
+        return bool(self.layers) and isinstance(self.layers[0], Fp8Layer)
+
+    def fp8(self) -> "Llama":
+        """This model with every layer's projections in 8 bits (weights, and
+        the rows they are multiplied with): half of the layers' weight bytes
+        and, on prompts, products at twice the bf16 rate.  The residual
+        stream, attention and K/V cache, the embeddings, the final norm and
+        the head stay as they are (the last three are shared with this
+        model).  For bf16 models on a GPU; logits differ from the bf16 model's
+        by the rounding of weights and activations to e4m3."""
+        if self.is_fp8:
+            return self
+        if self.dtype != torch.bfloat16 or self.device.type != "cuda":
+            raise NotImplementedError(f"8-bit projections are made of bf16 weights on a GPU (got {self.dtype} on "
+                                      f"{self.device})")
+        return replace(self, layers=[Fp8Layer.from_layer(layer) for layer in self.layers])
 
     @property
     def scaling(self) -> float:
