@@ -423,31 +423,41 @@ def fp8_scale_cols(k: int) -> int:
     return -(-k // (4 * FP8_GROUP)) * 4
 
 
-def _launch(dev: torch.device, entry, *args) -> int:
-    """`entry` on the current stream of `dev`, which need not be the current device."""
-    if _device_index is None or _device_index() == dev.index:
-        return entry(*args, stream())
-    with torch.cuda.device(dev):
-        return entry(*args, stream())
+def _launch(index: int, entry, *args) -> int:
+    """`entry` on the current stream of device `index`, which need not be the current one."""
+    if _raw_stream is None or _device_index is None:
+        with torch.cuda.device(index):
+            return entry(*args, stream())
+    if _device_index() == index:
+        return entry(*args, _raw_stream(index))
+    with torch.cuda.device(index):
+        return entry(*args, _raw_stream(index))
+
+
+def _rows_empty(dev: torch.device, lead, cols: int, dtype: torch.dtype) -> torch.Tensor:
+    """An empty contiguous [*lead, cols] (for the usual [rows, cols] by the call
+    that takes the host the least: 1.3 us where torch.empty takes 1.7)."""
+    if len(lead) == 1:
+        return torch.empty_strided((lead[0], cols), (cols, 1), dtype=dtype, device=dev)
+    return torch.empty((*lead, cols), dtype=dtype, device=dev)
 
 
 def _fp8_rows(dev: torch.device, lead, k: int, codes: torch.Tensor | None, scales: torch.Tensor | None):
     """codes [*lead, Kp] and scales [*lead, Gp] of rows of k values: given and checked, or new."""
-    cshape, sshape = (*lead, -(-k // 128) * 128), (*lead, -(-k // 512) * 4)
     if codes is None:
-        codes = torch.empty(cshape, dtype=FP8_CODE, device=dev)
+        codes = _rows_empty(dev, lead, -(-k // 128) * 128, FP8_CODE)
     else:
-        _fp8_given(dev, codes, cshape, FP8_CODE, 16, "codes")
+        _fp8_given(dev, codes, (*lead, -(-k // 128) * 128), FP8_CODE, 16, "codes")
     if scales is None:
-        scales = torch.empty(sshape, dtype=FP8_SCALE, device=dev)
+        scales = _rows_empty(dev, lead, -(-k // 512) * 4, FP8_SCALE)
     else:
-        _fp8_given(dev, scales, sshape, FP8_SCALE, 4, "scales")
+        _fp8_given(dev, scales, (*lead, -(-k // 512) * 4), FP8_SCALE, 4, "scales")
     return codes, scales
 
 
 def _fp8_given(dev: torch.device, t: torch.Tensor, shape, dtype: torch.dtype, align: int, name: str) -> None:
     _on(dev, t, name, dtype, True)
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)} (got {list(t.shape)})")
     if t.data_ptr() % align:
         raise ValueError(f"{name} must be {align}-byte aligned")
@@ -464,9 +474,10 @@ def _fp8_input(x: torch.Tensor, name: str) -> tuple[torch.Tensor, int, int, int,
     dt = _FP8_INPUTS.get(x.dtype)
     if dt is None:
         raise TypeError(f"{name} must be bf16 or fp32 (got {x.dtype})")
-    if x.dim() < 1 or x.shape[-1] == 0:
-        raise ValueError(f"{name} needs rows of at least one value (got {list(x.shape)})")
-    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    shape = x.shape
+    if not shape or shape[-1] == 0:
+        raise ValueError(f"{name} needs rows of at least one value (got {list(shape)})")
+    x2 = x if len(shape) == 2 else x.reshape(-1, shape[-1])
     rows, k = x2.shape
     stride, inner = x2.stride()
     if inner != 1 and k > 1 or rows > 1 and stride < k:  # transposed, or overlapping rows
@@ -486,7 +497,7 @@ def quantize_fp8(x: torch.Tensor, codes: torch.Tensor | None = None, scales: tor
     x2, dt, rows, k, stride = _fp8_input(x, "x")
     dev = x.device
     codes, scales = _fp8_rows(dev, x.shape[:-1], k, codes, scales)
-    st = _launch(dev, lib().specdec_quantize_fp8, x2.data_ptr(), dt, rows, k, stride, codes.data_ptr(),
+    st = _launch(dev.index, lib().specdec_quantize_fp8, x2.data_ptr(), dt, rows, k, stride, codes.data_ptr(),
                  scales.data_ptr())
     if st:
         _check(st, "quantize_fp8")
@@ -501,7 +512,7 @@ def silu_mul_fp8(gate_up: torch.Tensor, codes: torch.Tensor | None = None, scale
         raise ValueError(f"gate_up rows hold gate then up, an even number of values (got {two})")
     dev = gate_up.device
     codes, scales = _fp8_rows(dev, gate_up.shape[:-1], two // 2, codes, scales)
-    st = _launch(dev, lib().specdec_silu_mul_fp8, x2.data_ptr(), dt, rows, two // 2, stride, codes.data_ptr(),
+    st = _launch(dev.index, lib().specdec_silu_mul_fp8, x2.data_ptr(), dt, rows, two // 2, stride, codes.data_ptr(),
                  scales.data_ptr())
     if st:
         _check(st, "silu_mul_fp8")
@@ -535,7 +546,7 @@ def add_rmsnorm_fp8(hidden: torch.Tensor, delta: torch.Tensor | None, weight: to
     elif summed is not None:
         raise ValueError("summed is written where there is a delta only")
     codes, scales = _fp8_rows(dev, shape[:-1], dim, codes, scales)
-    st = _launch(dev, lib().specdec_add_rmsnorm_fp8, hidden.data_ptr(), delta_ptr, weight.data_ptr(), summed_ptr, dt,
+    st = _launch(dev.index, lib().specdec_add_rmsnorm_fp8, hidden.data_ptr(), delta_ptr, weight.data_ptr(), summed_ptr, dt,
                  count // dim, dim, eps, codes.data_ptr(), scales.data_ptr())
     if st:
         _check(st, "add_rmsnorm_fp8")
@@ -571,51 +582,56 @@ def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scale
     of at most 64 rows give a row the same bits whatever rows come with it."""
     if not w.is_cuda:
         gpu(w, "w")
-    dev, wshape = w.device, w.shape
-    if w.dtype != FP8_CODE or len(wshape) != 5 or wshape[2:] != (2, 64, 16) or not w.is_contiguous():
+    index, dev, wshape = w.get_device(), w.device, w.shape
+    if w.dtype is not FP8_CODE or len(wshape) != 5 or wshape[2:] != (2, 64, 16) or not w.is_contiguous():
         raise ValueError("w must be a tile_weight_fp8() result")
-    kp, gp = wshape[1] * 128, -(-wshape[1] // 4) * 4
-    _on(dev, w_scales, "w_scales", FP8_SCALE, True)
-    n = w_scales.shape[0]
-    if w_scales.dim() != 2 or w_scales.shape[1] != gp or -(-n // 16) != wshape[0]:
-        raise ValueError(f"w_scales must be [N, {gp}] with N in {16 * wshape[0] - 15} .. {16 * wshape[0]} "
-                         f"(got {list(w_scales.shape)})")
-    _on(dev, x, "x", FP8_CODE)
-    _on(dev, x_scales, "x_scales", FP8_SCALE)
-    lead = x.shape[:-1]
-    if x.shape[-1:] != (kp,) or x_scales.shape != (*lead, gp):
-        raise ValueError(f"x must be [..., {kp}] and x_scales [..., {gp}] "
-                         f"(got {list(x.shape)} and {list(x_scales.shape)})")
-    x2, x_ptr, x_stride = _fp8_operand(x, kp, 16)
-    rows = x2.shape[0]
-    s2, s_ptr, s_stride = _fp8_operand(x_scales, gp, 4)
+    tiles, groups = wshape[:2]
+    kp, gp = groups * 128, -(-groups // 4) * 4
+    if (w_scales.get_device() != index or w_scales.dtype is not FP8_SCALE or not w_scales.is_contiguous()
+            or x.get_device() != index or x.dtype is not FP8_CODE or x_scales.get_device() != index
+            or x_scales.dtype is not FP8_SCALE):
+        _on(dev, w_scales, "w_scales", FP8_SCALE, True)
+        _on(dev, x, "x", FP8_CODE)
+        _on(dev, x_scales, "x_scales", FP8_SCALE)
+    ws_shape, shape = w_scales.shape, x.shape
+    n = ws_shape[0] if len(ws_shape) == 2 else 0
+    if -(-n // 16) != tiles or ws_shape[1] != gp:
+        raise ValueError(f"w_scales must be [N, {gp}] with N in {16 * tiles - 15} .. {16 * tiles} "
+                         f"(got {list(ws_shape)})")
+    lead = shape[:-1]
+    if not shape or shape[-1] != kp or x_scales.shape != (*lead, gp):
+        raise ValueError(f"x must be [..., {kp}] and x_scales [..., {gp}] (got {list(shape)} and "
+                         f"{list(x_scales.shape)})")
+    x2, rows, x_ptr, x_stride = _fp8_operand(x, kp, 16)
+    s2, _, s_ptr, s_stride = _fp8_operand(x_scales, gp, 4)
     if add is None:
         add_ptr, add_stride = None, 0
     else:
         add_ptr, add_stride = _fp8_output(dev, add, rows, n, "add")
     if out is None:
-        result = torch.empty((*lead, n), dtype=torch.bfloat16, device=dev)
-        out_ptr, out_stride = result.data_ptr(), n
+        out = _rows_empty(dev, lead, n, torch.bfloat16)
+        out_ptr, out_stride = out.data_ptr(), n
     else:
-        result = out
         out_ptr, out_stride = _fp8_output(dev, out, rows, n, "out")
-    st = _launch(dev, lib().specdec_linear_fp8, x_ptr, x_stride, s_ptr, s_stride, w.data_ptr(), w_scales.data_ptr(),
+    st = _launch(index, lib().specdec_linear_fp8, x_ptr, x_stride, s_ptr, s_stride, w.data_ptr(), w_scales.data_ptr(),
                  rows, kp, n, add_ptr, add_stride, out_ptr, out_stride)
     if st:
         _check(st, "linear_fp8")
-    return result
+    return out
 
 
-def _fp8_operand(t: torch.Tensor, cols: int, align: int) -> tuple[torch.Tensor, int, int]:
+def _fp8_operand(t: torch.Tensor, cols: int, align: int) -> tuple[torch.Tensor, int, int, int]:
     """t [..., cols] of one-byte elements as rows whose starts are aligned: the
-    tensor that holds them, its address and its rows' stride."""
+    tensor that holds them, their number, address and stride."""
     t2 = t if t.dim() == 2 else t.reshape(-1, cols)
+    rows, address = t2.shape[0], t2.data_ptr()
     stride, inner = t2.stride()
-    if t2.shape[0] <= 1:  # a single row's stride means nothing
+    if rows <= 1:  # a single row's stride means nothing
         stride = cols
-    if inner != 1 or stride < cols or stride % align or t2.data_ptr() % align:
-        t2, stride = t2.clone(memory_format=torch.contiguous_format), cols
-    return t2, t2.data_ptr(), stride
+    if inner != 1 or stride < cols or stride % align or address % align:
+        t2 = t2.clone(memory_format=torch.contiguous_format)
+        address, stride = t2.data_ptr(), cols
+    return t2, rows, address, stride
 
 
 def _fp8_output(dev: torch.device, t: torch.Tensor, rows: int, n: int, name: str) -> tuple[int, int]:
