@@ -507,7 +507,8 @@ int specdec_add_rmsnorm_fp8(const void *hidden, const void *delta, const void *w
  * [out_features, 4 ceil(in_codes / 512)].  add (null for none) bf16, rows
  * add_stride apart; it may be out itself and may not overlap it otherwise.
  * Calls of at most 64 rows give a row the same bits whatever rows come with
- * it. */
+ * it.  At most 1048560 rows, 2^24 features, 2^23 inputs and strides of x and
+ * x_scales of 2^25 (else SPECDEC_EUNSUPPORTED). */
 int specdec_linear_fp8(const void *x, int64_t x_stride, const void *x_scales, int64_t x_scale_stride,
                        const void *w, const void *w_scales, int64_t rows, int64_t in_codes,
                        int64_t out_features, const void *add, int64_t add_stride, void *out,

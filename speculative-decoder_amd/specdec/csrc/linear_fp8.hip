@@ -18,6 +18,11 @@ typedef __attribute__((ext_vector_type(8))) int i32x8;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef __attribute__((ext_vector_type(2))) unsigned int u32x2;
 
+// What the kernels' 32-bit indexes reach: 16-row blocks of a grid's second
+// dimension, offsets of 64 rows.
+constexpr int64_t kLin8MaxRows = 65535 * 16, kLin8MaxFeatures = 1 << 24, kLin8MaxSteps = 1 << 16;
+constexpr int64_t kLin8MaxStride = 1 << 25;
+
 struct Lin8Args {
   const uint8_t *x;  // codes [M, x_stride], 128 `steps` of each row used
   int64_t x_stride;
@@ -44,10 +49,16 @@ __device__ __forceinline__ f32x4 mfma8(i32x8 a, i32x8 b, f32x4 c, unsigned sa, u
 }
 
 // More than 64 KB of LDS has to be allowed for, once a kernel and device.
-template <typename K> int allow_lds(K kernel, int bytes) {
-  return hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess
-             ? SPECDEC_OK
-             : SPECDEC_EHIP;
+template <auto Kernel> int allow_lds(int bytes) {
+  static bool ready[64];
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return SPECDEC_EHIP;
+  if (!ready[dev]) {
+    if (hipFuncSetAttribute((const void *)Kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
+      return SPECDEC_EHIP;
+    ready[dev] = true;
+  }
+  return SPECDEC_OK;
 }
 
 // ----------------------------------------------------------------- few rows --
@@ -202,7 +213,7 @@ template <int RT, int F, int KB> int launch_lin8(Lin8Args a, hipStream_t s) {
   const int waves = (a.steps + a.per_wave - 1) / a.per_wave, lds = waves * RT * F * 1024;
   const dim3 grid((unsigned)((tiles + F - 1) / F), (unsigned)((a.M + 16 * RT - 1) / (16 * RT)));
   if (lds > 65536) {
-    const int st = allow_lds((const void *)linear_fp8_kernel<RT, F, KB>, kLin8MaxWaves * RT * F * 1024);
+    const int st = allow_lds<linear_fp8_kernel<RT, F, KB>>(kLin8MaxWaves * RT * F * 1024);
     if (st != SPECDEC_OK) return st;
   }
   linear_fp8_kernel<RT, F, KB><<<grid, waves * 64, lds, s>>>(a);
@@ -299,13 +310,15 @@ __device__ __forceinline__ void product(f32x4 &acc, const i32x8 &w, const i32x8 
     asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[1,1,0] op_sel_hi:[1,1,0]"
                  : "+a"(acc) : "v"(w), "v"(x), "v"(sw), "v"(sx));
 }
-// Between writes to sums or operands by other instructions and the first
-// product, and between the last product and what reads a sum: the products that
-// are still in the unit end first (at most 18 cycles' wait is asked for).
-template <int TF> __device__ __forceinline__ void settle(f32x4 (&acc)[TF]) {
+// Behind the last product, before sums are read: what is still in the unit ends
+// first (at most 18 cycles are asked for).
+template <int TR, int TF> __device__ __forceinline__ void settle(f32x4 (&acc)[TR][TF]) {
+  asm volatile("s_nop 15\n\ts_nop 15");
 #pragma unroll
-  for (int j = 0; j < TF; j += 4)
-    asm volatile("s_nop 15\n\ts_nop 15" : "+a"(acc[j]), "+a"(acc[j + 1]), "+a"(acc[j + 2]), "+a"(acc[j + 3]));
+  for (int i = 0; i < TR; ++i)
+#pragma unroll
+    for (int j = 0; j < TF; j += 4)
+      asm volatile("" : "+a"(acc[i][j]), "+a"(acc[i][j + 1]), "+a"(acc[i][j + 2]), "+a"(acc[i][j + 3]));
 }
 
 // A tile of kRows x kFeatures a workgroup, on v_mfma_scale_f32_16x16x128_f8f6f4
@@ -534,8 +547,7 @@ __global__ __launch_bounds__(256, L::kPerCu > 2 ? 2 : L::kPerCu) void linear_fp8
   }
   // every load has landed and every wave is through with the rings
   wait_meet<0>();
-#pragma unroll
-  for (int i = 0; i < TR; ++i) settle(acc[i]);
+  settle(acc);
   // this lane's features of its rows to LDS, whole rows back
   uint8_t *mine = s_ring + wave * 16 * TR * L::kPitch;
   const int fbase = n0 + wn * TF * 16;
@@ -564,6 +576,7 @@ __global__ __launch_bounds__(256, L::kPerCu > 2 ? 2 : L::kPerCu) void linear_fp8
           u32x2{__builtin_bit_cast(unsigned, lo), __builtin_bit_cast(unsigned, hi)};
     }
   }
+  asm volatile("" ::: "memory");  // a wave reads its own rows, and its LDS accesses are done in order
   constexpr int kLanes = 2 * TF, kAtOnce = 64 / kLanes;  // lanes of a row, rows of an instruction
   const int rr0 = lane / kLanes, f0 = (lane % kLanes) * 8;
   const uint8_t *back = mine + rr0 * L::kPitch + f0 * 2;
@@ -596,14 +609,8 @@ template <typename L> bool tile8_fits(const Lin8Args &a) {
 }
 
 template <typename L, bool ADD> int launch_tile8_as(const Lin8Args &a, hipStream_t s) {
-  static bool ready[64];
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return SPECDEC_EHIP;
-  if (!ready[dev]) {
-    const int st = allow_lds(linear_fp8_tile_kernel<L, ADD>, L::kLds);
-    if (st != SPECDEC_OK) return st;
-    ready[dev] = true;
-  }
+  const int st = allow_lds<linear_fp8_tile_kernel<L, ADD>>(L::kLds);
+  if (st != SPECDEC_OK) return st;
   const int tm = (int)((a.M + L::kRows - 1) / L::kRows), tn = (a.N + L::kFeatures - 1) / L::kFeatures;
   linear_fp8_tile_kernel<L, ADD><<<tm * tn, 256, L::kLds, s>>>(a, tm, tn);
   return launch_status();
@@ -665,8 +672,8 @@ SPECDEC_API int specdec_linear_fp8(const void *x, int64_t x_stride, const void *
   if (rows > 1 && (x_stride < in_codes || x_scale_stride < scale_cols || out_stride < out_features ||
                    (add && add_stride < out_features)))
     return SPECDEC_EINVAL;
-  if (out_features > (int64_t)1 << 24 || steps > (int64_t)1 << 16 || rows > (int64_t)1 << 20)
-    return SPECDEC_EUNSUPPORTED;
+  if (out_features > kLin8MaxFeatures || steps > kLin8MaxSteps || rows > kLin8MaxRows) return SPECDEC_EUNSUPPORTED;
+  if (rows > 1 && (x_stride > kLin8MaxStride || x_scale_stride > kLin8MaxStride)) return SPECDEC_EUNSUPPORTED;
   if (rows == 0) return SPECDEC_OK;
   if (!x || !x_scales || !w || !w_scales || !out) return SPECDEC_EINVAL;
   if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)x_stride) & 15) return SPECDEC_EINVAL;

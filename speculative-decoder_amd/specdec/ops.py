@@ -525,7 +525,8 @@ def add_rmsnorm_fp8(hidden: torch.Tensor, delta: torch.Tensor | None, weight: to
     """h = hidden + delta (if given, rounded to hidden's type and written to
     `summed`, else back to hidden), then quantize_fp8(h * rsqrt(mean(h^2) +
     eps) * weight), the norm in fp32 with the one rounding to 8 bits.  hidden,
-    delta and summed [..., D] contiguous, bf16 or fp32, D <= 16384."""
+    delta and summed [..., D] contiguous, bf16 or fp32, D <= 16384; summed may
+    be hidden or delta itself, but not overlap them otherwise."""
     if not hidden.is_cuda:
         gpu(hidden, "hidden")
     dev, dtype = hidden.device, hidden.dtype
@@ -578,8 +579,9 @@ def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scale
     as quantize_fp8, add_rmsnorm_fp8 and silu_mul_fp8 give them) and an 8-bit
     weight (w = tile_weight_fp8 of its codes, w_scales [N, Gp]) transposed,
     accumulated in fp32 and rounded once: bf16 [..., N].  With `add` (bf16,
-    [..., N]; it may be `out`) out = x @ w.T + add inside that rounding.  Calls
-    of at most 64 rows give a row the same bits whatever rows come with it."""
+    [..., N]; it may be `out` itself, but not overlap it otherwise) out = x @
+    w.T + add inside that rounding.  Calls of at most 64 rows give a row the
+    same bits whatever rows come with it."""
     if not w.is_cuda:
         gpu(w, "w")
     index, dev, wshape = w.get_device(), w.device, w.shape
@@ -628,7 +630,7 @@ def _fp8_operand(t: torch.Tensor, cols: int, align: int) -> tuple[torch.Tensor, 
     stride, inner = t2.stride()
     if rows <= 1:  # a single row's stride means nothing
         stride = cols
-    if inner != 1 or stride < cols or stride % align or address % align:
+    if inner != 1 or stride < cols or stride % align or stride > 1 << 25 or address % align:
         t2 = t2.clone(memory_format=torch.contiguous_format)
         address, stride = t2.data_ptr(), cols
     return t2, rows, address, stride

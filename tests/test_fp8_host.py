@@ -72,4 +72,14 @@ def test_c_entries_check_their_arguments_before_launch():
     assert mm(xst=240) == 1 and mm(xsst=2) == 1 and mm(outst=47) == 1 and mm(add=fake, addst=47) == 1
     assert mm(xst=264) == 1 and mm(x=fake + 8) == 1 and mm(w=fake + 4) == 1 and mm(xs=fake + 1) == 1
     assert mm(x=None) == 1 and mm(out=None) == 1 and mm(ws=None) == 1
-    assert mm(rows=1 << 21, ) == 3 and mm(nf=1 << 25, outst=1 << 25) == 3
+    assert mm(rows=1048561) == 3 and mm(nf=1 << 25, outst=1 << 25) == 3
+    assert mm(xst=(1 << 25) + 16) == 3 and mm(xsst=(1 << 25) + 4) == 3 and mm(k=1 << 24, xst=1 << 24, xsst=1 << 17) == 3
+
+
+def test_models_off_the_gpu_or_in_fp32_have_no_8_bit_form():
+    from lm.model import Llama, LlamaShape
+
+    shape = LlamaShape(vocab_size=32, hidden_size=64, num_hidden_layers=1, num_attention_heads=1, num_key_value_heads=1,
+                       intermediate_size=64)
+    with pytest.raises(NotImplementedError):
+        Llama.random(shape, 0, "cpu").fp8()

@@ -375,6 +375,21 @@ def test_linear_fp8_strided_operands(rows):
     assert three.shape == (rows, 3, n)
 
 
+def test_linear_fp8_rows_far_apart():
+    """Rows 2^26 bytes apart (their offsets pass 32 bits) are copied first; 2^25
+    are read in place."""
+    w, ws = weight(0.05 * rows_of(40, 128, 1))
+    x, xs = ops.quantize_fp8(rows_of(70, 128, 2).to(DEV))
+    want = ops.linear_fp8(x, xs, w, ws)
+    for log in (25, 26):
+        far = torch.empty((69 << log) + 128, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn)
+        view = far.as_strided((70, 128), (1 << log, 1))
+        view.copy_(x)
+        assert torch.equal(ops.linear_fp8(view, xs, w, ws), want)
+        assert torch.equal(ops.linear_fp8(view[:64], xs[:64], w, ws), ops.linear_fp8(x[:64], xs[:64], w, ws))
+        del far, view
+
+
 @pytest.mark.parametrize("rows", [3, 80, 300])
 def test_linear_fp8_carries_nan(rows):
     """A NaN in a row makes that row NaN and no other; one in a weight's row that feature."""
@@ -465,6 +480,37 @@ def test_graph_replays_and_side_streams(rows):
             other = mlp(x, d, ln, gu, down)
         torch.cuda.current_stream().wait_stream(side)
         assert torch.equal(other, eager), i
+
+
+def test_first_call_inside_a_capture():
+    """Kernels that need more than 64 KB of LDS, called for the first time while a
+    stream is captured (in a process of its own)."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = """
+import torch
+from specdec import ops
+cases = []
+for rows, k, n in ((64, 8192, 16384), (100, 1300, 3001), (1000, 520, 2100), (1000, 600, 4500), (1990, 600, 8170)):
+    x, xs = ops.quantize_fp8(torch.randn(rows, k, device="cuda"))
+    wc, ws = ops.quantize_fp8(torch.randn(n, k, device="cuda"))
+    cases.append((x, xs, ops.tile_weight_fp8(wc), ws))
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    outs = [ops.linear_fp8(*c) for c in cases]
+for i in range(3):
+    for o in outs:
+        o.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, ops.linear_fp8(*c)) for o, c in zip(outs, cases)), i
+print("captured")
+"""
+    pkg = Path(__file__).resolve().parents[1] / "speculative-decoder_amd"
+    out = subprocess.run([sys.executable, "-c", code], cwd=pkg, capture_output=True, text=True, timeout=100)
+    assert out.returncode == 0 and "captured" in out.stdout, out.stderr[-2000:]
 
 
 def test_refusals():
