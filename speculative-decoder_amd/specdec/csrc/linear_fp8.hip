@@ -61,13 +61,22 @@ template <auto Kernel> int allow_lds(int bytes) {
   return SPECDEC_OK;
 }
 
+// At most N of this wave's loads still on their way and none of its LDS
+// accesses, and every wave of the workgroup here; no memory access moves across.
+template <int N> __device__ __forceinline__ void wait_meet() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x70);
+  asm volatile("s_barrier" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 // ----------------------------------------------------------------- few rows --
 constexpr int kLin8MaxWaves = 8;
 
 // The steps of a wave: a power of two (so that four steps' scales are in one
-// word), at most 16 waves a feature tile and, where that leaves enough of them,
-// 16 waves a compute unit.  Of the weight's sizes alone: the order of a row's
-// sums does not depend on the other rows of the call.
+// word), at most four waves while a wave has fewer than four steps, then at most
+// eight.  Of the weight's sizes alone: the order of a row's sums does not depend
+// on the other rows of the call.
 inline int lin8_steps_per_wave(int steps) {
   int per = 1;
   while (per < 4 ? (steps + per - 1) / per > 4 : (steps + per - 1) / per > kLin8MaxWaves) per *= 2;
@@ -82,15 +91,26 @@ __device__ __forceinline__ u32x4 from_partner(u32x4 v) {
   return r;
 }
 
+// The words of a row's scales that are worth LDS: see launch_lin8.
+constexpr int kLin8LeastWords = 15, kLin8MostWords = 62;
+
+__device__ __forceinline__ const __attribute__((address_space(1))) void *to_global(const uint8_t *p) {
+  return (const __attribute__((address_space(1))) void *)p;
+}
+__device__ __forceinline__ __attribute__((address_space(3))) void *to_lds(unsigned *p) {
+  return (__attribute__((address_space(3))) void *)p;
+}
+
 // 16 RT rows and F feature tiles a workgroup; the waves split the steps and
 // their sums are added in wave order.  A wave asks for KB steps of W and x at
-// once and there are up to 16 waves of up to 128 registers, so x, which every
+// once and there are up to 8 waves of up to 256 registers, so x, which every
 // workgroup reads, comes from L2 straight to registers.  What bounds that is
 // the cache lines the memory path looks up (about three cycles each), so one
 // load takes eight whole lines, 128 inputs of eight rows: lanes c < 8 of each 16
 // take the first halves of rows c, then c + 8, lanes c >= 8 the second halves of
 // rows c - 8, then c, and partners exchange what is not their row's.
-template <int RT, int F, int KB> __global__ __launch_bounds__(kLin8MaxWaves * 64) void linear_fp8_kernel(Lin8Args a) {
+template <int RT, int F, int KB, bool STAGED>
+__global__ __launch_bounds__(kLin8MaxWaves * 64) void linear_fp8_kernel(Lin8Args a) {
   extern __shared__ f32x4 s_acc[];  // [wave][RT][F][64]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
   const int c = lane & 15, g = lane >> 4;
@@ -127,6 +147,20 @@ template <int RT, int F, int KB> __global__ __launch_bounds__(kLin8MaxWaves * 64
       pre[i] = a.add[(m0 + min(row, m_last)) * a.add_stride + min(f0 + i, a.N - 1)];
   };
   if (a.add && wave < RT * F) load_add(wave);
+  // the scales, a load a row: [F feature tiles, RT row tiles][16][words + 1]
+  const int words = ws_stride / 4;
+  unsigned *s_scales = reinterpret_cast<unsigned *>(s_acc + nw * RT * F * 64);
+  if constexpr (STAGED) {
+    if (lane < words) {
+      for (int r = wave; r < 16 * (F + RT); r += nw) {
+        const uint8_t *row = r < 16 * F ? wsb + (unsigned)(min(n0 + r, a.N - 1) - n0) * ws_stride
+                                        : xsb + (unsigned)min(r - 16 * F, m_last) * (unsigned)a.xs_stride;
+        __builtin_amdgcn_global_load_lds(to_global(row + 4 * lane), to_lds(s_scales + r * (words + 1)), 4, 0, 0);
+      }
+    }
+    asm volatile("" ::: "memory");  // the loads below come behind these
+    __builtin_amdgcn_sched_barrier(0);
+  }
   f32x4 acc[RT][F];
 #pragma unroll
   for (int t = 0; t < RT; ++t)
@@ -135,10 +169,12 @@ template <int RT, int F, int KB> __global__ __launch_bounds__(kLin8MaxWaves * 64
   for (int s4 = s_lo; s4 < s_hi; s4 += 4) {  // the steps of a word of scales
     const int word = s4 & ~3;
     unsigned sa[F], sb[RT];
+    if constexpr (!STAGED) {
 #pragma unroll
-    for (int f = 0; f < F; ++f) sa[f] = *reinterpret_cast<const unsigned *>(wsb + word + wsoff[f]);
+      for (int f = 0; f < F; ++f) sa[f] = *reinterpret_cast<const unsigned *>(wsb + word + wsoff[f]);
 #pragma unroll
-    for (int t = 0; t < RT; ++t) sb[t] = *reinterpret_cast<const unsigned *>(xsb + word + xsoff[t]);
+      for (int t = 0; t < RT; ++t) sb[t] = *reinterpret_cast<const unsigned *>(xsb + word + xsoff[t]);
+    }
     const int end = min(s4 + 4, s_hi);
 #pragma unroll
     for (int h = 0; h < 4; h += KB) {
@@ -160,6 +196,15 @@ template <int RT, int F, int KB> __global__ __launch_bounds__(kLin8MaxWaves * 64
             for (int e = 0; e < 2; ++e) X[j][t][e] = *reinterpret_cast<const u32x4 *>(xs + xoff[t][e]);
         }
         __builtin_amdgcn_sched_barrier(0);  // all of them before the first product
+        if (STAGED && h == 0) {
+          // once a wave, and each has a step: its first batch stays on its way
+          if (s4 == s_lo) wait_meet<KB * 2 * (F + RT)>();
+          const unsigned *at = s_scales + c * (words + 1) + (s4 >> 2);
+#pragma unroll
+          for (int f = 0; f < F; ++f) sa[f] = at[16 * f * (words + 1)];
+#pragma unroll
+          for (int t = 0; t < RT; ++t) sb[t] = at[16 * (F + t) * (words + 1)];
+        }
 #pragma unroll
         for (int j = 0; j < KB; ++j) {
           const int s = s4 + h + j;
@@ -207,17 +252,32 @@ template <int RT, int F, int KB> __global__ __launch_bounds__(kLin8MaxWaves * 64
   }
 }
 
-template <int RT, int F, int KB> int launch_lin8(Lin8Args a, hipStream_t s) {
-  const int tiles = (a.N + 15) / 16;
-  a.per_wave = lin8_steps_per_wave(a.steps);
-  const int waves = (a.steps + a.per_wave - 1) / a.per_wave, lds = waves * RT * F * 1024;
-  const dim3 grid((unsigned)((tiles + F - 1) / F), (unsigned)((a.M + 16 * RT - 1) / (16 * RT)));
+template <int RT, int F, int KB, bool STAGED> int launch_lin8(const Lin8Args &a, int waves, hipStream_t s) {
+  constexpr int kScaleRows = STAGED ? 16 * (RT + F) * 4 : 0;
+  constexpr int kMost = kLin8MaxWaves * RT * F * 1024 + kScaleRows * (kLin8MostWords + 1);
+  static_assert(kMost <= 160 * 1024 && KB * 2 * (F + RT) < 64, "");
+  const int lds = waves * RT * F * 1024 + kScaleRows * ((a.steps + 3) / 4 + 1);
+  const dim3 grid((unsigned)(((a.N + 15) / 16 + F - 1) / F), (unsigned)((a.M + 16 * RT - 1) / (16 * RT)));
   if (lds > 65536) {
-    const int st = allow_lds<linear_fp8_kernel<RT, F, KB>>(kLin8MaxWaves * RT * F * 1024);
+    const int st = allow_lds<linear_fp8_kernel<RT, F, KB, STAGED>>(kMost);
     if (st != SPECDEC_OK) return st;
   }
-  linear_fp8_kernel<RT, F, KB><<<grid, waves * 64, lds, s>>>(a);
+  linear_fp8_kernel<RT, F, KB, STAGED><<<grid, waves * 64, lds, s>>>(a);
   return launch_status();
+}
+
+// Every wave looks up the lines of its rows' scales; where there are many rows
+// and many words a row, the workgroup brings them to LDS once instead.
+// 40 x 8192 x 2048 (16 words a row) 9.3 us -> 8.45, 40 x 16384 x 2048 16.3 ->
+// 14.3, 5 x 8192 x 2048 6.2 -> 6.1, but 1 x 8192 x 2048 5.45 -> 5.6 and
+// 1 x 12288 x 2048 6.45 -> 6.9; 40 x 6144 x 2048 7.3 -> 7.25 and 16 x 7168 x 2048
+// 6.75 -> 6.85 gain nothing and 40 x 5120 x 2048 6.2 -> 6.75 loses.
+template <int RT, int F, int KB> int launch_lin8(Lin8Args a, hipStream_t s) {
+  a.per_wave = lin8_steps_per_wave(a.steps);
+  const int waves = (a.steps + a.per_wave - 1) / a.per_wave, words = (a.steps + 3) / 4;
+  if (a.M > 4 && words >= kLin8LeastWords && words <= kLin8MostWords)
+    return launch_lin8<RT, F, KB, true>(a, waves, s);
+  return launch_lin8<RT, F, KB, false>(a, waves, s);
 }
 
 // The largest block of rows and features that leaves three workgroups for every
@@ -279,15 +339,6 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t from_corner(const uint8_t *bas
 // `off` of the resource go to dst + 16 l.
 __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t from, uint8_t *dst, int lane_off, int off) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void *)dst, 16, lane_off, off, 0, 0);
-}
-
-// At most N of this wave's loads still on their way and none of its LDS
-// accesses, and every wave of the workgroup here; no memory access moves across.
-template <int N> __device__ __forceinline__ void wait_meet() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x70);
-  asm volatile("s_barrier" ::: "memory");
-  __builtin_amdgcn_sched_barrier(0);
 }
 
 // acc += w x, the operands scaled by byte K of sw and sx.  In assembly so that
