@@ -295,27 +295,37 @@ template <int RT, int F, int KB> int launch_lin8(Lin8Args a, hipStream_t s) {
   return launch_lin8<RT, F, KB, false>(a, waves, s);
 }
 
-// The largest block of rows and features that leaves three workgroups for every
-// four compute units: a block of RT x F tiles reads x and W 1 / F and 1 / RT as
-// often, but below that the idle compute units cost more.  Measured, block for
-// block: 40 x 2048 x 16384 9.1 us with 3 x 4 (256 workgroups), 10.2 with 3 x 2,
-// 11 with 1 x 2; 40 x 8192 x 2048 9.3 us with 1 x 2 (192), 11.8 with 1 x 1, 20
-// with 3 x 2 (64); 20 x 2048 x 2048 3.7 us with 1 x 1 (256), 4.0 with 1 x 2.
-inline int launch_few_rows(const Lin8Args &a, hipStream_t s) {
-  const int64_t tiles = (a.N + 15) / 16, rt = (a.M + 15) / 16;
-  const int cus = cu_count();
-  if (cus == 0) return SPECDEC_EHIP;
-  const auto enough = [&](int r, int f) { return (tiles + f - 1) / f * ((rt + r - 1) / r) * 4 >= 3 * cus; };
-  if (rt == 3) {
-    if (enough(3, 4)) return launch_lin8<3, 4, 2>(a, s);
-    if (enough(3, 2)) return launch_lin8<3, 2, 2>(a, s);
-  } else if (rt > 1) {
-    if (rt > 2 && enough(4, 4)) return launch_lin8<4, 4, 2>(a, s);
-    if (enough(2, 4)) return launch_lin8<2, 4, 2>(a, s);
-    if (enough(2, 2)) return launch_lin8<2, 2, 4>(a, s);
-  }
-  if (enough(1, 2)) return launch_lin8<1, 2, 4>(a, s);
-  return launch_lin8<1, 1, 4>(a, s);
+// The blocks of RT x F tiles, and how long a step of the fullest compute unit's
+// take: 9 a tile of rows, whose lines lie in rows apart and whose halves are
+// exchanged, and 4 a tile of features.
+template <int RT, int F> inline int64_t few_cost(const Lin8Args &a, int64_t cus) {
+  const int64_t blocks = (a.M + 16 * RT - 1) / (16 * RT) * ((a.N + 16 * F - 1) / (16 * F));
+  return (blocks + cus - 1) / cus * (9 * RT + 4 * F);
+}
+
+struct FewRows {
+  int (*launch)(Lin8Args, hipStream_t);
+  int64_t cost;
+};
+
+// The block with the least cost.  Measured, block for block (cost in brackets):
+// 40 x 2048 x 16384 7.8 us with 3 x 4 (43), 8.4 with 4 x 4 (52), 8.7 with 2 x 4
+// (68), 9.4 with 1 x 4 (75); 40 x 4096 x 4096 7.4 us with 1 x 4 (25), 8.7 with
+// 1 x 2 (34), 9.4 with 3 x 2 (35); 40 x 8192 x 2048 8.5 us with 1 x 2 (17), 10.4
+// with 1 x 4 (25), 11.1 with 1 x 1 (26); 16 x 2048 x 6144 4.0 us with 1 x 2 (17),
+// 4.7 with 1 x 4 (25), 4.9 with 1 x 1 (26); 200 x 2048 x 2048 6.2 us with 2 x 4
+// (34), 6.8 with 1 x 4 (50).  Steps asked for at once, KB: 1 against 2 8.3 and
+// 8.5 us at 32 x 2048 x 16384, 2 against 1 9.6 and 9.9 at 64 rows.
+inline FewRows few_rows(const Lin8Args &a, int64_t cus) {
+  const FewRows all[] = {
+      {launch_lin8<1, 1, 4>, few_cost<1, 1>(a, cus)}, {launch_lin8<1, 2, 4>, few_cost<1, 2>(a, cus)},
+      {launch_lin8<1, 4, 4>, few_cost<1, 4>(a, cus)}, {launch_lin8<2, 4, 1>, few_cost<2, 4>(a, cus)},
+      {launch_lin8<3, 2, 2>, few_cost<3, 2>(a, cus)}, {launch_lin8<3, 4, 1>, few_cost<3, 4>(a, cus)},
+      {launch_lin8<4, 4, 2>, few_cost<4, 4>(a, cus)}};
+  const FewRows *best = all;
+  for (const FewRows &f : all)
+    if (f.cost < best->cost) best = &f;
+  return *best;
 }
 
 // ---------------------------------------------------------------- many rows --
@@ -682,8 +692,8 @@ template <typename L> int launch_tile8(const Lin8Args &a, hipStream_t s) {
   return a.add ? launch_tile8_as<L, true>(a, s) : launch_tile8_as<L, false>(a, s);
 }
 
-// More than 64 rows: blocks of the few-row kernel where there are few of them,
-// else the tile that a simple account of its time makes the fastest.
+// More than 64 rows: the few-row kernel or the tile that a simple account of
+// its time makes the fastest.
 //   A tile shape takes, for each round of as many workgroups as the card holds,
 //   a start and end and so much a step of 128 inputs (measured, us, 2048 inputs
 //   unless said):
@@ -695,26 +705,25 @@ template <typename L> int launch_tile8(const Lin8Args &a, hipStream_t s) {
 //   which gets 65 x 2048 x 16384 (8.5 us, 12 with 128 x 128), 2048 x 8192 x 2048
 //   (31.5, 42 with 64 x 128), 4096 x 2048 x 2048 (19.4, 24.5 and 27 with the
 //   smallest and largest) and 4096 x 2048 x 16384 (117, 136 with 128 x 128) right.
-//   The few-row kernel, with up to one block of 32 x 32 a compute unit: 65 x 2048
-//   x 2048 5.2 us (tiles 7.3), 128 x 8192 x 2048 13.2 (18.8), 200 x 1536 x 576 3.7
-//   (7.0); with more, 288 x 2048 x 2048 9.7 (7.6), 100 x 2048 x 6144 9.6 (7.7).
-inline int launch_many_rows(const Lin8Args &a, hipStream_t s) {
+//   The few-row kernel takes 2.6 and 0.0054 a step and unit of its cost: 128 x
+//   2048 x 2048 4.8 us (tiles 7.2), 128 x 8192 x 2048 10.7 (18.7), 256 x 8192 x
+//   2048 15.5 (19.5); 288 x 2048 x 2048 9.1 (7.4), 100 x 2048 x 6144 8.8 (7.4).
+inline int launch_many_rows(const Lin8Args &a, int64_t cus, hipStream_t s) {
   using Small = Tile8<2, 4, 2, 2, 4>;
   using Deep = Tile8<4, 4, 2, 2, 4>;
   using Pair = Tile8<4, 4, 2, 2, 3>;
   using Large = Tile8<8, 8, 2, 2, 3>;
-  const int64_t cus = cu_count();
-  if (cus == 0) return SPECDEC_EHIP;
   const auto blocks = [&](int64_t rows, int64_t features) {
     return (a.M + rows - 1) / rows * ((a.N + features - 1) / features);
   };
-  if (!tile8_fits<Large>(a) || blocks(32, 32) * 4 <= 5 * cus) return launch_few_rows(a, s);
   const auto cost = [&](int64_t tiles, int64_t at_once, float ends, float step) {
     return (float)((tiles + at_once - 1) / at_once) * (ends + step * (float)a.steps);
   };
   const float small = cost(blocks(64, 128), cus, 2.4f, 0.28f), deep = cost(blocks(128, 128), cus, 2.4f, 0.43f);
   const float pair = cost(blocks(128, 128), 2 * cus, 2.0f, 0.95f), large = cost(blocks(256, 256), cus, 6.0f, 1.43f);
   const float least = std::min(std::min(small, deep), std::min(pair, large));
+  const FewRows few = few_rows(a, cus);
+  if (!tile8_fits<Large>(a) || 2.6f + 0.0054f * (float)(few.cost * a.steps) <= least) return few.launch(a, s);
   if (large == least) return launch_tile8<Large>(a, s);
   if (pair == least) return launch_tile8<Pair>(a, s);
   if (deep == least) return launch_tile8<Deep>(a, s);
@@ -745,5 +754,7 @@ SPECDEC_API int specdec_linear_fp8(const void *x, int64_t x_stride, const void *
              (const uint8_t *)w_scales, (uint16_t *)out, out_stride, (const uint16_t *)add, add_stride, rows,
              (int)out_features, (int)steps, 0};
   hipStream_t s = as_stream(stream);
-  return rows > 64 ? launch_many_rows(a, s) : launch_few_rows(a, s);
+  const int64_t cus = cu_count();
+  if (cus == 0) return SPECDEC_EHIP;
+  return rows > 64 ? launch_many_rows(a, cus, s) : few_rows(a, cus).launch(a, s);
 }
