@@ -469,8 +469,10 @@ int specdec_linear_silu(const void *x, int64_t x_stride, const void *w, int64_t 
  *
  * The three entries below write it from bf16 or fp32 rows (dtype), the values
  * kept in fp32 up to the one rounding.  Input rows need no alignment beyond
- * their element's.  A row's codes do not depend on the other rows.  No
- * counterpart in the reference, whose projections run in the model's type. */
+ * their element's.  A row's codes do not depend on the other rows.  Calls of
+ * more than 2^27 groups, or a norm's of more than 2^31 - 1 rows, return
+ * SPECDEC_EUNSUPPORTED.  No counterpart in the reference, whose projections run
+ * in the model's type. */
 
 /* y = x: rows [rows, dim], row_stride apart. */
 int specdec_quantize_fp8(const void *x, int dtype, int64_t rows, int64_t dim, int64_t row_stride,

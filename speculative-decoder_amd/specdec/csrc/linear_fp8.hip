@@ -10,6 +10,7 @@
 #include "fp8.h"
 
 #include <algorithm>
+#include <atomic>
 
 namespace specdec {
 
@@ -49,7 +50,7 @@ __device__ __forceinline__ f32x4 mfma8(i32x8 a, i32x8 b, f32x4 c, unsigned sa, u
 
 // More than 64 KB of LDS has to be allowed for, once a kernel and device.
 template <auto Kernel> int allow_lds(int bytes) {
-  static bool ready[64];
+  static std::atomic<bool> ready[64];
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return SPECDEC_EHIP;
   if (!ready[dev]) {
@@ -311,7 +312,7 @@ struct FewRows {
 // The block with the least cost.  Measured, block for block (cost in brackets):
 // 40 x 2048 x 16384 7.8 us with 3 x 4 (43), 8.4 with 4 x 4 (52), 8.7 with 2 x 4
 // (68), 9.4 with 1 x 4 (75); 40 x 4096 x 4096 7.4 us with 1 x 4 (25), 8.7 with
-// 1 x 2 (34), 9.4 with 3 x 2 (35); 40 x 8192 x 2048 8.5 us with 1 x 2 (17), 10.4
+// 1 x 2 (34), 9.5 with 2 x 4 (34); 40 x 8192 x 2048 8.5 us with 1 x 2 (17), 10.4
 // with 1 x 4 (25), 11.1 with 1 x 1 (26); 16 x 2048 x 6144 4.0 us with 1 x 2 (17),
 // 4.7 with 1 x 4 (25), 4.9 with 1 x 1 (26); 200 x 2048 x 2048 6.2 us with 2 x 4
 // (34), 6.8 with 1 x 4 (50).  Steps asked for at once, KB: 1 against 2 8.3 and
@@ -320,8 +321,7 @@ inline FewRows few_rows(const Lin8Args &a, int64_t cus) {
   const FewRows all[] = {
       {launch_lin8<1, 1, 4>, few_cost<1, 1>(a, cus)}, {launch_lin8<1, 2, 4>, few_cost<1, 2>(a, cus)},
       {launch_lin8<1, 4, 4>, few_cost<1, 4>(a, cus)}, {launch_lin8<2, 4, 1>, few_cost<2, 4>(a, cus)},
-      {launch_lin8<3, 2, 2>, few_cost<3, 2>(a, cus)}, {launch_lin8<3, 4, 1>, few_cost<3, 4>(a, cus)},
-      {launch_lin8<4, 4, 2>, few_cost<4, 4>(a, cus)}};
+      {launch_lin8<3, 4, 1>, few_cost<3, 4>(a, cus)}, {launch_lin8<4, 4, 2>, few_cost<4, 4>(a, cus)}};
   const FewRows *best = all;
   for (const FewRows &f : all)
     if (f.cost < best->cost) best = &f;

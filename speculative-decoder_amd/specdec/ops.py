@@ -413,16 +413,6 @@ FP8_GROUP = 128  # values that share a scale
 FP8_CODE, FP8_SCALE = torch.float8_e4m3fn, torch.float8_e8m0fnu
 
 
-def fp8_code_cols(k: int) -> int:
-    """Codes of a row of k values: whole groups, zeros past k."""
-    return -(-k // FP8_GROUP) * FP8_GROUP
-
-
-def fp8_scale_cols(k: int) -> int:
-    """Scales of a row of k values: a multiple of four, ones past the groups."""
-    return -(-k // (4 * FP8_GROUP)) * 4
-
-
 def _launch(index: int, entry, *args) -> int:
     """`entry` on the current stream of device `index`, which need not be the current one."""
     if _raw_stream is None or _device_index is None:

@@ -65,6 +65,36 @@ def test_tiles(rows, k, n, add):
     assert bool((out[0] == 7).all()) and bool((out[-1] == 7).all())
 
 
+# Few rows: each block of 16 x 16, 16 x 32, 16 x 64, 32 x 64, 48 x 64 and 64 x 64
+# (on 256 compute units), rows and features that end inside it, with scales read
+# from memory (up to 7168 inputs, and past 31744) and by way of LDS, and up to 4 rows
+FEW = [(16, 1000), (11, 5000), (15, 16001), (30, 16001), (41, 16001), (60, 16001), (120, 2039), (170, 2039), (4, 1000)]
+
+
+@pytest.mark.parametrize("k", [600, 5000, 7300, 8192])
+@pytest.mark.parametrize("rows,n", FEW)
+def test_blocks_of_few_rows(rows, n, k):
+    x, xs = operand(rows, k, rows + k)
+    wc, ws = operand(n, k, n, 0.05)
+    w = ops.tile_weight_fp8(wc)
+    base = torch.randn(rows, n, generator=gen(1), device=DEV).to(torch.bfloat16)
+    out = torch.full((rows + 2, n), 7.0, dtype=torch.bfloat16, device=DEV)
+    ops.linear_fp8(x, xs, w, ws, out=out[1:-1], add=base)
+    check(out[1:-1], values(x, xs), values(wc, ws), base)
+    assert bool((out[0] == 7).all()) and bool((out[-1] == 7).all())
+    if rows <= 64:  # however many rows, and so whichever block and way of the scales
+        for m in (1, 4, 5, 17, 33):
+            if m < rows:
+                assert torch.equal(ops.linear_fp8(x[:m], xs[:m], w, ws, add=base[:m]), out[1:1 + m]), m
+
+
+@pytest.mark.parametrize("rows,k,n", [(5, 31700, 100), (60, 31700, 16001), (5, 31800, 100), (60, 31800, 3001), (90, 70000, 100)])
+def test_long_rows(rows, k, n):
+    x, xs = operand(rows, k, rows + k)
+    wc, ws = operand(n, k, n, 0.05)
+    check(ops.linear_fp8(x, xs, ops.tile_weight_fp8(wc), ws), values(x, xs), values(wc, ws))
+
+
 def test_tiles_repeat_their_bits():
     """The same call again, alone and among others on a second stream: the same bits."""
     for rows, k, n in ((100, 1300, 3001), (1000, 520, 2100), (1000, 600, 4500), (1990, 600, 8170)):
