@@ -415,13 +415,10 @@ FP8_CODE, FP8_SCALE = torch.float8_e4m3fn, torch.float8_e8m0fnu
 
 def _launch(index: int, entry, *args) -> int:
     """`entry` on the current stream of device `index`, which need not be the current one."""
-    if _raw_stream is None or _device_index is None:
-        with torch.cuda.device(index):
-            return entry(*args, stream())
-    if _device_index() == index:
+    if _raw_stream is not None and _device_index is not None and _device_index() == index:
         return entry(*args, _raw_stream(index))
     with torch.cuda.device(index):
-        return entry(*args, _raw_stream(index))
+        return entry(*args, stream())
 
 
 def _rows_empty(dev: torch.device, lead, cols: int, dtype: torch.dtype) -> torch.Tensor:
@@ -467,8 +464,11 @@ def _fp8_input(x: torch.Tensor, name: str) -> tuple[torch.Tensor, int, int, int,
     shape = x.shape
     if not shape or shape[-1] == 0:
         raise ValueError(f"{name} needs rows of at least one value (got {list(shape)})")
-    x2 = x if len(shape) == 2 else x.reshape(-1, shape[-1])
-    rows, k = x2.shape
+    k = shape[-1]
+    if x.is_contiguous():
+        return x, dt, x.numel() // k, k, k
+    x2 = x if len(shape) == 2 else x.reshape(-1, k)
+    rows = x2.shape[0]
     stride, inner = x2.stride()
     if inner != 1 and k > 1 or rows > 1 and stride < k:  # transposed, or overlapping rows
         x2, stride = x2.contiguous(), k
@@ -615,6 +615,9 @@ def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scale
 def _fp8_operand(t: torch.Tensor, cols: int, align: int) -> tuple[torch.Tensor, int, int, int]:
     """t [..., cols] of one-byte elements as rows whose starts are aligned: the
     tensor that holds them, their number, address and stride."""
+    address = t.data_ptr()
+    if t.is_contiguous() and address % align == 0:
+        return t, t.numel() // cols, address, cols
     t2 = t if t.dim() == 2 else t.reshape(-1, cols)
     rows, address = t2.shape[0], t2.data_ptr()
     stride, inner = t2.stride()
