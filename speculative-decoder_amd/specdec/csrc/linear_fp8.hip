@@ -315,16 +315,21 @@ struct FewRows {
 // 1 x 2 (34), 9.5 with 2 x 4 (34); 40 x 8192 x 2048 8.5 us with 1 x 2 (17), 10.4
 // with 1 x 4 (25), 11.1 with 1 x 1 (26); 16 x 2048 x 6144 4.0 us with 1 x 2 (17),
 // 4.7 with 1 x 4 (25), 4.9 with 1 x 1 (26); 200 x 2048 x 2048 6.2 us with 2 x 4
-// (34), 6.8 with 1 x 4 (50).  Steps asked for at once, KB: 1 against 2 8.3 and
-// 8.5 us at 32 x 2048 x 16384, 2 against 1 9.6 and 9.9 at 64 rows.
+// (34), 6.8 with 1 x 4 (50).  One tile of rows brings little beside the weight,
+// and where that comes from memory (many weights in turn) the smaller blocks
+// spread it better: 5 x 4096 x 14336 12.7 us with 1 x 2, 14.5 with 1 x 4, 5 x
+// 2048 x 16384 8.0 and 8.5 (the same weight again and again: 4.5 with either).
+// Steps asked for at once, KB: 1 against 2 8.3 and 8.5 us at 32 x 2048 x 16384, 2
+// against 1 9.6 and 9.9 at 64 rows.
 inline FewRows few_rows(const Lin8Args &a, int64_t cus) {
   const FewRows all[] = {
       {launch_lin8<1, 1, 4>, few_cost<1, 1>(a, cus)}, {launch_lin8<1, 2, 4>, few_cost<1, 2>(a, cus)},
       {launch_lin8<1, 4, 4>, few_cost<1, 4>(a, cus)}, {launch_lin8<2, 4, 1>, few_cost<2, 4>(a, cus)},
       {launch_lin8<3, 4, 1>, few_cost<3, 4>(a, cus)}, {launch_lin8<4, 4, 2>, few_cost<4, 4>(a, cus)}};
+  const int choices = a.M <= 16 ? 2 : 6;
   const FewRows *best = all;
-  for (const FewRows &f : all)
-    if (f.cost < best->cost) best = &f;
+  for (int i = 1; i < choices; ++i)
+    if (all[i].cost < best->cost) best = &all[i];
   return *best;
 }
 
