@@ -27,7 +27,6 @@ import torch
 
 own = False
 
-_PACKAGE = str(Path(__file__).resolve().parent.parent / "speculative-decoder_amd")
 GROUP = 128
 EPS = 1e-5
 DTYPES = {"bf16": torch.bfloat16, "f32": torch.float32}
@@ -253,8 +252,9 @@ def exact(case, seed):
 
 # ------------------------------------------------------ the framework's own --
 def _run_own(state):
-    if _PACKAGE not in sys.path:
-        sys.path.insert(0, _PACKAGE)
+    package = str(Path(__file__).resolve().parent.parent / "speculative-decoder_amd")
+    if package not in sys.path:
+        sys.path.insert(0, package)
     from specdec import ops
 
     kind = state["kind"]
