@@ -5,7 +5,7 @@
 // All values stay in fp32 up to the one rounding to 8 bits; the format has
 // nothing to gain from bf16 steps in between.  These kernels move bytes, at what
 // a large copy does (5.2 TB/s) or near it: quantize 4096 x 2048 in bf16 5.3 us,
-// 4.7 TB/s; SiLU 3001 x 8192 in bf16 26.1 us, 4.7 TB/s.  A thread takes 8
+// 4.7 TB/s; SiLU 3001 x 8192 in bf16 23.6 us, 5.2 TB/s.  A thread takes 8
 // consecutive values and the 16 lanes of a DPP row make a group, so a group's
 // maximum is four lane moves and no memory, and a wave's loads and stores are
 // contiguous.  Rows of any width and stride: the loads need no alignment (bf16
@@ -57,26 +57,44 @@ __device__ __forceinline__ void store_group(const float (&y)[kPer], int r, uint8
   if (r <= pad) scale[r] = (uint8_t)(r == 0 ? byte : kFp8ScaleOne);
 }
 
-// SiLU(g) * u = g / (1 + e^-g) * u in fp32, as exactly as with a library's exp
-// and a division (each about half a unit) and in half of their instructions,
-// which would take longer than the rows' bytes (3001 x 8192 in bf16: 31.2 us
-// with them).  e^-g is 2^t on the hardware's exp2, t = -g log2 e in two parts of
-// which the small one is applied after; the quotient is g times the hardware's
-// reciprocal with one correction by its remainder.  Gates are taken as at least
-// -88.5 (e^-g still finite; the value there is below 4e-37); infinite ones give
-// NaN, as -inf / inf does, through 0 * g.
+// SiLU(g) * u = g / (1 + e^-g) * u in fp32 for g >= kSiluFar, as exactly as with a
+// library's exp and a division (each about half a unit) and in half of their
+// instructions, which would take longer than the rows' bytes (3001 x 8192 in
+// bf16: 31.2 us with them).  e^-g is 2^t on the hardware's exp2, t = -g log2 e in
+// two parts of which the small one is applied after; the quotient is g times the
+// hardware's reciprocal with one correction by its remainder.  From g = 88.5 on
+// e^-g adds nothing to 1.  Infinite gates give NaN, a code's NaN as well as an
+// infinity's.
+constexpr float kLog2e = 1.44269502f, kLog2eLow = 1.92596303e-8f, kLn2 = 0.693147182f;
+constexpr float kSiluFar = -80.0f;
+
 __device__ __forceinline__ float silu_mul_f32(float g, float u) {
 #pragma clang fp contract(off)
-  constexpr float kLog2e = 1.44269502f, kLog2eLow = 1.92596303e-8f, kLn2 = 0.693147182f;
-  const float x = __builtin_amdgcn_fmed3f(g, -88.5f, 88.5f), top = fmaxf(g, -88.5f);
+  const float x = __builtin_amdgcn_fmed3f(g, -88.5f, 88.5f);
   const float t = -x * kLog2e;
   const float low = fmaf(-x, kLog2eLow, fmaf(-x, kLog2e, -t));
   const float e0 = __builtin_amdgcn_exp2f(t);
   const float d = 1.0f + fmaf(e0, low * kLn2, e0);
   const float r = __builtin_amdgcn_rcpf(d);
-  const float s0 = top * r;
-  const float s = fmaf(fmaf(-d, s0, top), r, s0);
-  return fmaf(0.0f, g, s) * u;
+  const float s0 = g * r;
+  return fmaf(fmaf(-d, s0, g), r, s0) * u;
+}
+
+// The same for g < kSiluFar, rare in a model's rows.  1 + e^g is 1 there, so
+// SiLU(g) = g e^g, which falls below fp32's normal values (and whose 1 + e^-g
+// passes fp32) while its product with a large u is well inside: e^g = 2^k 2^f,
+// and of 2^k only what keeps g e^g normal comes before u.  Below -200 the product
+// is under 2^-152 with any u, a zero code as at -200.
+__device__ __forceinline__ float silu_mul_far(float g, float u) {
+#pragma clang fp contract(off)
+  const float x = fmaxf(g, -200.0f);
+  const float t = x * kLog2e;
+  const float low = fmaf(x, kLog2eLow, fmaf(x, kLog2e, -t));
+  const float k = rintf(t);
+  const float e0 = __builtin_amdgcn_exp2f(t - k);
+  const int all = (int)k, first = max(all, -120);
+  const float s = ldexpf(x * fmaf(e0, low * kLn2, e0), first);
+  return fmaf(0.0f, g, ldexpf(s * u, all - first));  // 0 * g: NaN for g = -inf, as -inf / inf
 }
 
 // One group for every 16 lanes; SILU: rows hold gate then up, `dim` each.
@@ -95,8 +113,20 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_kernel(const T *__rest
   if constexpr (SILU) {
     float u[kPer];
     load8(src + dim, i, dim, u);
+    // the most negative gate: among negative values the largest as bits
+    unsigned least = 0;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) y[j] = silu_mul_f32(y[j], u[j]);
+    for (int j = 0; j < kPer; ++j) least = max(least, __float_as_uint(y[j]));
+    float v[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) v[j] = silu_mul_f32(y[j], u[j]);
+    if (least > __float_as_uint(kSiluFar)) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j)
+        if (y[j] < kSiluFar) v[j] = silu_mul_far(y[j], u[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) y[j] = v[j];
   }
   const int64_t cols = (int64_t)groups * kFp8Group, gcols = fp8_scale_cols(dim);
   const int pad = grp + 1 == groups ? (int)(gcols - groups) : 0;

@@ -1,0 +1,54 @@
+"""The 8-bit operators where their values or their operands are at an edge:
+gates whose SiLU is below fp32's normal values while the product with `up` is
+not.  Tolerances as in test_gpu_fp8."""
+import pytest
+import torch
+
+from specdec import ops
+from test_gpu_fp8 import SILU_EPS, TYPES, check_near, gen
+
+pytestmark = pytest.mark.gpu
+
+DEV = torch.device("cuda", 0)
+G = 128
+
+# around the border of the two forms (-80), where 1 / (1 + e^-g) turns subnormal
+# (-126 log 2 = -87.34), where e^-g passes fp32 (-128 log 2 = -88.72), where g e^g
+# times the largest up falls below the least code (2^-136, near -188), and past it
+GATES = [-60.0, -79.5, -79.99999, -80.0, -80.00001, -80.5, -87.0, -87.3, -87.4, -88.0, -88.5, -88.6, -88.7, -88.8,
+         -89.0, -92.0, -95.0, -100.0, -103.9, -110.0, -130.0, -150.0, -170.0, -174.0, -180.0, -185.0, -187.0, -190.0,
+         -200.0, -1000.0, -3e38]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("most", [1.0, 1e10, 1e20, 1e30, 3e38])
+def test_silu_of_far_gates_times_large_values(dtype, most):
+    """A group of 128 for each gate, so that a group's scale is its values'.  A
+    value below fp32's normal ones is within half of fp32's least step, 2^-150,
+    and another for the product before it."""
+    g = gen(int(torch.tensor(most).log2()))
+    gate = torch.tensor(GATES).repeat_interleave(G).repeat(3, 1)
+    gate[1] *= 1 + 1e-3 * torch.rand(gate.shape[1], generator=g)
+    gate[2, ::2] = torch.randn(gate.shape[1] // 2, generator=g)  # near and far gates in one thread's values
+    gate = gate.clamp_min(-3e38)
+    up = most * (0.25 + 0.75 * torch.rand(gate.shape, generator=g)) * (1 - 2.0 * (torch.rand(gate.shape, generator=g) < 0.5))
+    gu = torch.cat([gate, up], dim=1).to(dtype)
+    codes, scales = ops.silu_mul_fp8(gu.to(DEV))
+    gate, up = gu.double().split(gate.shape[1], dim=1)
+    y = gate / (1 + torch.exp(-gate)) * up
+    # a near gate's product with 3e38 can pass fp32's largest value: an infinity there
+    y = torch.where(y.abs() > torch.finfo(torch.float32).max, y.sign() * float("inf"), y)
+    check_near(codes, scales, y, SILU_EPS, tiny=2.0 ** -149)
+
+
+def test_silu_of_infinite_gates_and_values():
+    """-inf gives -inf / inf = NaN and +inf an infinity, both NaN codes, beside far gates too."""
+    inf, nan = float("inf"), float("nan")
+    gate = torch.full((2, 256), -100.0)
+    gate[1] = 1.0
+    up = torch.full((2, 256), 1e30)
+    gate[:, 0], gate[:, 1], gate[:, 2], gate[:, 3] = -inf, inf, nan, -nan
+    up[:, 4], up[:, 5], up[:, 6] = inf, -inf, nan
+    codes, scales = ops.silu_mul_fp8(torch.cat([gate, up], dim=1).to(DEV))
+    g, u = gate.double(), up.double()
+    check_near(codes, scales, g / (1 + torch.exp(-g)) * u, SILU_EPS, tiny=2.0 ** -149)
