@@ -470,9 +470,9 @@ int specdec_linear_silu(const void *x, int64_t x_stride, const void *w, int64_t 
  * The three entries below write it from bf16 or fp32 rows (dtype), the values
  * kept in fp32 up to the one rounding.  Input rows need no alignment beyond
  * their element's.  A row's codes do not depend on the other rows.  Calls of
- * more than 2^27 groups, or a norm's of more than 2^31 - 1 rows, return
- * SPECDEC_EUNSUPPORTED.  No counterpart in the reference, whose projections run
- * in the model's type. */
+ * more than 2^27 groups return SPECDEC_EUNSUPPORTED (the norm has a limit of its
+ * own, below).  No counterpart in the reference, whose projections run in the
+ * model's type. */
 
 /* y = x: rows [rows, dim], row_stride apart. */
 int specdec_quantize_fp8(const void *x, int dtype, int64_t rows, int64_t dim, int64_t row_stride,
@@ -487,8 +487,10 @@ int specdec_silu_mul_fp8(const void *gate_up, int dtype, int64_t rows, int64_t i
  * rounded to the element type, written to `summed` (which may be hidden
  * itself); else h = hidden and `summed` is not used.  Then
  * y = h * rsqrt(mean(h^2) + eps) * weight.  hidden, delta and summed
- * [rows, dim] contiguous, weight [dim]; dim <= 16384 (else
- * SPECDEC_EUNSUPPORTED). */
+ * [rows, dim] contiguous, weight [dim].  dim <= 16384, and at most 2^26 - 4
+ * rows for dim <= 512, 2^25 - 2 for dim <= 1024, 2^24 - 1 for dim <= 2048,
+ * 2^23 - 1 for dim <= 4096, 2^22 - 1 past that (what a launch holds of 64 to
+ * 1024 lanes a row), else SPECDEC_EUNSUPPORTED. */
 int specdec_add_rmsnorm_fp8(const void *hidden, const void *delta, const void *weight, void *summed,
                             int dtype, int64_t rows, int64_t dim, float eps, void *codes,
                             void *scales, void *stream);

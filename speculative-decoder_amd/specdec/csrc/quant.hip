@@ -233,36 +233,32 @@ int launch_quantize(const void *x, int64_t rows, int64_t dim, int64_t stride, ui
 }
 
 template <typename T, int CH, int LANES>
-void launch_add_rmsnorm_as(const void *hidden, const void *delta, const void *weight, void *summed, int64_t rows,
-                           int64_t dim, float eps, uint8_t *codes, uint8_t *scales, hipStream_t s) {
+int launch_add_rmsnorm_as(const void *hidden, const void *delta, const void *weight, void *summed, int64_t rows,
+                          int64_t dim, float eps, uint8_t *codes, uint8_t *scales, hipStream_t s) {
   constexpr int threads = LANES < kQuantThreads ? kQuantThreads : LANES, at_once = threads / LANES;
-  add_rmsnorm_quant_kernel<T, CH, LANES><<<(unsigned)((rows + at_once - 1) / at_once), threads, 0, s>>>(
+  const int64_t blocks = (rows + at_once - 1) / at_once;
+  if (blocks > UINT32_MAX / threads) return SPECDEC_EUNSUPPORTED;  // a launch holds fewer than 2^32 threads
+  add_rmsnorm_quant_kernel<T, CH, LANES><<<(unsigned)blocks, threads, 0, s>>>(
       (const T *)hidden, (const T *)delta, (const T *)weight, (T *)summed, rows, dim, eps,
       (unsigned)((dim + kFp8Group - 1) / kFp8Group), codes, scales);
+  return launch_status();
 }
 
 template <typename T>
 int launch_add_rmsnorm_quant(const void *hidden, const void *delta, const void *weight, void *summed, int64_t rows,
                              int64_t dim, float eps, uint8_t *codes, uint8_t *scales, hipStream_t s) {
   const auto run = [&](auto ch, auto lanes) {
-    launch_add_rmsnorm_as<T, decltype(ch)::value, decltype(lanes)::value>(hidden, delta, weight, summed, rows, dim, eps,
-                                                                          codes, scales, s);
+    return launch_add_rmsnorm_as<T, decltype(ch)::value, decltype(lanes)::value>(hidden, delta, weight, summed, rows,
+                                                                                 dim, eps, codes, scales, s);
   };
   using std::integral_constant;
   const integral_constant<int, 1> one;
-  if (dim <= 512)
-    run(one, integral_constant<int, 64>());
-  else if (dim <= 1024)
-    run(one, integral_constant<int, 128>());
-  else if (dim <= 2048)
-    run(one, integral_constant<int, 256>());
-  else if (dim <= 4096)
-    run(one, integral_constant<int, 512>());
-  else if (dim <= 8192)
-    run(one, integral_constant<int, kNormMaxLanes>());
-  else
-    run(integral_constant<int, kNormMaxCh>(), integral_constant<int, kNormMaxLanes>());
-  return launch_status();
+  if (dim <= 512) return run(one, integral_constant<int, 64>());
+  if (dim <= 1024) return run(one, integral_constant<int, 128>());
+  if (dim <= 2048) return run(one, integral_constant<int, 256>());
+  if (dim <= 4096) return run(one, integral_constant<int, 512>());
+  if (dim <= 8192) return run(one, integral_constant<int, kNormMaxLanes>());
+  return run(integral_constant<int, kNormMaxCh>(), integral_constant<int, kNormMaxLanes>());
 }
 
 }  // namespace specdec
@@ -302,7 +298,7 @@ SPECDEC_API int specdec_add_rmsnorm_fp8(const void *hidden, const void *delta, c
                                         void *stream) {
   if (rows < 0 || dim <= 0) return SPECDEC_EINVAL;
   if (dtype != SPECDEC_BF16 && dtype != SPECDEC_F32) return SPECDEC_EINVAL;
-  if (dim > (int64_t)kNormMaxLanes * kPer * kNormMaxCh || rows > INT32_MAX) return SPECDEC_EUNSUPPORTED;
+  if (dim > (int64_t)kNormMaxLanes * kPer * kNormMaxCh || rows > UINT32_MAX) return SPECDEC_EUNSUPPORTED;
   if (rows == 0) return SPECDEC_OK;
   if (!hidden || !weight || (delta && !summed) || !quant_out_ok(codes, scales)) return SPECDEC_EINVAL;
   uint8_t *c = (uint8_t *)codes, *sc = (uint8_t *)scales;

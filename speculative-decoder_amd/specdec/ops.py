@@ -517,7 +517,9 @@ def add_rmsnorm_fp8(hidden: torch.Tensor, delta: torch.Tensor | None, weight: to
     `summed`, else back to hidden), then quantize_fp8(h * rsqrt(mean(h^2) +
     eps) * weight), the norm in fp32 with the one rounding to 8 bits.  hidden,
     delta and summed [..., D] contiguous, bf16 or fp32, D <= 16384; summed may
-    be hidden or delta itself, but not overlap them otherwise."""
+    be hidden or delta itself, but not overlap them otherwise.  At most 2^26 - 4
+    rows for D <= 512, 2^25 - 2 for D <= 1024, 2^24 - 1 for D <= 2048, 2^23 - 1
+    for D <= 4096, 2^22 - 1 past that."""
     if not hidden.is_cuda:
         gpu(hidden, "hidden")
     dev, dtype = hidden.device, hidden.dtype

@@ -52,3 +52,18 @@ def test_silu_of_infinite_gates_and_values():
     codes, scales = ops.silu_mul_fp8(torch.cat([gate, up], dim=1).to(DEV))
     g, u = gate.double(), up.double()
     check_near(codes, scales, g / (1 + torch.exp(-g)) * u, SILU_EPS, tiny=2.0 ** -149)
+
+
+def test_norm_of_the_most_rows_a_call_takes():
+    rows, dim = (1 << 26) - 4, 16
+    h = torch.zeros(rows, dim, dtype=torch.bfloat16, device=DEV)
+    h[-9:] = torch.randn(9, dim, generator=gen(1)).to(torch.bfloat16)
+    h[:3] = torch.randn(3, dim, generator=gen(2)).to(torch.bfloat16)
+    w = torch.ones(dim, dtype=torch.bfloat16, device=DEV)
+    codes, scales = ops.add_rmsnorm_fp8(h, None, w, 1e-5)
+    for part in (slice(0, 5), slice(rows - 12, rows)):
+        c, s = ops.add_rmsnorm_fp8(h[part].contiguous(), None, w, 1e-5)
+        assert torch.equal(codes[part].view(torch.uint8), c.view(torch.uint8))
+        assert torch.equal(scales[part].view(torch.uint8), s.view(torch.uint8))
+    with pytest.raises(NotImplementedError):
+        ops.add_rmsnorm_fp8(torch.zeros(rows + 1, dim, dtype=torch.bfloat16, device=DEV), None, w, 1e-5)
