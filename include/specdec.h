@@ -484,8 +484,8 @@ int specdec_silu_mul_fp8(const void *gate_up, int dtype, int64_t rows, int64_t i
                          int64_t row_stride, void *codes, void *scales, void *stream);
 
 /* Residual addition and RMSNorm: with delta not null, h = hidden + delta
- * rounded to the element type, written to `summed` (which may be hidden
- * itself); else h = hidden and `summed` is not used.  Then
+ * rounded to the element type, written to `summed` (which may be hidden or
+ * delta itself); else h = hidden and `summed` is not used.  Then
  * y = h * rsqrt(mean(h^2) + eps) * weight.  hidden, delta and summed
  * [rows, dim] contiguous, weight [dim].  dim <= 16384, and at most 2^26 - 4
  * rows for dim <= 512, 2^25 - 2 for dim <= 1024, 2^24 - 1 for dim <= 2048,

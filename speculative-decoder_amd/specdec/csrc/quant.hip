@@ -138,6 +138,8 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_kernel(const T *__rest
 // hidden alone without delta; then y = summed * rsqrt(mean(summed^2) + eps) *
 // weight in fp32.  The row's sum is taken in an order that dim alone fixes, so a
 // row has the same bits whatever rows come with it.
+// `summed` may be hidden or delta itself: the thread that writes a value has read
+// it from both.
 // One group of 8 values a thread and a whole row at once, as far as a workgroup
 // reaches: a row's time is one round trip to memory and one sum.  4096 x 2048 in
 // bf16 with the sum written 12.1 us (4.8 TB/s, what a large copy does is 5.2;
@@ -146,8 +148,8 @@ constexpr int kNormMaxLanes = 1024, kNormMaxCh = 2;
 
 template <typename T, int CH, int LANES>
 __global__ __launch_bounds__(LANES < kQuantThreads ? kQuantThreads : LANES) void add_rmsnorm_quant_kernel(
-    const T *hidden, const T *__restrict__ delta, const T *__restrict__ weight, T *summed, int64_t rows, int64_t dim,
-    float eps, unsigned groups, uint8_t *codes, uint8_t *scales) {
+    const T *hidden, const T *delta, const T *__restrict__ weight, T *summed, int64_t rows, int64_t dim, float eps,
+    unsigned groups, uint8_t *codes, uint8_t *scales) {
 #pragma clang fp contract(off)
   constexpr int kThreads = LANES < kQuantThreads ? kQuantThreads : LANES;
   __shared__ float red[kThreads / kWave];

@@ -67,3 +67,26 @@ def test_norm_of_the_most_rows_a_call_takes():
         assert torch.equal(scales[part].view(torch.uint8), s.view(torch.uint8))
     with pytest.raises(NotImplementedError):
         ops.add_rmsnorm_fp8(torch.zeros(rows + 1, dim, dtype=torch.bfloat16, device=DEV), None, w, 1e-5)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,dim", [(1, 1), (3, 77), (5, 512), (7, 1003), (40, 2048), (3, 4099), (2, 8192), (5, 8203),
+                                      (3, 16384)])
+def test_norm_writes_the_sum_over_delta(dtype, rows, dim):
+    """summed may be delta, or hidden, itself: the same bits as elsewhere."""
+    g = gen(rows + dim)
+    hidden, delta = (torch.randn(rows, dim, generator=g).to(dtype).to(DEV) for _ in range(2))
+    w = (1 + 0.2 * torch.randn(dim, generator=g)).to(dtype).to(DEV)
+    summed = torch.empty_like(hidden)
+    codes, scales = ops.add_rmsnorm_fp8(hidden, delta, w, 1e-5, summed=summed)
+    assert torch.equal(summed, (hidden.float() + delta.float()).to(dtype))
+    over = delta.clone()
+    before = hidden.clone()
+    c, s = ops.add_rmsnorm_fp8(hidden, over, w, 1e-5, summed=over)
+    assert torch.equal(over, summed) and torch.equal(hidden, before)
+    assert torch.equal(c.view(torch.uint8), codes.view(torch.uint8))
+    assert torch.equal(s.view(torch.uint8), scales.view(torch.uint8))
+    c, s = ops.add_rmsnorm_fp8(before, delta, w, 1e-5, summed=before)
+    assert torch.equal(before, summed)
+    assert torch.equal(c.view(torch.uint8), codes.view(torch.uint8))
+    assert torch.equal(s.view(torch.uint8), scales.view(torch.uint8))
