@@ -571,9 +571,10 @@ def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scale
     """The product of 8-bit rows (codes x [..., Kp], scales x_scales [..., Gp],
     as quantize_fp8, add_rmsnorm_fp8 and silu_mul_fp8 give them) and an 8-bit
     weight (w = tile_weight_fp8 of its codes, w_scales [N, Gp]) transposed,
-    accumulated in fp32 and rounded once: bf16 [..., N].  With `add` (bf16,
-    [..., N]; it may be `out` itself, but not overlap it otherwise) out = x @
-    w.T + add inside that rounding.  Calls of at most 64 rows give a row the
+    accumulated in fp32 and rounded once: bf16 [..., N], in `out` where given.
+    With `add` (it may be `out` itself, but not overlap it otherwise) out = x @
+    w.T + add inside that rounding.  out and add are bf16 [..., N], or its rows
+    as one [rows, N].  Calls of at most 64 rows give a row the
     same bits whatever rows come with it.  At most 1048560 rows, 2^24 features
     and 2^23 inputs."""
     if not w.is_cuda:
@@ -603,12 +604,12 @@ def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scale
     if add is None:
         add_ptr, add_stride = None, 0
     else:
-        add_ptr, add_stride = _fp8_output(dev, add, rows, n, "add")
+        add_ptr, add_stride = _fp8_output(dev, add, lead, rows, n, "add")
     if out is None:
         out = _rows_empty(dev, lead, n, torch.bfloat16)
         out_ptr, out_stride = out.data_ptr(), n
     else:
-        out_ptr, out_stride = _fp8_output(dev, out, rows, n, "out")
+        out_ptr, out_stride = _fp8_output(dev, out, lead, rows, n, "out")
     st = _launch(index, lib().specdec_linear_fp8, x_ptr, x_stride, s_ptr, s_stride, w.data_ptr(), w_scales.data_ptr(),
                  rows, kp, n, add_ptr, add_stride, out_ptr, out_stride)
     if st:
@@ -633,16 +634,25 @@ def _fp8_operand(t: torch.Tensor, cols: int, align: int) -> tuple[torch.Tensor, 
     return t2, rows, address, stride
 
 
-def _fp8_output(dev: torch.device, t: torch.Tensor, rows: int, n: int, name: str) -> tuple[int, int]:
-    """Address and row stride of a bf16 [..., N] tensor that a product adds or writes."""
+def _fp8_output(dev: torch.device, t: torch.Tensor, lead: torch.Size, rows: int, n: int, name: str) -> tuple[int, int]:
+    """Address and row stride of a bf16 [*lead, N] tensor, or its rows [rows, N], that a product adds or writes."""
     _on(dev, t, name, torch.bfloat16)
-    t2 = t if t.dim() == 2 else t.view(-1, t.shape[-1])
-    stride, inner = t2.stride()
-    if rows <= 1:
+    shape = t.shape
+    if shape == (rows, n):
+        stride, inner = t.stride()
+    elif shape == (*lead, n):
+        try:
+            stride, inner = t.view(rows, n).stride()
+        except RuntimeError:  # rows that no one stride reaches
+            stride, inner = -1, 1
+    else:
+        stride, inner = -1, 1
+    if rows <= 1 and stride >= 0:
         stride = n
-    if t2.shape != (rows, n) or inner != 1 and n > 1 or stride < n:
-        raise ValueError(f"{name} must be bf16 [rows, N] = [{rows}, {n}] with unit inner stride and rows apart")
-    return t2.data_ptr(), stride
+    if inner != 1 and n > 1 or stride < n:
+        raise ValueError(f"{name} must be bf16 {[*lead, n]} or [{rows}, {n}] with unit inner stride and rows one stride "
+                         f"apart that do not overlap (got {list(shape)} with strides {t.stride()})")
+    return t.data_ptr(), stride
 
 
 def head_logits(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:

@@ -1,8 +1,10 @@
-"""Sizes that the 8-bit operators refuse because a launch cannot hold them (no
-GPU needed: each call returns before any launch)."""
+"""What the 8-bit operators refuse: sizes that a launch cannot hold, and outputs
+and addends of another shape than the product's (no GPU needed: each call
+returns before any launch)."""
 import pytest
+import torch
 
-from specdec import _lib
+from specdec import _lib, ops
 
 EUNSUPPORTED, BF16, F32 = 3, 2, 0
 FAKE = 1 << 20  # never dereferenced
@@ -18,3 +20,30 @@ def test_norm_refuses_more_lanes_than_a_launch_holds(dim, lanes, dtype):
     for rows in (((1 << 32) - max(lanes, 256)) // lanes + 1, (1 << 32) // lanes, (1 << 32) // lanes + 1, 1 << 31, 1 << 40):
         assert norm(FAKE, None, FAKE, None, dtype, rows, dim, 1e-5, FAKE, FAKE, None) == EUNSUPPORTED, rows
         assert norm(FAKE, FAKE, FAKE, FAKE, dtype, rows, dim, 1e-5, FAKE, FAKE, None) == EUNSUPPORTED, rows
+
+
+def test_a_product_of_rows_of_several_dimensions_takes_an_output_of_its_shape():
+    """x [2, 3, Kp]: an out or add [3, 2, N] holds as many rows, in another order."""
+    cpu, bf16 = torch.device("cpu"), torch.bfloat16
+    lead, rows, n = torch.Size((2, 3)), 6, 5
+
+    def check(t):
+        return ops._fp8_output(cpu, t, lead, rows, n, "add")
+
+    good = torch.zeros(2, 3, 5, dtype=bf16)
+    wide = torch.zeros(2, 3, 9, dtype=bf16)
+    assert check(good) == (good.data_ptr(), 5)
+    assert check(good.view(6, 5)) == (good.data_ptr(), 5)  # its rows
+    assert check(wide[..., 2:7]) == (wide.data_ptr() + 4, 9)
+    for bad in (torch.zeros(3, 2, 5, dtype=bf16), torch.zeros(6, 1, 5, dtype=bf16), torch.zeros(30, dtype=bf16),
+                torch.zeros(2, 3, 6, dtype=bf16), torch.zeros((), dtype=bf16), torch.zeros(1, 5, dtype=bf16).expand(6, 5),
+                torch.zeros(3, 2, 5, dtype=bf16).transpose(0, 1),  # rows that no one stride reaches
+                torch.zeros(2, 5, 3, dtype=bf16).transpose(1, 2)):
+        with pytest.raises(ValueError, match="add must be"):
+            check(bad)
+    one = torch.zeros(5, dtype=bf16)
+    assert ops._fp8_output(cpu, one, torch.Size(()), 1, 5, "out") == (one.data_ptr(), 5)
+    with pytest.raises(ValueError, match="out must be"):
+        ops._fp8_output(cpu, one[:4], torch.Size(()), 1, 5, "out")
+    none = torch.zeros(2, 0, 5, dtype=bf16)
+    assert ops._fp8_output(cpu, none, torch.Size((2, 0)), 0, 5, "out")[1] == 5

@@ -90,3 +90,24 @@ def test_norm_writes_the_sum_over_delta(dtype, rows, dim):
     assert torch.equal(before, summed)
     assert torch.equal(c.view(torch.uint8), codes.view(torch.uint8))
     assert torch.equal(s.view(torch.uint8), scales.view(torch.uint8))
+
+
+@pytest.mark.parametrize("rows", [(2, 3), (20, 50)])
+def test_product_of_rows_of_two_dimensions_and_its_outputs(rows):
+    """out and add of the product's shape, or of its rows; the same rows in
+    another arrangement are refused."""
+    k, n = 200, 40
+    x, xs = ops.quantize_fp8(torch.randn(*rows, k, generator=gen(1)).to(DEV))
+    codes, ws = ops.quantize_fp8(torch.randn(n, k, generator=gen(2)).to(DEV))
+    w = ops.tile_weight_fp8(codes)
+    add = torch.randn(*rows, n, generator=gen(3)).to(torch.bfloat16).to(DEV)
+    want = ops.linear_fp8(x.view(-1, x.shape[-1]), xs.view(-1, xs.shape[-1]), w, ws, add=add.view(-1, n))
+    out = torch.zeros(*rows, n, dtype=torch.bfloat16, device=DEV)
+    assert ops.linear_fp8(x, xs, w, ws, out=out, add=add) is out and torch.equal(out.view(-1, n), want)
+    flat = torch.zeros(rows[0] * rows[1], n, dtype=torch.bfloat16, device=DEV)
+    ops.linear_fp8(x, xs, w, ws, out=flat, add=add.view(-1, n))
+    assert torch.equal(flat, want)
+    turned = torch.zeros(rows[1], rows[0], n, dtype=torch.bfloat16, device=DEV)
+    for bad in ({"add": turned}, {"out": turned}, {"add": turned.transpose(0, 1)}, {"out": turned.transpose(0, 1)}):
+        with pytest.raises(ValueError):
+            ops.linear_fp8(x, xs, w, ws, **bad)
