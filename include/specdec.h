@@ -518,6 +518,13 @@ int specdec_linear_fp8(const void *x, int64_t x_stride, const void *x_scales, in
                        int64_t out_features, const void *add, int64_t add_stride, void *out,
                        int64_t out_stride, void *stream);
 
+/* The workgroup that specdec_linear_fp8 takes for a call of these sizes on a GPU
+ * of `compute_units` (0: the current device's): block[0] rows x block[1]
+ * features, block[2] steps of 128 inputs of the rows held in LDS at once, 0 for
+ * the kernel of few rows, which holds none.  Launches nothing. */
+int specdec_linear_fp8_block(int64_t rows, int64_t x_stride, int64_t in_codes, int64_t out_features,
+                             int64_t compute_units, int32_t *block);
+
 /* ------------------------------------------------------------------ head --- */
 
 /* Output head: logits [rows, vocab] fp32 (logits_stride apart) = x [rows,

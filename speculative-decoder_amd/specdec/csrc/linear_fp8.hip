@@ -288,7 +288,8 @@ template <int RT, int F, int KB, bool STAGED> int launch_lin8(const Lin8Args &a,
 // 14.3, 5 x 8192 x 2048 6.2 -> 6.1, but 1 x 8192 x 2048 5.45 -> 5.6 and
 // 1 x 12288 x 2048 6.45 -> 6.9; 40 x 6144 x 2048 7.3 -> 7.25 and 16 x 7168 x 2048
 // 6.75 -> 6.85 gain nothing and 40 x 5120 x 2048 6.2 -> 6.75 loses.
-template <int RT, int F, int KB> int launch_lin8(Lin8Args a, hipStream_t s) {
+template <int RT, int F, int KB> int launch_lin8(const Lin8Args &call, hipStream_t s) {
+  Lin8Args a = call;
   a.per_wave = lin8_steps_per_wave(a.steps);
   const int waves = (a.steps + a.per_wave - 1) / a.per_wave, words = (a.steps + 3) / 4;
   if (a.M > 4 && words >= kLin8LeastWords && words <= kLin8MostWords)
@@ -304,9 +305,12 @@ template <int RT, int F> inline int64_t few_cost(const Lin8Args &a, int64_t cus)
   return (blocks + cus - 1) / cus * (9 * RT + 4 * F);
 }
 
-struct FewRows {
-  int (*launch)(Lin8Args, hipStream_t);
-  int64_t cost;
+// What a call runs on: rows x features of a workgroup, and how many steps of
+// rows its ring in LDS holds (0: the few-row kernel, rows straight to registers).
+struct Lin8Choice {
+  int (*launch)(const Lin8Args &, hipStream_t);
+  int rows, features, ring;
+  int64_t cost;  // of the few-row kernel's blocks
 };
 
 // The block with the least cost.  Measured, block for block (cost in brackets):
@@ -321,13 +325,15 @@ struct FewRows {
 // 2048 x 16384 8.0 and 8.5 (the same weight again and again: 4.5 with either).
 // Steps asked for at once, KB: 1 against 2 8.3 and 8.5 us at 32 x 2048 x 16384, 2
 // against 1 9.6 and 9.9 at 64 rows.
-inline FewRows few_rows(const Lin8Args &a, int64_t cus) {
-  const FewRows all[] = {
-      {launch_lin8<1, 1, 4>, few_cost<1, 1>(a, cus)}, {launch_lin8<1, 2, 4>, few_cost<1, 2>(a, cus)},
-      {launch_lin8<1, 4, 4>, few_cost<1, 4>(a, cus)}, {launch_lin8<2, 4, 1>, few_cost<2, 4>(a, cus)},
-      {launch_lin8<3, 4, 1>, few_cost<3, 4>(a, cus)}, {launch_lin8<4, 4, 2>, few_cost<4, 4>(a, cus)}};
+template <int RT, int F, int KB> inline Lin8Choice few_choice(const Lin8Args &a, int64_t cus) {
+  return {launch_lin8<RT, F, KB>, 16 * RT, 16 * F, 0, few_cost<RT, F>(a, cus)};
+}
+
+inline Lin8Choice few_rows(const Lin8Args &a, int64_t cus) {
+  const Lin8Choice all[] = {few_choice<1, 1, 4>(a, cus), few_choice<1, 2, 4>(a, cus), few_choice<1, 4, 4>(a, cus),
+                            few_choice<2, 4, 1>(a, cus), few_choice<3, 4, 1>(a, cus), few_choice<4, 4, 2>(a, cus)};
   const int choices = a.M <= 16 ? 2 : 6;
-  const FewRows *best = all;
+  const Lin8Choice *best = all;
   for (int i = 1; i < choices; ++i)
     if (all[i].cost < best->cost) best = &all[i];
   return *best;
@@ -713,7 +719,11 @@ template <typename L> int launch_tile8(const Lin8Args &a, hipStream_t s) {
 //   The few-row kernel takes 2.6 and 0.0054 a step and unit of its cost: 128 x
 //   2048 x 2048 4.8 us (tiles 7.2), 128 x 8192 x 2048 10.7 (18.7), 256 x 8192 x
 //   2048 15.5 (19.5); 288 x 2048 x 2048 9.1 (7.4), 100 x 2048 x 6144 8.8 (7.4).
-inline int launch_many_rows(const Lin8Args &a, int64_t cus, hipStream_t s) {
+template <typename L> inline Lin8Choice tile_choice() {
+  return {launch_tile8<L>, L::kRows, L::kFeatures, L::kSlotsX, 0};
+}
+
+inline Lin8Choice many_rows(const Lin8Args &a, int64_t cus) {
   using Small = Tile8<2, 4, 2, 2, 4>;
   using Deep = Tile8<4, 4, 2, 2, 4>;
   using Pair = Tile8<4, 4, 2, 2, 3>;
@@ -727,39 +737,72 @@ inline int launch_many_rows(const Lin8Args &a, int64_t cus, hipStream_t s) {
   const float small = cost(blocks(64, 128), cus, 2.4f, 0.28f), deep = cost(blocks(128, 128), cus, 2.4f, 0.43f);
   const float pair = cost(blocks(128, 128), 2 * cus, 2.0f, 0.95f), large = cost(blocks(256, 256), cus, 6.0f, 1.43f);
   const float least = std::min(std::min(small, deep), std::min(pair, large));
-  const FewRows few = few_rows(a, cus);
-  if (!tile8_fits<Large>(a) || 2.6f + 0.0054f * (float)(few.cost * a.steps) <= least) return few.launch(a, s);
-  if (large == least) return launch_tile8<Large>(a, s);
-  if (pair == least) return launch_tile8<Pair>(a, s);
-  if (deep == least) return launch_tile8<Deep>(a, s);
-  return launch_tile8<Small>(a, s);
+  const Lin8Choice few = few_rows(a, cus);
+  if (!tile8_fits<Large>(a) || 2.6f + 0.0054f * (float)(few.cost * a.steps) <= least) return few;
+  if (large == least) return tile_choice<Large>();
+  if (pair == least) return tile_choice<Pair>();
+  if (deep == least) return tile_choice<Deep>();
+  return tile_choice<Small>();
 }
+
+inline Lin8Choice lin8_choice(const Lin8Args &a, int64_t cus) { return a.M > 64 ? many_rows(a, cus) : few_rows(a, cus); }
 
 }  // namespace specdec
 
 using namespace specdec;
 
+// The sizes of a call, checked: SPECDEC_OK and `a` filled in as far as they go.
+static int lin8_sizes(int64_t rows, int64_t x_stride, int64_t x_scale_stride, int64_t in_codes, int64_t out_features,
+                      Lin8Args &a) {
+  if (rows < 0 || in_codes <= 0 || in_codes % kFp8Group || out_features <= 0) return SPECDEC_EINVAL;
+  const int64_t steps = in_codes / kFp8Group, scale_cols = (steps + 3) / 4 * 4;
+  if (rows > 1 && (x_stride < in_codes || x_scale_stride < scale_cols)) return SPECDEC_EINVAL;
+  if (out_features > kLin8MaxFeatures || steps > kLin8MaxSteps || rows > kLin8MaxRows) return SPECDEC_EUNSUPPORTED;
+  if (rows > 1 && (x_stride > kLin8MaxStride || x_scale_stride > kLin8MaxStride)) return SPECDEC_EUNSUPPORTED;
+  a.x_stride = x_stride;
+  a.xs_stride = x_scale_stride;
+  a.M = rows;
+  a.N = (int)out_features;
+  a.steps = (int)steps;
+  return SPECDEC_OK;
+}
+
 SPECDEC_API int specdec_linear_fp8(const void *x, int64_t x_stride, const void *x_scales, int64_t x_scale_stride,
                                    const void *w, const void *w_scales, int64_t rows, int64_t in_codes,
                                    int64_t out_features, const void *add, int64_t add_stride, void *out,
                                    int64_t out_stride, void *stream) {
-  if (rows < 0 || in_codes <= 0 || in_codes % kFp8Group || out_features <= 0) return SPECDEC_EINVAL;
-  const int64_t steps = in_codes / kFp8Group, scale_cols = (steps + 3) / 4 * 4;
-  if (rows > 1 && (x_stride < in_codes || x_scale_stride < scale_cols || out_stride < out_features ||
-                   (add && add_stride < out_features)))
-    return SPECDEC_EINVAL;
-  if (out_features > kLin8MaxFeatures || steps > kLin8MaxSteps || rows > kLin8MaxRows) return SPECDEC_EUNSUPPORTED;
-  if (rows > 1 && (x_stride > kLin8MaxStride || x_scale_stride > kLin8MaxStride)) return SPECDEC_EUNSUPPORTED;
-  if (rows == 0) return SPECDEC_OK;
+  if (rows > 1 && (out_stride < out_features || (add && add_stride < out_features))) return SPECDEC_EINVAL;
+  Lin8Args a{};
+  const int st = lin8_sizes(rows, x_stride, x_scale_stride, in_codes, out_features, a);
+  if (st != SPECDEC_OK || rows == 0) return st;
   if (!x || !x_scales || !w || !w_scales || !out) return SPECDEC_EINVAL;
   if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)x_stride) & 15) return SPECDEC_EINVAL;
   if (((uintptr_t)x_scales | (uintptr_t)w_scales | (uintptr_t)x_scale_stride) & 3) return SPECDEC_EINVAL;
   if (((uintptr_t)out | (uintptr_t)add) & 1) return SPECDEC_EINVAL;
-  Lin8Args a{(const uint8_t *)x, x_stride,   (const uint8_t *)x_scales, x_scale_stride, (const uint8_t *)w,
-             (const uint8_t *)w_scales, (uint16_t *)out, out_stride, (const uint16_t *)add, add_stride, rows,
-             (int)out_features, (int)steps, 0};
-  hipStream_t s = as_stream(stream);
+  a.x = (const uint8_t *)x;
+  a.xs = (const uint8_t *)x_scales;
+  a.w = (const uint8_t *)w;
+  a.ws = (const uint8_t *)w_scales;
+  a.out = (uint16_t *)out;
+  a.out_stride = out_stride;
+  a.add = (const uint16_t *)add;
+  a.add_stride = add_stride;
   const int64_t cus = cu_count();
   if (cus == 0) return SPECDEC_EHIP;
-  return rows > 64 ? launch_many_rows(a, cus, s) : few_rows(a, cus).launch(a, s);
+  return lin8_choice(a, cus).launch(a, as_stream(stream));
+}
+
+SPECDEC_API int specdec_linear_fp8_block(int64_t rows, int64_t x_stride, int64_t in_codes, int64_t out_features,
+                                         int64_t compute_units, int32_t *block) {
+  if (!block || compute_units < 0 || rows <= 0) return SPECDEC_EINVAL;
+  Lin8Args a{};
+  const int st = lin8_sizes(rows, x_stride, kLin8MaxStride, in_codes, out_features, a);
+  if (st != SPECDEC_OK) return st;
+  const int64_t cus = compute_units ? compute_units : cu_count();
+  if (cus == 0) return SPECDEC_EHIP;
+  const Lin8Choice c = lin8_choice(a, cus);
+  block[0] = c.rows;
+  block[1] = c.features;
+  block[2] = c.ring;
+  return SPECDEC_OK;
 }

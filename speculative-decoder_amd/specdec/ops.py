@@ -617,6 +617,21 @@ def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scale
     return out
 
 
+def linear_fp8_block(rows: int, in_codes: int, out_features: int, x_stride: int | None = None,
+                     compute_units: int = 0) -> tuple[int, int, int]:
+    """The workgroup that linear_fp8 takes for `rows` rows of in_codes = Kp
+    codes, x_stride apart (in_codes where not given), on a GPU of
+    `compute_units` (0: the current one): its rows, its features, and the steps
+    of 128 inputs that it holds of the rows in LDS, 0 for the kernel of few
+    rows."""
+    import ctypes
+
+    block = (ctypes.c_int32 * 3)()
+    _check(lib().specdec_linear_fp8_block(rows, in_codes if x_stride is None else x_stride, in_codes, out_features,
+                                          compute_units, block), "linear_fp8_block")
+    return tuple(block)
+
+
 def _fp8_operand(t: torch.Tensor, cols: int, align: int) -> tuple[torch.Tensor, int, int, int]:
     """t [..., cols] of one-byte elements as rows whose starts are aligned: the
     tensor that holds them, their number, address and stride."""

@@ -47,3 +47,38 @@ def test_a_product_of_rows_of_several_dimensions_takes_an_output_of_its_shape():
         ops._fp8_output(cpu, one[:4], torch.Size(()), 1, 5, "out")
     none = torch.zeros(2, 0, 5, dtype=bf16)
     assert ops._fp8_output(cpu, none, torch.Size((2, 0)), 0, 5, "out")[1] == 5
+
+
+def test_the_choice_of_a_workgroup():
+    """On 256 compute units: the tiles that test_gpu_fp8_tiles relies on, and blocks of few rows."""
+    from test_gpu_fp8_tiles import CALLS
+
+    def block(rows, k, n, **kw):
+        return ops.linear_fp8_block(rows, -(-k // 128) * 128, n, compute_units=256, **kw)
+
+    for tile, call in CALLS:
+        assert block(*call) == tile, call
+    assert block(1, 576, 960) == (16, 16, 0)
+    assert block(5, 2048, 16384) == (16, 32, 0)
+    assert block(40, 2048, 16384) == (48, 64, 0)
+    assert block(64, 2048, 16384) == (64, 64, 0)
+    assert block(288, 2048, 6144) == (64, 128, 4)
+    assert block(4096, 2048, 16384) == (256, 256, 3)
+    # rows too far apart for a tile's 32-bit offsets are left to the few-row kernel
+    assert block(4096, 2048, 16384, x_stride=1 << 25)[2] == 0
+
+
+def test_the_choice_refuses_what_the_product_refuses():
+    assert ops.linear_fp8_block(1048560, 128, 16, compute_units=256)
+    for bad in ((-1, 256, 16), (2, 200, 16), (2, 0, 16), (2, 256, 0)):
+        with pytest.raises(ops.KernelError):
+            ops.linear_fp8_block(*bad, compute_units=256)
+    with pytest.raises(ops.KernelError):
+        ops.linear_fp8_block(2, 256, 16, x_stride=128, compute_units=256)
+    with pytest.raises(ops.KernelError):
+        ops.linear_fp8_block(2, 256, 16, compute_units=-1)
+    for far in ((1048561, 256, 16), (2, (1 << 23) + 128, 16), (2, 256, (1 << 24) + 1)):
+        with pytest.raises(NotImplementedError):
+            ops.linear_fp8_block(*far, compute_units=256)
+    with pytest.raises(NotImplementedError):
+        ops.linear_fp8_block(2, 256, 16, x_stride=(1 << 25) + 16, compute_units=256)
