@@ -108,9 +108,11 @@ def mean_accept_len(stats):
 # ------------------------------------------------------ algorithmic bytes ---
 def weight_bytes(llama) -> int:
     """Bytes of weights one forward reads as stored: every projection of every
-    layer and the output head (embedding rows and norm vectors are noise)."""
-    n = sum(t.numel() * t.element_size() for layer in llama.layers for t in (layer.wqkv, layer.wo, layer.wgu, layer.wd))
-    return n + llama.head_wide.numel() * llama.head_wide.element_size()
+    layer (8-bit ones as codes and scales) and the output head (embedding rows
+    and norm vectors are noise)."""
+    projections = [w for layer in llama.layers for w in (layer.wqkv, layer.wo, layer.wgu, layer.wd)]
+    held = [t for w in projections for t in (w if isinstance(w, tuple) else (w,))]
+    return sum(t.numel() * t.element_size() for t in (*held, llama.head_wide))
 
 
 def kv_bytes_per_position(llama) -> int:
