@@ -200,7 +200,9 @@ class Llama:
     def fp8(self) -> "Llama":
         """This model with every layer's projections in 8 bits (weights, and
         the rows they are multiplied with): half of the layers' weight bytes
-        and, on prompts, products at twice the bf16 rate.  The residual
+        and faster large products (the 1.7B's gate/up of 4096 rows 118 us,
+        bf16 190).  Prompts and verifies of many requests gain by it, a single
+        request's steps do not: nine launches a layer against five.  The residual
         stream, attention and K/V cache, the embeddings, the final norm and
         the head stay as they are (the last three are shared with this
         model).  For bf16 models on a GPU; logits differ from the bf16 model's

@@ -108,12 +108,17 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t from_corner(const uint8_t *bas
 // 16 RT rows and F feature tiles a workgroup; the waves split the steps and
 // their sums are added in wave order.  A wave asks for KB steps of W and x at
 // once and there are up to 8 waves of up to 256 registers, so x, which every
-// workgroup reads, comes from L2 straight to registers.  What bounds that is
-// the cache lines the memory path looks up (about three cycles each), so one
-// load takes eight whole lines, 128 inputs of eight rows: lanes c < 8 of each 16
-// take the first halves of rows c, then c + 8, lanes c >= 8 the second halves of
-// rows c - 8, then c, and partners exchange what is not their row's.  The loads
-// go through buffer resources (one base and the lane's 32-bit offset), in the
+// workgroup reads, comes from L2 straight to registers.  One load takes eight
+// whole lines, 128 inputs of eight rows, so that no line is asked for in halves:
+// lanes c < 8 of each 16 take the first halves of rows c, then c + 8, lanes c >= 8
+// the second halves of rows c - 8, then c, and partners exchange what is not their
+// row's.  What the L1 does most is look up x: neighbouring lanes share a look-up
+// where their 16 bytes are one piece of 64, so a load of W is 16, but a load of x,
+// whose neighbouring lanes hold different rows, 64 (8 where the rows are past the
+// end and so one), and an unstaged load of scales 64.  Counted
+// (TCP_TOTAL_CACHE_ACCESSES), 40 x 8192 x 2048: 11.4 K a workgroup, 4.1 K of them
+// W's and 7.0 K x's; lanes along a row would look up a quarter of the latter.
+// The loads go through buffer resources (one base and the lane's 32-bit offset), in the
 // order in which the products read them, and the first word's steps stand before
 // the loop: 40 x 2048 x 16384 9.2 us -> 7.8, 64 x 2048 x 16384 10.7 -> 9.6,
 // 1 x 2048 x 16384 4.9 -> 4.6.
@@ -298,8 +303,9 @@ template <int RT, int F, int KB> int launch_lin8(const Lin8Args &call, hipStream
 }
 
 // The blocks of RT x F tiles, and how long a step of the fullest compute unit's
-// take: 9 a tile of rows, whose lines lie in rows apart and whose halves are
-// exchanged, and 4 a tile of features.
+// take: 9 a tile of rows, whose loads look up the most and whose halves are
+// exchanged, and 4 a tile of features.  The two numbers are fitted to the times
+// at few_rows().
 template <int RT, int F> inline int64_t few_cost(const Lin8Args &a, int64_t cus) {
   const int64_t blocks = (a.M + 16 * RT - 1) / (16 * RT) * ((a.N + 16 * F - 1) / (16 * F));
   return (blocks + cus - 1) / cus * (9 * RT + 4 * F);
@@ -313,6 +319,10 @@ struct Lin8Choice {
   int64_t cost;  // of the few-row kernel's blocks
 };
 
+template <int RT, int F, int KB> inline Lin8Choice few_choice(const Lin8Args &a, int64_t cus) {
+  return {launch_lin8<RT, F, KB>, 16 * RT, 16 * F, 0, few_cost<RT, F>(a, cus)};
+}
+
 // The block with the least cost.  Measured, block for block (cost in brackets):
 // 40 x 2048 x 16384 7.8 us with 3 x 4 (43), 8.4 with 4 x 4 (52), 8.7 with 2 x 4
 // (68), 9.4 with 1 x 4 (75); 40 x 4096 x 4096 7.4 us with 1 x 4 (25), 8.7 with
@@ -323,12 +333,12 @@ struct Lin8Choice {
 // and where that comes from memory (many weights in turn) the smaller blocks
 // spread it better: 5 x 4096 x 14336 12.7 us with 1 x 2, 14.5 with 1 x 4, 5 x
 // 2048 x 16384 8.0 and 8.5 (the same weight again and again: 4.5 with either).
+// The least cost is not the least time everywhere: of one tile of rows and 8192
+// features and inputs, 1 row takes 13.7 us with the 1 x 2 chosen and 12.2 with 1 x 1
+// (weights from memory 16.1 and 14.6), 5 rows 13.4 and 12.6 (16.0 and 15.7), 16
+// rows 13.6 and 13.2 (but 16.5 and 17.9).
 // Steps asked for at once, KB: 1 against 2 8.3 and 8.5 us at 32 x 2048 x 16384, 2
 // against 1 9.6 and 9.9 at 64 rows.
-template <int RT, int F, int KB> inline Lin8Choice few_choice(const Lin8Args &a, int64_t cus) {
-  return {launch_lin8<RT, F, KB>, 16 * RT, 16 * F, 0, few_cost<RT, F>(a, cus)};
-}
-
 inline Lin8Choice few_rows(const Lin8Args &a, int64_t cus) {
   const Lin8Choice all[] = {few_choice<1, 1, 4>(a, cus), few_choice<1, 2, 4>(a, cus), few_choice<1, 4, 4>(a, cus),
                             few_choice<2, 4, 1>(a, cus), few_choice<3, 4, 1>(a, cus), few_choice<4, 4, 2>(a, cus)};
@@ -408,8 +418,8 @@ template <int TR, int TF> __device__ __forceinline__ void settle(f32x4 (&acc)[TR
 // (at this size the card's power bounds the matrix unit, and of its two shapes
 // this one does more per watt: with random operands in registers 3765 TFLOP/s,
 // 32x32x64 3113).  Operands go from memory straight to LDS, in instructions of
-// 1 KB that touch eight whole cache lines (the memory path looks up a line at a
-// time): features in the order in which they are stored, rows with the 16-byte
+// 1 KB that touch eight whole cache lines, eight neighbouring lanes to a row (16
+// look-ups in L1 each): features in the order in which they are stored, rows with the 16-byte
 // chunk c of row r at place c ^ (r / 2 % 8) of its 128 bytes, so that the
 // 16-byte LDS reads of either meet in no bank.  A turn multiplies 128 inputs of
 // half of a wave's features with all its rows; its operands are in registers
