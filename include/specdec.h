@@ -581,6 +581,104 @@ int specdec_head_softmax(const void *x, int64_t x_stride, const void *w, int64_t
                          int64_t index_stride, float *workspace, int64_t workspace_floats,
                          void *stream);
 
+/* -------------------------------------------------------------- sampling --- */
+
+/* A token for each row of logits [rows, vocab] (F32 or BF16, row_stride apart)
+ * from the row's uniform u[row], under the row's temperature, top_k, top_p and
+ * min_p: the value given, or where the array beside it is not null that array's
+ * [rows].  Ids are ordered by falling logit, ties by the lower id, and weigh
+ * w = exp((x - max) / temperature).  Kept is the shortest of three prefixes of
+ * that order: the first top_k ids (all where top_k <= 0); the ids with
+ * w >= min_p (all where min_p <= 0); the least prefix whose mass reaches top_p
+ * of the mass of the first top_k (all where top_p >= 1).  The first id is always
+ * kept.  token[row] (int64) is the least id whose running sum of kept weights,
+ * in the order of ids, exceeds u times their total: the rule of
+ * specdec_sample_inverse_cdf, with weights and sums in 64 bits.  A temperature
+ * that is not above 0 keeps the first id alone.  NaN and -inf weigh nothing; of
+ * a row with +inf only those logits weigh.  A row of nothing else gets token -1.
+ * u is taken into [0, 1].  With probs not null, row `row` of it (fp32,
+ * probs_stride apart) receives w / total of the kept ids and zeros elsewhere, all
+ * zeros for token -1.  vocab <= 2^24.  No counterpart in the reference, which
+ * draws from the whole softmax (lm/sampling.py:4-18). */
+int specdec_sample(const void *logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride,
+                   const float *u, float temperature, const float *temperatures, int32_t top_k,
+                   const int32_t *top_ks, float top_p, const float *top_ps, float min_p,
+                   const float *min_ps, int64_t *token, float *probs, int64_t probs_stride,
+                   void *stream);
+
+/* ------------------------------------------------------------------ trees --- */
+
+/* A tree of drafted tokens has `nodes` <= 256 nodes a row, numbered parents
+ * first, node 0 the last token of the context, which the cache does not hold
+ * yet.  meta (int32 [3, batch]) holds each row's table row, cached length
+ * (past) and live nodes (at most `nodes`).  Rows that it describes wrongly (a
+ * table row or a past outside the tables, a block id outside the pool) get NaN
+ * and read nothing out of range; so do positions past max_positions.  No
+ * counterpart in the reference, which verifies a chain. */
+
+/* Floats of the workspace of specdec_tree_attention for these sizes (0: none;
+ * needs no initialisation). */
+int specdec_tree_attention_workspace(int32_t batch, int32_t nodes, int32_t first, int32_t n_heads,
+                                     int32_t n_kv_heads, int32_t head_dim, int dtype,
+                                     int32_t block_size, int32_t max_kv_len, int64_t *floats);
+
+/* Attention of the tree's nodes first .. nodes - 1 of each row over its cached
+ * keys and the tree.  qkv [batch, nodes, (H + 2 Hkv) * head_dim] (F32 or BF16;
+ * batch_stride and token_stride apart; q heads, k heads, v heads) holds the
+ * projections of every node before RoPE, cos and sin [max_positions,
+ * head_dim / 2] the tables, depth int32 [batch, nodes] each node's distance from
+ * node 0 and mask int64 [batch, nodes - first, ceil(nodes / 64)] a bit for each
+ * node that the query sees (bit j % 64 of word j / 64; its own is not implied;
+ * bits of nodes that are not live are ignored); a batch stride of 0 shares one
+ * tree.  Node j stands at position past + depth[j]: its q and k are rotated there
+ * and rounded to the element type, as specdec_rope_append does.  Query i sees the
+ * cached keys 0 .. past - 1, read through the block table in place, and its
+ * mask's nodes; out [batch, nodes - first, H * head_dim] (out_batch_stride and
+ * out_token_stride apart, apart from the inputs) receives the softmax-weighted
+ * values, zeros for a query that sees nothing; queries that are not live are
+ * not written.  The cache is read only.  head_dim 64 or 128.  Softmax in fp32 with
+ * `scale`.  max_kv_len is the cached length that the launch is laid out for;
+ * longer rows are right too, and slower.  Without the whole of
+ * specdec_tree_attention_workspace's floats the call runs without any; calls
+ * sharing a workspace must be ordered. */
+int specdec_tree_attention(const void *qkv, int dtype, int64_t batch_stride, int64_t token_stride,
+                           const float *cos_table, const float *sin_table, int64_t max_positions,
+                           const void *k_pool, const void *v_pool, int64_t num_blocks,
+                           const int32_t *tables, int64_t table_stride, int32_t table_rows,
+                           int32_t table_cols, const int32_t *meta, const int64_t *mask,
+                           int64_t mask_batch_stride, int64_t mask_row_stride, const int32_t *depth,
+                           int64_t depth_batch_stride, int32_t batch, int32_t nodes, int32_t first,
+                           int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
+                           int32_t block_size, float scale, int32_t max_kv_len, float *workspace,
+                           int64_t workspace_floats, void *out, int64_t out_batch_stride,
+                           int64_t out_token_stride, void *stream);
+
+/* The walk down each row's tree along the tokens sampled at its nodes, and the
+ * append of its path to the cache.  tokens and sampled int64 [batch, nodes]
+ * (strides apart) hold the token that a node carries and the one sampled after
+ * it, parents int32 [batch, nodes] (a stride of 0 shares one tree).  From node 0
+ * the walk goes on to the lowest live child, of a higher number, that carries
+ * the token sampled at the node, until there is none or the path has `room`
+ * nodes.  verdict int64 [nodes + 1, batch] receives the drafted tokens accepted
+ * (n), the token sampled at the path's last node, and the accepted tokens, -1
+ * after them; path int32 [batch, nodes] the path's n + 1 nodes, -1 after them.
+ * With layers > 0, path node j's k of every layer, rotated at position past + j,
+ * and its v, from qkv [layers, batch, nodes, (H + 2 Hkv) * head_dim], are written
+ * to slot past + j of k_pool [layers, num_blocks, Hkv, block_size, head_dim] and
+ * v_pool [layers, num_blocks, Hkv, head_dim, block_size]; the row's table must
+ * hold the blocks of `room` slots, and the path ends before a slot outside the
+ * tables, the pool or the positions.  A row with no live node or no slot gets n =
+ * -1 and token -1.  head_dim even. */
+int specdec_tree_commit(const int64_t *tokens, int64_t tokens_stride, const int32_t *parents,
+                        int64_t parents_stride, const int64_t *sampled, int64_t sampled_stride,
+                        const int32_t *meta, int32_t batch, int32_t nodes, int32_t room,
+                        int64_t *verdict, int32_t *path, const void *qkv, int dtype, int32_t layers,
+                        int64_t layer_stride, int64_t batch_stride, int64_t token_stride,
+                        const float *cos_table, const float *sin_table, int64_t max_positions,
+                        int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int32_t block_size,
+                        void *k_pool, void *v_pool, int64_t num_blocks, const int32_t *tables,
+                        int64_t table_stride, int32_t table_rows, int32_t table_cols, void *stream);
+
 /* fp32 split partials the library holds per GPU for
  * specdec_paged_attention_static (8 MiB). */
 #define SPECDEC_STATIC_PARTIAL_FLOATS (2 * 1024 * 1024)

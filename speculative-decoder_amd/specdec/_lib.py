@@ -57,6 +57,12 @@ SIGNATURES: dict[str, list] = {
     "specdec_silu_mul_fp8": [P, c_int, I64, I64, I64, P, P, P],
     "specdec_add_rmsnorm_fp8": [P, P, P, P, c_int, I64, I64, c_float, P, P, P],
     "specdec_linear_fp8": [P, I64, P, I64, P, P, I64, I64, I64, P, I64, P, I64, P],
+    "specdec_sample": [P, c_int, I64, I64, I64, P, c_float, P, I32, P, c_float, P, c_float, P, P, P, I64, P],
+    "specdec_tree_attention_workspace": [I32, I32, I32, I32, I32, I32, c_int, I32, I32, P],
+    "specdec_tree_attention": [P, c_int, I64, I64, P, P, I64, P, P, I64, P, I64, I32, I32, P, P, I64, I64, P, I64, I32,
+                               I32, I32, I32, I32, I32, I32, c_float, I32, P, I64, P, I64, I64, P],
+    "specdec_tree_commit": [P, I64, P, I64, P, I64, P, I32, I32, I32, P, P, P, c_int, I32, I64, I64, I64, P, P, I64,
+                            I32, I32, I32, I32, P, P, I64, P, I64, I32, I32, P],
     "specdec_linear_fp8_block": [I64, I64, I64, I64, I64, P],
     "specdec_paged_attention_static": [P, c_int, I64, P, P, P, I64, P, I32, I32, I32, I32, I32, I32, c_float,
                                        I32, I32, P, I64, P],

@@ -1184,3 +1184,245 @@ def rope_paged_attention(qkv, cos, sin, k_pool, v_pool, tables, meta, batch, wid
                                             stream())
     _check(st, "rope_paged_attention")
     return out
+
+
+# ---------------------------------------------------------------- sampling --
+def _per_row(v, dev: torch.device, rows: int, dtype: torch.dtype, name: str, lo: float, hi: float):
+    """A sampling parameter as (value, array): a number in lo .. hi, or a
+    tensor of one value a row, which the kernel reads."""
+    if isinstance(v, torch.Tensor):
+        return 0, _on(dev, v, name, dtype, True, rows).data_ptr()
+    if not lo <= v <= hi:
+        raise ValueError(f"{name} must be in {lo} .. {hi} (got {v})")
+    return v, None
+
+
+def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+           out: torch.Tensor | None = None, probs: torch.Tensor | None = None) -> torch.Tensor:
+    """A token for each row of logits [..., V] (fp32 or bf16) from the row's
+    uniform u [...] (fp32): int64 [...], in `out` where given.
+
+    Ids are ordered by falling logit, ties by the lower id, with weights w =
+    exp((x - max) / temperature).  Kept is the shortest of three prefixes of
+    that order: the first top_k (0: all); those with w >= min_p; the least
+    prefix whose mass reaches top_p of the mass of the first top_k (1: all).
+    The first id is always kept, and alone at temperature 0.  The token is the
+    least id whose running sum of kept weights, in the order of ids, exceeds u
+    times their total, in 64-bit arithmetic.  NaN and -inf logits weigh nothing;
+    a row of nothing else gets -1.
+
+    temperature, top_p and min_p are numbers or fp32 tensors of a value a row,
+    top_k an int or an int32 tensor.  `probs` (fp32 [..., V], rows of any
+    stride) receives the distribution that the token was drawn from, for an
+    accept-reject against it; zeros in a row without a token."""
+    if not logits.is_cuda:
+        gpu(logits, "logits")
+    dt = _FP8_INPUTS.get(logits.dtype)
+    if dt is None:
+        raise TypeError(f"logits must be bf16 or fp32 (got {logits.dtype})")
+    shape = logits.shape
+    if not shape or shape[-1] == 0:
+        raise ValueError(f"logits need rows of at least one value (got {list(shape)})")
+    dev, lead, v = logits.device, shape[:-1], shape[-1]
+    x = logits if len(shape) == 2 else logits.reshape(-1, v)
+    rows = x.shape[0]
+    if x.stride(1) != 1 and v > 1 or rows > 1 and x.stride(0) < v:
+        x = x.contiguous()
+    _on(dev, u, "u", torch.float32, True, rows)
+    t, t_ptr = _per_row(temperature, dev, rows, torch.float32, "temperature", 0.0, 3.4e38)
+    k, k_ptr = _per_row(top_k, dev, rows, torch.int32, "top_k", 0, 2 ** 31 - 1)
+    p, p_ptr = _per_row(top_p, dev, rows, torch.float32, "top_p", 0.0, 1.0)
+    m, m_ptr = _per_row(min_p, dev, rows, torch.float32, "min_p", 0.0, 1.0)
+    if out is None:
+        out = torch.empty(lead, dtype=torch.int64, device=dev)
+    else:
+        _on(dev, out, "out", torch.int64, True, rows)
+    probs_ptr, probs_stride = None, 0
+    if probs is not None:
+        _on(dev, probs, "probs", torch.float32)
+        if probs.shape != shape and probs.shape != (rows, v):
+            raise ValueError(f"probs must be {list(shape)} or [{rows}, {v}] (got {list(probs.shape)})")
+        p2 = probs if probs.dim() == 2 else probs.view(rows, v)
+        if p2.stride(1) != 1 and v > 1 or rows > 1 and p2.stride(0) < v:
+            raise ValueError("probs needs unit inner stride and rows that do not overlap")
+        probs_ptr, probs_stride = p2.data_ptr(), p2.stride(0)
+    st = _launch(dev.index, lib().specdec_sample, x.data_ptr(), dt, rows, v, x.stride(0), u.data_ptr(), t, t_ptr, k, k_ptr,
+                 p, p_ptr, m, m_ptr, out.data_ptr(), probs_ptr, probs_stride)
+    if st:
+        _check(st, "sample")
+    return out
+
+
+# ------------------------------------------------------------------- trees --
+TREE_NODES = 256  # nodes of a tree, at most
+
+
+def _tree_side(dev: torch.device, dtype: torch.dtype, cos, sin, k_pool, v_pool, tables, layered: int) -> tuple[int, ...]:
+    """(blocks, kv heads, block size, head_dim) of the paged pools [(layers,)
+    blocks, kv heads, block size, head_dim] (V with the last two swapped), and
+    the checks of what else a tree's kernels read the cache with."""
+    shape = k_pool.shape
+    if len(shape) != 4 + layered or v_pool.shape != (*shape[:-2], shape[-1], shape[-2]):
+        raise ValueError(f"the pools must be {'[layers, ' if layered else '['}blocks, kv heads, block size, head_dim] and "
+                         f"the same with the last two swapped (got {list(shape)} and {list(v_pool.shape)})")
+    _on(dev, k_pool, "k_pool", dtype, True)
+    _on(dev, v_pool, "v_pool", dtype, True)
+    _on(dev, cos, "cos", torch.float32, True)
+    _on(dev, sin, "sin", torch.float32, True)
+    if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] * 2 != shape[-1]:
+        raise ValueError(f"cos and sin must be [positions, {shape[-1] // 2}] (got {list(cos.shape)} and {list(sin.shape)})")
+    _on(dev, tables, "tables", torch.int32)
+    if tables.dim() != 2 or tables.stride(1) != 1 or tables.shape[0] > 1 and tables.stride(0) < tables.shape[1]:
+        raise ValueError("block tables must be int32 [rows, capacity] with unit inner stride")
+    return shape[-4:]
+
+
+def _tree_rows(qkv: torch.Tensor, kv_heads: int, head_dim: int) -> int:
+    """Query heads of projection rows [..., (H + 2 Hkv) * head_dim]."""
+    heads = qkv.shape[-1] // head_dim - 2 * kv_heads
+    if heads <= 0 or (heads + 2 * kv_heads) * head_dim != qkv.shape[-1]:
+        raise ValueError(f"qkv rows of {qkv.shape[-1]} values do not hold q, k and v of {kv_heads} kv heads of {head_dim}")
+    if qkv.stride(-1) != 1 or qkv.shape[-2] > 1 and qkv.stride(-2) < qkv.shape[-1]:
+        raise ValueError("qkv needs unit inner stride and rows that do not overlap")
+    return heads
+
+
+def _per_tree(dev: torch.device, t: torch.Tensor, batch: int, shape: tuple, dtype: torch.dtype, name: str) -> int:
+    """Batch stride of t [batch or 1, *shape], 0 where one tree serves every row."""
+    _on(dev, t, name, dtype)
+    got = t.shape
+    if len(got) != 1 + len(shape) or got[0] not in (1, batch) or got[1:] != shape:
+        raise ValueError(f"{name} must be [{batch} or 1, {', '.join(map(str, shape))}] (got {list(got)})")
+    if t.stride(-1) != 1 and shape[-1] > 1:
+        raise ValueError(f"{name} needs unit inner stride")
+    return 0 if got[0] == 1 else t.stride(0)
+
+
+def tree_attention(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                   tables: torch.Tensor, meta: torch.Tensor, mask: torch.Tensor, depth: torch.Tensor, n_heads: int,
+                   scale: float, max_kv_len: int, first: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of a tree's nodes first .. N - 1 over the paged cache and the
+    tree: [B, N - first, H * head_dim], in `out` where given.
+
+    qkv [B, N, (H + 2 Hkv) * head_dim] (bf16 or fp32) holds the projections of
+    every node before RoPE, parents before children, node 0 the last token of
+    the context.  Node j of a row with `past` cached positions is rotated at past
+    + depth[j]; query i sees the cached keys and the nodes of its mask.  mask is
+    int64 [B or 1, N - first, ceil(N / 64)] ([.., N - first] up to 64 nodes), bit j
+    % 64 of word j / 64 for node j, depth int32 [B or 1, N] (lm.tree.plan makes
+    both).  meta int32 [3, B]: table row, past, live nodes; queries past the live
+    nodes are not written, one that sees nothing gets zeros.  Pools as KVCache
+    keeps a layer's; the cache is read only (tree_commit writes it).  head_dim 64
+    or 128.  max_kv_len is the cached length the launch is laid out for; longer
+    rows are right too, and slower."""
+    if not qkv.is_cuda:
+        gpu(qkv, "qkv")
+    dev, dt = qkv.device, _FP8_INPUTS.get(qkv.dtype)
+    if dt is None:
+        raise TypeError(f"qkv must be bf16 or fp32 (got {qkv.dtype})")
+    if qkv.dim() != 3:
+        raise ValueError(f"qkv must be [B, N, (H + 2 Hkv) * head_dim] (got {list(qkv.shape)})")
+    blocks, kv_heads, bs, d = _tree_side(dev, qkv.dtype, cos, sin, k_pool, v_pool, tables, 0)
+    batch, nodes, _ = qkv.shape
+    if _tree_rows(qkv, kv_heads, d) != n_heads:
+        raise ValueError(f"qkv rows of {qkv.shape[2]} values do not hold {n_heads} query and {kv_heads} kv heads of {d}")
+    if not 0 <= first <= nodes or nodes > TREE_NODES:
+        raise ValueError(f"a tree has at most {TREE_NODES} nodes, first among them (got {nodes}, {first})")
+    _on(dev, meta, "meta", torch.int32, True, 3 * batch)
+    words, width = -(-nodes // 64), nodes - first
+    if mask.dim() == 2 and words == 1:
+        mask = mask[:, :, None]
+    mask_stride = _per_tree(dev, mask, batch, (width, words), torch.int64, "mask")
+    depth_stride = _per_tree(dev, depth, batch, (nodes,), torch.int32, "depth")
+    if out is None:
+        out = torch.empty(batch, width, n_heads * d, dtype=qkv.dtype, device=dev)
+    else:
+        _on(dev, out, "out", qkv.dtype)
+        if out.shape != (batch, width, n_heads * d):
+            raise ValueError(f"out must be {[batch, width, n_heads * d]} (got {list(out.shape)})")
+        s0, s1, s2 = out.stride()
+        if s2 != 1 or width > 1 and s1 < n_heads * d or batch > 1 and s0 < (width - 1) * s1 + n_heads * d:
+            raise ValueError("out needs unit inner stride and rows that do not overlap")
+    ws = _tree_workspace(dev, batch, nodes, first, n_heads, kv_heads, d, dt, bs, max_kv_len)
+    st = _launch(dev.index, lib().specdec_tree_attention, qkv.data_ptr(), dt, qkv.stride(0), qkv.stride(1), cos.data_ptr(),
+                 sin.data_ptr(), cos.shape[0], k_pool.data_ptr(), v_pool.data_ptr(), blocks, tables.data_ptr(),
+                 tables.stride(0), tables.shape[0], tables.shape[1], meta.data_ptr(), mask.data_ptr(), mask_stride,
+                 mask.stride(1), depth.data_ptr(), depth_stride, batch, nodes, first, n_heads, kv_heads, d, bs, scale,
+                 max_kv_len, ptr(ws), 0 if ws is None else ws.numel(), out.data_ptr(), out.stride(0), out.stride(1))
+    if st:
+        _check(st, "tree_attention")
+    return out
+
+
+def _tree_workspace(dev: torch.device, *sizes) -> torch.Tensor | None:
+    """A call's split partials: memory of the call's own, from torch's
+    allocator, so calls on several streams or in several graphs share none."""
+    import ctypes
+
+    floats = ctypes.c_int64()
+    _check(lib().specdec_tree_attention_workspace(*sizes, ctypes.byref(floats)), "tree_attention")
+    return torch.empty(floats.value, dtype=torch.float32, device=dev) if floats.value else None
+
+
+def tree_commit(tokens: torch.Tensor, parents: torch.Tensor, sampled: torch.Tensor, meta: torch.Tensor,
+                room: int | None = None, qkv: torch.Tensor | None = None, cos: torch.Tensor | None = None,
+                sin: torch.Tensor | None = None, k_pool: torch.Tensor | None = None,
+                v_pool: torch.Tensor | None = None, tables: torch.Tensor | None = None):
+    """The walk down each row's tree along the tokens sampled at its nodes, and
+    with a cache the append of the path's keys and values to every layer of it,
+    in one launch: (verdict int64 [N + 1, B], path int32 [B, N]).
+
+    tokens and sampled int64 [B, N] are the token that a node carries and the one
+    sampled after it, parents int32 [B or 1, N] (-1 for node 0), meta int32 [3, B]
+    as tree_attention's.  From node 0 the walk goes on to the lowest live child
+    that carries the token sampled at the node.  verdict: the number n of drafted
+    tokens accepted, the token sampled at the path's last node, then the accepted
+    tokens; path: its n + 1 nodes; -1 past them.
+
+    qkv [layers, B, N, (H + 2 Hkv) * head_dim] are the projections that the
+    layers' tree_attention read; path node j's k, rotated at position past + j, and
+    v go to slot past + j of the pools [layers, blocks, ..], whose tables hold the
+    blocks of `room` slots past each row's cached length.  The path has at most
+    `room` nodes (N where not given).  A row without a live node or a slot gets n =
+    -1 and token -1."""
+    if not tokens.is_cuda:
+        gpu(tokens, "tokens")
+    dev = tokens.device
+    if tokens.dim() != 2:
+        raise ValueError(f"tokens must be [B, N] (got {list(tokens.shape)})")
+    batch, nodes = tokens.shape
+    if not 0 < nodes <= TREE_NODES:
+        raise ValueError(f"a tree has 1 to {TREE_NODES} nodes (got {nodes})")
+    room = nodes if room is None else room
+    if room < 1:
+        raise ValueError(f"room must be at least 1, for node 0 (got {room})")
+    tokens_stride = _per_tree(dev, tokens, batch, (nodes,), torch.int64, "tokens")
+    sampled_stride = _per_tree(dev, sampled, batch, (nodes,), torch.int64, "sampled")
+    if sampled.shape[0] != batch:
+        raise ValueError(f"sampled must be [{batch}, {nodes}] (got {list(sampled.shape)})")
+    parents_stride = _per_tree(dev, parents, batch, (nodes,), torch.int32, "parents")
+    _on(dev, meta, "meta", torch.int32, True, 3 * batch)
+    cache = [None, F32, 0, 0, 0, 0, None, None, 0, 0, 0, 0, 0, None, None, 0, None, 0, 0, 0]
+    if qkv is not None:
+        dt = _FP8_INPUTS.get(qkv.dtype)
+        if dt is None:
+            raise TypeError(f"qkv must be bf16 or fp32 (got {qkv.dtype})")
+        _on(dev, qkv, "qkv")
+        blocks, kv_heads, bs, d = _tree_side(dev, qkv.dtype, cos, sin, k_pool, v_pool, tables, 1)
+        if qkv.dim() != 4 or qkv.shape[:3] != (k_pool.shape[0], batch, nodes):
+            raise ValueError(f"qkv must be [{k_pool.shape[0]}, {batch}, {nodes}, (H + 2 Hkv) * head_dim] (got "
+                             f"{list(qkv.shape)})")
+        heads = _tree_rows(qkv, kv_heads, d)
+        cache = [qkv.data_ptr(), dt, qkv.shape[0], qkv.stride(0), qkv.stride(1), qkv.stride(2), cos.data_ptr(),
+                 sin.data_ptr(), cos.shape[0], heads, kv_heads, d, bs, k_pool.data_ptr(), v_pool.data_ptr(), blocks,
+                 tables.data_ptr(), tables.stride(0), tables.shape[0], tables.shape[1]]
+    elif k_pool is not None or v_pool is not None:
+        raise ValueError("a commit to a cache needs the layers' qkv")
+    verdict = torch.empty(nodes + 1, batch, dtype=torch.int64, device=dev)
+    path = torch.empty(batch, nodes, dtype=torch.int32, device=dev)
+    st = _launch(dev.index, lib().specdec_tree_commit, tokens.data_ptr(), tokens_stride, parents.data_ptr(), parents_stride,
+                 sampled.data_ptr(), sampled_stride, meta.data_ptr(), batch, nodes, room, verdict.data_ptr(),
+                 path.data_ptr(), *cache)
+    if st:
+        _check(st, "tree_commit")
+    return verdict, path
