@@ -14,6 +14,9 @@
 
 namespace specdec {
 
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+
 constexpr int kTreeMaxNodes = 256;
 
 struct TreeArgs {
@@ -144,6 +147,438 @@ __global__ __launch_bounds__(kWave) void tree_attention_any_kernel(TreeArgs a) {
     out[lane + e * kWave] = from_f32<T>(!good ? NAN : l > 0.0f || l != l ? o[e] / l : 0.0f);
 }
 
+// The grid of matrix-instruction tiles.
+//
+// A wave owns chunks of CK keys (32 in bf16, 16 in fp32: 4 lane groups of a
+// 16-byte piece) and up to NT tiles of 16 query rows, the nodes and query heads
+// of one kv head.  With lane = 16 g + c:
+//   S^T[key, query] = K Q^T    A: K row of lane c, B: query c, pieces of 16 bytes
+//                              at dims CK j + EPL g
+//   O^T[dim, query] += V^T P^T A: V row of dim 16 t + c, keys EPL g .. + EPL - 1
+// Row 4 g + i of score tile t is key EPL g + 4 t + i of the chunk, so the scores
+// that a lane holds are the keys of the V piece that it loads: P goes from one
+// product to the next in registers, and K and V pass from memory to registers
+// once for all of the wave's query rows, with no LDS and no barrier before the
+// end, where the workgroup's waves fold their (m, l, O).
+// A lane's row of K holds pieces j and j + NP / 2 of a rotated pair of dims, so the
+// tree's own keys are rotated in the registers that they arrive in.
+constexpr int kTreeWaves = 4;
+
+template <typename T, int D> struct TreeTile {
+  static constexpr int EPL = 16 / sizeof(T);  // elements of a piece
+  static constexpr int CK = 4 * EPL;
+  static constexpr int NTK = CK / 16;  // score tiles of a chunk
+  static constexpr int NP = D / CK;    // pieces of a lane's K or Q row
+  static constexpr int ND = D / 16;    // pieces of V, tiles of O
+};
+
+__device__ __forceinline__ f32x4 tree_mma(__hip_bfloat16, u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 tree_mma(float, u32x4 a, u32x4 b, f32x4 c) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[e]), __uint_as_float(b[e]), c, 0, 0, 0);
+  return c;
+}
+__device__ __forceinline__ void tree_unpack(u32x4 v, float (&x)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = __uint_as_float((e & 1) ? v[e / 2] & 0xFFFF0000u : v[e / 2] << 16);
+}
+__device__ __forceinline__ void tree_unpack(u32x4 v, float (&x)[4]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(v[e]);
+}
+__device__ __forceinline__ u32x4 tree_pack(const float (&x)[8]) {
+  bf16x8 v;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = (__bf16)x[e];  // to nearest even
+  return __builtin_bit_cast(u32x4, v);
+}
+__device__ __forceinline__ u32x4 tree_pack(const float (&x)[4]) {
+  return u32x4{__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])};
+}
+
+// The pieces lo = dims d .. d + EPL - 1 and hi = those half a head later, rotated at a position.
+template <int EPL> __device__ __forceinline__ void tree_rotate(u32x4 &lo, u32x4 &hi, const float *c, const float *s, bool in) {
+  float x1[EPL], x2[EPL];
+  tree_unpack(lo, x1);
+  tree_unpack(hi, x2);
+#pragma unroll
+  for (int e = 0; e < EPL; ++e) {
+    float y1, y2;
+    rope_pair(x1[e], x2[e], in ? c[e] : NAN, in ? s[e] : NAN, y1, y2);
+    x1[e] = y1;
+    x2[e] = y2;
+  }
+  lo = tree_pack(x1);
+  hi = tree_pack(x2);
+}
+
+// Row pieces of a q or k row at a position of the tree, rotated and rounded.
+template <typename T, int D>
+__device__ __forceinline__ void tree_row_pieces(const TreeArgs &a, const T *row, int64_t pos, int g,
+                                                u32x4 (&r)[TreeTile<T, D>::NP]) {
+  using L = TreeTile<T, D>;
+  const bool in = pos >= 0 && pos < a.positions;
+  const int64_t at = in ? pos * (D / 2) : 0;
+#pragma unroll
+  for (int j = 0; j < L::NP; ++j) r[j] = *(const u32x4 *)(row + L::CK * j + L::EPL * g);
+#pragma unroll
+  for (int j = 0; j < L::NP / 2; ++j) {
+    float c[L::EPL], s[L::EPL];
+#pragma unroll
+    for (int e = 0; e < L::EPL; e += 4) {
+      *(f32x4 *)&c[e] = *(const f32x4 *)(a.cos_t + at + L::CK * j + L::EPL * g + e);
+      *(f32x4 *)&s[e] = *(const f32x4 *)(a.sin_t + at + L::CK * j + L::EPL * g + e);
+    }
+    tree_rotate<L::EPL>(r[j], r[j + L::NP / 2], c, s, in);
+  }
+}
+
+// How a call is cut: tiles of a wave, groups of them over a kv head's query
+// rows, splits over the cached keys.
+struct TreeCut {
+  int tiles, groups, splits;
+  __host__ __device__ int64_t rows() const { return (int64_t)groups * tiles * 16; }  // of a kv head, with padding
+};
+
+// Split partials: for each (row, kv head, split) the query rows' m and l, then
+// their O, not divided.
+struct TreeParts {
+  float *ml, *o;
+};
+__host__ __device__ inline TreeParts tree_parts(float *ws, int64_t unit, int64_t units, int64_t rows, int d) {
+  return TreeParts{ws + unit * rows * 2, ws + units * rows * 2 + unit * rows * d};
+}
+
+// Waves a SIMD that a variant's registers are held to.
+constexpr int tree_waves(int d, int tiles) { return d == 64 ? (tiles == 1 ? 3 : tiles == 2 ? 2 : 1) : (tiles == 1 ? 2 : 1); }
+
+template <typename T, int D, int NT>
+__global__ __launch_bounds__(kTreeWaves *kWave)
+    __attribute__((amdgpu_waves_per_eu(tree_waves(D, NT), tree_waves(D, NT)))) void tree_attention_kernel(TreeArgs a, TreeCut cut, int shift, float *ws) {
+  using L = TreeTile<T, D>;
+  constexpr int EPL = L::EPL, CK = L::CK, NTK = L::NTK, NP = L::NP, ND = L::ND, NW = kTreeWaves;
+  constexpr int MT = NT < 2 ? 1 : 2;  // tiles folded at a time
+  __shared__ float s_o[NW][MT][16][D + 4];
+  __shared__ float s_ml[NW][MT][16][2];
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, c = lane & 15, g = lane / 16;
+  // query groups that read the same keys run next to one another on one XCD,
+  // whose L2 then serves all but the first (workgroups go to the XCDs in turn)
+  const int units = a.batch * a.Hkv * cut.splits;
+  int unit = blockIdx.x, qg = 0;
+  if (cut.groups > 1) {
+    const int rest = unit / 8;
+    qg = rest % cut.groups;
+    unit = rest / cut.groups * 8 + unit % 8;
+    if (unit >= units) return;
+  }
+  const int split = unit % cut.splits, bh = unit / cut.splits, hk = bh % a.Hkv, b = bh / a.Hkv;
+  const int G = a.H / a.Hkv;
+  const TreeRow r = tree_row(a, b);
+  const int row0 = qg * NT * 16, nrows = (r.live - a.first) * G;
+  if (row0 >= nrows) return;
+  const int tiles = min(NT, (nrows - row0 + 15) / 16);
+  bool bad = !r.fits;
+  const int past = r.fits ? r.past : 0, live = r.live;
+  const T *rows = (const T *)a.qkv + b * a.batch_stride;
+  const int32_t *depth = a.depth + b * a.depth_batch_stride;
+  const int32_t *table = a.tables + (r.fits ? r.row * a.table_stride : 0);
+
+  u32x4 q[NT][NP];
+  f32x4 o[NT][ND];
+  float m[NT], l[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int qr = min(row0 + 16 * t + c, nrows - 1), node = a.first + qr / G;
+    if (t < tiles)
+      tree_row_pieces<T, D>(a, rows + node * a.token_stride + (int64_t)(hk * G + qr % G) * D, (int64_t)r.past + depth[node], g,
+                            q[t]);
+    m[t] = -INFINITY;
+    l[t] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const float sc = a.scale * 1.4426950408889634f;  // scores in log2 units
+
+  // the chunk's weights of tile t, in log2 units against the running maximum,
+  // which is raised when a score passes it by 2^8 only: rarely after the first
+  // chunks, and p <= 2^8 loses nothing
+  auto weigh = [&](int t, float (&s)[EPL]) {
+    float top = s[0];
+#pragma unroll
+    for (int e = 1; e < EPL; ++e) top = fmaxf(top, s[e]);
+    top *= sc;
+    if (__any(top > m[t] + 8.0f)) {
+      top = fmaxf(top, __shfl_xor(top, 16, kWave));
+      top = fmaxf(top, __shfl_xor(top, 32, kWave));
+      const float m_new = fmaxf(m[t], top);
+      const float f = m[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[t] - m_new);
+      m[t] = m_new;
+      l[t] *= f;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) o[t][d] *= f;
+    }
+    const float base = m[t] == -INFINITY ? 0.0f : m[t];
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) {
+      s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], sc, -base));
+      l[t] += s[e];
+    }
+  };
+  auto scores = [&](int t, const u32x4 (&k)[NTK][NP], float (&s)[EPL]) {
+#pragma unroll
+    for (int tk = 0; tk < NTK; ++tk) {
+      f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < NP; ++j) acc = tree_mma(T(), k[tk][j], q[t][j], acc);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[4 * tk + i] = acc[i];
+    }
+  };
+
+  // ---- the tree's own keys, chunks dealt over the splits' waves
+  for (int n0 = (wave * cut.splits + split) * CK; n0 < live; n0 += NW * cut.splits * CK) {
+    u32x4 k[NTK][NP], v[ND];
+#pragma unroll
+    for (int tk = 0; tk < NTK; ++tk) {
+      const int node = min(n0 + EPL * (c / 4) + 4 * tk + c % 4, live - 1);
+      tree_row_pieces<T, D>(a, rows + node * a.token_stride + (int64_t)(a.H + hk) * D, (int64_t)r.past + depth[node], g, k[tk]);
+    }
+    // V rows are tokens here: a piece's keys are gathered
+    const T *vrows = rows + (int64_t)(a.H + a.Hkv + hk) * D;
+    bool finite = true;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      float x[EPL];
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) {
+        x[e] = to_f32(vrows[min(n0 + EPL * g + e, live - 1) * a.token_stride + 16 * d + c]);
+        finite &= fabsf(x[e]) < INFINITY;
+      }
+      v[d] = tree_pack(x);
+    }
+    finite = __all(finite);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      if (t >= tiles) break;
+      float s[EPL];
+      scores(t, k, s);
+      const int qr = min(row0 + 16 * t + c, nrows - 1);
+      const uint64_t word = a.mask[b * a.mask_batch_stride + qr / G * a.mask_row_stride + n0 / 64];
+      const unsigned seen = (unsigned)(word >> (n0 % 64 + EPL * g));
+#pragma unroll
+      for (int e = 0; e < EPL; ++e)
+        if (!(seen >> e & 1) || n0 + EPL * g + e >= live) s[e] = -INFINITY;
+      weigh(t, s);
+      if (finite) {
+        const u32x4 p = tree_pack(s);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[t][d] = tree_mma(T(), v[d], p, o[t][d]);
+      } else {
+        // a value that is no number reaches the queries that see its node, and
+        // no other: 0 times it is left out, key by key
+        for (int key = 0; key < min(CK, live - n0); ++key) {
+          float pk = 0.0f;
+#pragma unroll
+          for (int e = 0; e < EPL; ++e) pk = key % EPL == e ? s[e] : pk;
+          pk = __shfl(pk, key / EPL * 16 + c, kWave);
+          if (pk == 0.0f) continue;
+          const T *vr = vrows + (n0 + key) * a.token_stride + 4 * g;
+#pragma unroll
+          for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[t][d][i] += pk * to_f32(vr[16 * d + i]);
+        }
+      }
+    }
+  }
+
+  // ---- the cached keys: this split's chunks, dealt over its waves
+  const int chunks = (past + CK - 1) / CK, per = (chunks + cut.splits - 1) / cut.splits;
+  const int end = min(chunks, (split + 1) * per);
+  const int64_t tile = (int64_t)a.bs * D, stride = tile * a.Hkv;
+  const T *kp = (const T *)a.k_pool + hk * tile, *vp = (const T *)a.v_pool + hk * tile;
+  const int last_run = (past - 1) & ~(EPL - 1);
+  struct Where {
+    int k_id, v_id, k_slot, v_slot;
+  };
+  auto block_of = [&](int key, int &slot) {
+    const int j = shift >= 0 ? key >> shift : key / a.bs;
+    slot = key - j * a.bs;
+    return table[j];
+  };
+  auto where = [&](int ch) {
+    Where w;
+    w.k_id = block_of(min(ch * CK + EPL * (c / 4), last_run), w.k_slot);
+    w.v_id = block_of(min(ch * CK + EPL * g, last_run), w.v_slot);
+    return w;
+  };
+  struct Pieces {
+    u32x4 k[NTK][NP], v[ND];
+  };
+  auto load = [&](const Where &w, Pieces &x) {
+    bad |= (unsigned)w.k_id >= (unsigned)a.num_blocks || (unsigned)w.v_id >= (unsigned)a.num_blocks;
+    const unsigned most = a.num_blocks - 1;
+    const T *k = kp + min((unsigned)w.k_id, most) * stride + (int64_t)(w.k_slot + c % 4) * D + EPL * g;
+    const T *v = vp + min((unsigned)w.v_id, most) * stride + (int64_t)c * a.bs + w.v_slot;
+#pragma unroll
+    for (int tk = 0; tk < NTK; ++tk)
+#pragma unroll
+      for (int j = 0; j < NP; ++j) x.k[tk][j] = *(const u32x4 *)(k + 4 * tk * D + CK * j);
+#pragma unroll
+    for (int d = 0; d < ND; ++d) x.v[d] = *(const u32x4 *)(v + (int64_t)16 * d * a.bs);
+  };
+  auto compute = [&](int ch, Pieces &x) {
+    const int left = past - ch * CK - EPL * g;  // keys of this lane's V piece that there are, or more
+    const bool edge = (ch + 1) * CK > past;
+    if (edge) {  // slots behind the cached length hold anything at all
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          if constexpr (sizeof(T) == 2)
+            x.v[d][w] = 2 * w + 1 < left ? x.v[d][w] : 2 * w < left ? x.v[d][w] & 0xFFFFu : 0u;
+          else
+            x.v[d][w] = w < left ? x.v[d][w] : 0u;
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      if (t >= tiles) break;
+      float s[EPL];
+      scores(t, x.k, s);
+      if (edge) {
+#pragma unroll
+        for (int e = 0; e < EPL; ++e)
+          if (e >= left) s[e] = -INFINITY;
+      }
+      weigh(t, s);
+      const u32x4 p = tree_pack(s);
+#pragma unroll
+      for (int d = 0; d < ND; ++d) o[t][d] = tree_mma(T(), x.v[d], p, o[t][d]);
+    }
+  };
+  int ch = split * per + wave;
+  if (ch < end) {
+    // block ids two chunks ahead of the products, K and V one
+    Pieces x0, x1;
+    load(where(ch), x0);
+    Where w = where(min(ch + NW, end - 1));
+    while (true) {
+      if (ch + NW >= end) {
+        compute(ch, x0);
+        break;
+      }
+      load(w, x1);
+      w = where(min(ch + 2 * NW, end - 1));
+      compute(ch, x0);
+      ch += NW;
+      if (ch + NW >= end) {
+        compute(ch, x1);
+        break;
+      }
+      load(w, x0);
+      w = where(min(ch + 2 * NW, end - 1));
+      compute(ch, x1);
+      ch += NW;
+    }
+  }
+
+  // ---- fold the waves, MT tiles at a time
+  bad = __any(bad);
+  const TreeParts parts = tree_parts(ws, unit, units, cut.rows(), D);
+#pragma unroll
+  for (int t0 = 0; t0 < NT; t0 += MT) {
+    if (t0 >= tiles) break;
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < MT; ++u) {
+      const int t = t0 + u;
+      float sum = l[t] + __shfl_xor(l[t], 16, kWave);
+      sum += __shfl_xor(sum, 32, kWave);
+      if (g == 0) {
+        s_ml[wave][u][c][0] = m[t];
+        s_ml[wave][u][c][1] = bad ? NAN : sum;
+      }
+#pragma unroll
+      for (int d = 0; d < ND; ++d) *(f32x4 *)&s_o[wave][u][c][16 * d + 4 * g] = o[t][d];
+    }
+    __syncthreads();
+    for (int x = tid; x < MT * 16 * (D / 4); x += NW * kWave) {
+      const int u = x / (4 * D), rr = x / (D / 4) % 16, d = x % (D / 4) * 4;
+      const int qr = row0 + 16 * (t0 + u) + rr;
+      if (qr >= nrows) continue;
+      float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) top = fmaxf(top, s_ml[w][u][rr][0]);
+      f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float mw = s_ml[w][u][rr][0], f = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - top);
+        const float lw = s_ml[w][u][rr][1];
+        sum += mw == -INFINITY ? lw : lw * f;  // 0, or NaN
+        acc += f * *(const f32x4 *)&s_o[w][u][rr][d];
+      }
+      if (cut.splits > 1) {
+        *(f32x4 *)&parts.o[(int64_t)qr * D + d] = acc;
+        if (d == 0) {
+          parts.ml[qr * 2] = top;
+          parts.ml[qr * 2 + 1] = sum;
+        }
+      } else {
+        T *out = (T *)a.out + b * a.out_batch_stride + qr / G * a.out_token_stride + (int64_t)(hk * G + qr % G) * D + d;
+        const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out[i] = from_f32<T>(sum != 0.0f ? acc[i] * inv : 0.0f);
+      }
+    }
+  }
+}
+
+// Folds the splits' partials, D / 4 lanes a query row.
+template <typename T, int D> __global__ __launch_bounds__(256) void tree_fold_kernel(TreeArgs a, TreeCut cut, float *ws) {
+  constexpr int LANES = D / 4, PER = 256 / LANES;
+  const int b = blockIdx.z, hk = blockIdx.y, G = a.H / a.Hkv, S = cut.splits;
+  const int qr = blockIdx.x * PER + threadIdx.x / LANES, d = threadIdx.x % LANES * 4;
+  const int live = min(a.meta[2 * a.batch + b], a.nodes);
+  if (qr >= (live - a.first) * G) return;
+  const int64_t units = (int64_t)a.batch * a.Hkv * S, unit0 = ((int64_t)b * a.Hkv + hk) * S, rows = cut.rows();
+  float top = -INFINITY, sum = 0.0f;
+  for (int s = 0; s < S; ++s) top = fmaxf(top, tree_parts(ws, unit0 + s, units, rows, D).ml[qr * 2]);
+  f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < S; ++s) {
+    const TreeParts p = tree_parts(ws, unit0 + s, units, rows, D);
+    const float ms = p.ml[qr * 2], ls = p.ml[qr * 2 + 1];
+    const float f = ms == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ms - top);
+    sum += ms == -INFINITY ? ls : ls * f;
+    acc += f * *(const f32x4 *)&p.o[(int64_t)qr * D + d];
+  }
+  T *out = (T *)a.out + b * a.out_batch_stride + qr / G * a.out_token_stride + (int64_t)(hk * G + qr % G) * D + d;
+  const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) out[i] = from_f32<T>(sum != 0.0f ? acc[i] * inv : 0.0f);
+}
+
+// Cut of a call whose rows hold up to max_kv cached keys.
+inline TreeCut tree_cut(int batch, int queries, int H, int Hkv, int d, int dtype, int max_kv) {
+  const int rows = queries * (H / Hkv), need = (rows + 15) / 16;
+  TreeCut cut;
+  cut.tiles = need <= 1 ? 1 : need <= 2 || d == 128 ? 2 : 4;
+  cut.groups = (need + cut.tiles - 1) / cut.tiles;
+  const int ck = dtype == SPECDEC_BF16 ? 32 : 16, chunks = (max_kv + ck - 1) / ck;
+  const int64_t units = (int64_t)batch * Hkv * cut.groups;
+  int64_t splits = (1024 + units - 1) / units;
+  splits = splits < chunks / kTreeWaves ? splits : chunks / kTreeWaves;
+  cut.splits = (int)(splits < 1 ? 1 : splits > 64 ? 64 : splits);
+  return cut;
+}
+inline int64_t tree_floats(const TreeCut &cut, int batch, int Hkv, int d) {
+  return cut.splits > 1 ? (int64_t)batch * Hkv * cut.splits * cut.rows() * (d + 2) : 0;
+}
+
 // ------------------------------------------------------------------ commit --
 struct CommitArgs {
   const int64_t *tokens, *sampled;
@@ -250,10 +685,37 @@ template <typename T> __global__ __launch_bounds__(kCommitThreads) void tree_com
   }
 }
 
-template <typename T> int launch_tree_attention(const TreeArgs &a, int d, hipStream_t s) {
+template <typename T, int D> int launch_tree_tiles(const TreeArgs &a, const TreeCut &cut, float *ws, hipStream_t s) {
+  const int64_t units = (int64_t)a.batch * a.Hkv * cut.splits;
+  const int64_t grid = cut.groups > 1 ? (units + 7) / 8 * 8 * cut.groups : units;
+  if (grid > INT32_MAX) return SPECDEC_EUNSUPPORTED;
+  int shift = 0;
+  while (1 << shift < a.bs) ++shift;
+  if (1 << shift != a.bs) shift = -1;
+  const dim3 block(kTreeWaves * kWave);
+  if (cut.tiles == 1) tree_attention_kernel<T, D, 1><<<(unsigned)grid, block, 0, s>>>(a, cut, shift, ws);
+  else if (cut.tiles == 2) tree_attention_kernel<T, D, 2><<<(unsigned)grid, block, 0, s>>>(a, cut, shift, ws);
+  else if constexpr (D == 64) tree_attention_kernel<T, D, 4><<<(unsigned)grid, block, 0, s>>>(a, cut, shift, ws);
+  if (cut.splits > 1) {
+    const int rows = (a.nodes - a.first) * (a.H / a.Hkv), per = 256 / (D / 4);
+    tree_fold_kernel<T, D><<<dim3((rows + per - 1) / per, a.Hkv, a.batch), 256, 0, s>>>(a, cut, ws);
+  }
+  return launch_status();
+}
+
+template <typename T, int D>
+int launch_tree_attention(const TreeArgs &a, int dtype, int max_kv, float *ws, int64_t floats, hipStream_t s) {
+  // pieces of 16 bytes: rows, tables and pools aligned, blocks of whole pieces
+  constexpr int EPL = 16 / (int)sizeof(T);
+  const auto aligned = [](const void *p) { return (uintptr_t)p % 16 == 0; };
+  if (aligned(a.qkv) && a.batch_stride % EPL == 0 && a.token_stride % EPL == 0 && aligned(a.cos_t) && aligned(a.sin_t) &&
+      aligned(a.k_pool) && aligned(a.v_pool) && a.bs % EPL == 0) {
+    TreeCut cut = tree_cut(a.batch, a.nodes - a.first, a.H, a.Hkv, D, dtype, max_kv);
+    if (tree_floats(cut, a.batch, a.Hkv, D) > floats || !ws || !aligned(ws)) cut.splits = 1;
+    return launch_tree_tiles<T, D>(a, cut, ws, s);
+  }
   const dim3 grid((unsigned)(a.nodes - a.first), (unsigned)a.H, (unsigned)a.batch);
-  if (d == 64) tree_attention_any_kernel<T, 64><<<grid, kWave, 0, s>>>(a);
-  else tree_attention_any_kernel<T, 128><<<grid, kWave, 0, s>>>(a);
+  tree_attention_any_kernel<T, D><<<grid, kWave, 0, s>>>(a);
   return launch_status();
 }
 
@@ -267,8 +729,12 @@ SPECDEC_API int specdec_tree_attention_workspace(int32_t batch, int32_t nodes, i
   if (batch < 0 || nodes < 0 || first < 0 || first > nodes || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads ||
       head_dim <= 0 || block_size <= 0 || max_kv_len < 0 || !floats)
     return SPECDEC_EINVAL;
-  (void)dtype;
-  *floats = 0;
+  if (head_dim != 64 && head_dim != 128) return SPECDEC_EUNSUPPORTED;
+  if (dtype != SPECDEC_F32 && dtype != SPECDEC_BF16) return SPECDEC_EUNSUPPORTED;
+  if (nodes > kTreeMaxNodes) return SPECDEC_EUNSUPPORTED;
+  *floats = batch == 0 || nodes == first ? 0
+            : tree_floats(tree_cut(batch, nodes - first, n_heads, n_kv_heads, head_dim, dtype, max_kv_len), batch,
+                          n_kv_heads, head_dim);
   return SPECDEC_OK;
 }
 
@@ -297,13 +763,17 @@ SPECDEC_API int specdec_tree_attention(const void *qkv, int dtype, int64_t batch
   // a cache of no block or no table can hold rows of no cached position alone
   if (num_blocks == 0 || table_rows == 0) table_cols = 0;
   if (table_cols > 0 && (!k_pool || !v_pool || !tables)) return SPECDEC_EINVAL;
-  (void)workspace;
   TreeArgs a{qkv, batch_stride, token_stride, cos_table, sin_table, (int)max_positions, k_pool, v_pool, (int)num_blocks,
              tables, table_stride, table_rows, table_cols, meta, mask, mask_batch_stride, mask_row_stride, depth,
              depth_batch_stride, batch, nodes, first, n_heads, n_kv_heads, block_size, scale, out, out_batch_stride,
              out_token_stride};
-  if (dtype == SPECDEC_F32) return launch_tree_attention<float>(a, head_dim, as_stream(stream));
-  return launch_tree_attention<__hip_bfloat16>(a, head_dim, as_stream(stream));
+  const hipStream_t s = as_stream(stream);
+  if (dtype == SPECDEC_F32)
+    return head_dim == 64 ? launch_tree_attention<float, 64>(a, dtype, max_kv_len, workspace, workspace_floats, s)
+                          : launch_tree_attention<float, 128>(a, dtype, max_kv_len, workspace, workspace_floats, s);
+  return head_dim == 64
+             ? launch_tree_attention<__hip_bfloat16, 64>(a, dtype, max_kv_len, workspace, workspace_floats, s)
+             : launch_tree_attention<__hip_bfloat16, 128>(a, dtype, max_kv_len, workspace, workspace_floats, s);
 }
 
 SPECDEC_API int specdec_tree_commit(const int64_t *tokens, int64_t tokens_stride, const int32_t *parents,
