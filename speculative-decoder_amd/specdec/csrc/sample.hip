@@ -7,23 +7,40 @@
 // first top_k.  The token is the least id whose running sum of kept weights, in
 // the order of ids, exceeds u times their total.
 //
-// A prefix of the order is a cut (key, ties): every id whose key is higher, and
-// the first `ties` of those that have it, the key being the logit's bits in an
-// order that integers compare.  So no row is sorted: a cut is found by halving
-// the range of keys, counting (top-k) or adding up weights (top-p) above the
-// middle.
+// A prefix of the order is a cut (x, id): every larger logit, and the equal ones
+// up to that id.  No row is sorted as a whole.  One workgroup takes a row:
+//   1. It reads the row once, a wave a contiguous range.  The largest logits of
+//      its threads in the first part bound the k-th largest of the row from below
+//      (k of them are k logits), so what reaches that bound is collected in LDS on
+//      the way, together with the maximum and the sum of weights.
+//   2. The few hundred collected are ranked by counting; running sums over them
+//      give the cuts, and over their ids the token.  Most rows end here.
+//   3. A cut that is not among them (a nucleus of thousands of ids, a large
+//      top-k) is found by a histogram of the row over 2048 ranges of x, of counts
+//      or of weights, then by ranking the range that the cut falls into; the
+//      row is read again for each, mostly from the last-level cache.
+//   4. Without a cut, or past one, the sums of the waves' ranges say which range
+//      the token is in, and a scan of that range which id it is.
 //
 // Weights and their sums are held in 64 bits: a token is a comparison of u's
 // multiple of the total with a running sum of up to 2^18 weights, and in 32 bits
 // about one row in a hundred of a wide distribution would get the token beside.
+// A histogram's sums are integers, so their order does not matter: a weight in
+// units of 2^-45 of the largest that its range can hold.
 #include "common.h"
 
+#include <float.h>
+#include <limits.h>
 #include <math.h>
 
 namespace specdec {
 
-constexpr int kSampleThreads = 1024;
-constexpr int kSampleWaves = kSampleThreads / kWave;
+constexpr int kSamplePieces = 6;    // pieces of 16 bytes of a part; the next part's are in flight
+constexpr int kSampleRaw = 2048;    // logits that are collected, each wave its share
+constexpr int kSampleMost = 1024;   // logits that are ranked at once
+constexpr int kSampleBins = 2048;
+constexpr int kSampleTopK = 400;    // the largest top_k that is bounded by the threads' maxima
+constexpr int kSampleGuess = 128;   // reach the bound in the first part, for a nucleus of unknown size
 
 struct SampleArgs {
   const void *logits;
@@ -39,11 +56,8 @@ struct SampleArgs {
   int64_t probs_stride;
 };
 
-// Bits of x in an order that unsigned integers compare as floats do; both zeros
-// are one value, a NaN is -inf.
-constexpr unsigned kKeyNegInf = 0x007FFFFFu;  // the key of -inf
+// Bits of x in an order that unsigned integers compare as floats do; both zeros are one value.
 __device__ __forceinline__ unsigned sample_key(float x) {
-  if (x != x) return kKeyNegInf;
   const unsigned b = __float_as_uint(x + 0.0f);
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
@@ -51,141 +65,772 @@ __device__ __forceinline__ float sample_value(unsigned key) {
   return __uint_as_float((key & 0x80000000u) ? (key & 0x7FFFFFFFu) : ~key);
 }
 
-// w of the value with this key; the largest weighs 1 whatever it is (+inf too)
-__device__ __forceinline__ double sample_weight(unsigned key, unsigned top, double inv_t) {
-  if (key == top) return 1.0;
-  const double d = (double)sample_value(key) - (double)sample_value(top);
-  return d > -INFINITY ? exp(d * inv_t) : 0.0;
+// a b + c with c in scalar registers: as an accumulation hipcc copies each
+// coefficient to vector registers first
+__device__ __forceinline__ double sample_fma(double a, double b, double c) {
+  double r;
+  __asm__("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "s"(c));
+  return r;
 }
 
+// w[k] = 2^((e[k] - base) c) within 4e-14 relative, for powers up to 1000; at
+// least 2^-1000.  2^n by the exponent's bits; 2^f, |f| <= 1/2, as 1 + f q(f), q of
+// the 8th power through (2^f - 1) / f at the 9 Chebyshev points, so 2^0 is 1.  N
+// side by side: the chain of one takes its latency 17 times.
+template <int N> __device__ __forceinline__ void sample_weights(const float (&e)[N], double base, double c, double (&w)[N]) {
+  constexpr double magic = 6755399441055744.0;  // 1.5 2^52: n in the low bits of a sum
+  double f[N];
+  int n[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const double y = fmax(((double)e[k] - base) * c, -1000.0);
+    const double t = y + magic;
+    n[k] = (int)__double2loint(t);
+    f[k] = y - (t - magic);
+    w[k] = 1.0203121063391729e-07;
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k) w[k] = sample_fma(w[k], f[k], 1.3255224878668817e-06);
+#pragma unroll
+  for (int k = 0; k < N; ++k) w[k] = sample_fma(w[k], f[k], 1.525268684626772e-05);
+#pragma unroll
+  for (int k = 0; k < N; ++k) w[k] = sample_fma(w[k], f[k], 0.00015403455852453838);
+#pragma unroll
+  for (int k = 0; k < N; ++k) w[k] = sample_fma(w[k], f[k], 0.0013333558179043112);
+#pragma unroll
+  for (int k = 0; k < N; ++k) w[k] = sample_fma(w[k], f[k], 0.009618129159402558);
+#pragma unroll
+  for (int k = 0; k < N; ++k) w[k] = sample_fma(w[k], f[k], 0.055504108664760424);
+#pragma unroll
+  for (int k = 0; k < N; ++k) w[k] = sample_fma(w[k], f[k], 0.2402265069581299);
+#pragma unroll
+  for (int k = 0; k < N; ++k) w[k] = sample_fma(w[k], f[k], 0.6931471805599453);
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    w[k] = fma(w[k], f[k], 1.0);
+    w[k] = __hiloint2double(__double2hiint(w[k]) + (n[k] << 20), __double2loint(w[k]));
+  }
+}
+__device__ __forceinline__ double sample_weight(float v, double base, double c) {
+  const float e[1] = {v};
+  double w[1];
+  sample_weights(e, base, c, w);
+  return w[0];
+}
+
+// What is kept: larger logits, and the equal ones up to an id.
 struct Cut {
-  unsigned key;
-  int ties;
+  float x;
+  int id;
+  __device__ bool keeps(float v, int i) const { return v > x || (v == x && i <= id); }
 };
 __device__ __forceinline__ Cut shorter(Cut a, Cut b) {
-  if (a.key != b.key) return a.key > b.key ? a : b;
-  return a.ties < b.ties ? a : b;
+  if (a.x != b.x) return a.x > b.x ? a : b;
+  return a.id < b.id ? a : b;
 }
 
-template <typename T>
-__global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
-  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & (kWave - 1);
-  const T *x = (const T *)a.logits + row * a.row_stride;
+// A row of logits as a workgroup reads it: pieces of 16 aligned bytes, wave w
+// the pieces (w per + j) 64 + lane, j < per.  They come through a buffer resource,
+// whose bounds stand for the row's ends: up to the 16 bytes that hold its first
+// and last logit, and what is not of the row is put to -inf when it is unpacked.
+template <typename T, int THREADS> struct SampleRow {
+  static constexpr int EPL = 16 / sizeof(T);
+  const T *x;
+  int V, lead, per;  // lead: elements of the first piece that belong to the row before
+  __amdgpu_buffer_rsrc_t rows;
+  unsigned offset;   // of this thread's first piece
+  bool infinite;     // the row has +inf: those weigh the same, the others nothing
+
+  __device__ SampleRow(const void *logits, int64_t first, int vocab) : x((const T *)logits + first), V(vocab), infinite(false) {
+    lead = (int)((uintptr_t)x % 16 / sizeof(T));
+    const int pieces = (lead + V + EPL - 1) / EPL;
+    per = (pieces + THREADS - 1) / THREADS;
+    rows = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(x - lead), 0, pieces * 16, 0x00020000);
+    offset = ((threadIdx.x / kWave) * per * kWave + (threadIdx.x & (kWave - 1))) * 16u;
+  }
+  __device__ int id0(int j) const { return (int)(offset / 16 + j * kWave) * EPL - lead; }  // id of the first element of piece j
+  __device__ u32x4 piece(int j) const {
+    return __builtin_amdgcn_raw_buffer_load_b128(rows, j < per ? offset + j * (kWave * 16u) : 0xFFFFFF00u, 0, 0);
+  }
+  __device__ float value(float v) const {
+    v = fmaxf(v, -INFINITY);  // a NaN is -inf
+    return infinite ? (v == INFINITY ? 0.0f : -INFINITY) : v;
+  }
+  __device__ void unpack(u32x4 v, int j, float (&e)[EPL]) const {
+#pragma unroll
+    for (int k = 0; k < EPL; ++k) {
+      if constexpr (sizeof(T) == 4) e[k] = fmaxf(__uint_as_float(v[k]), -INFINITY);
+      else e[k] = fmaxf(__uint_as_float((k & 1) ? v[k / 2] & 0xFFFF0000u : v[k / 2] << 16), -INFINITY);
+    }
+    const int i = id0(j);
+    if (infinite || i < 0 || i + EPL > V) {
+#pragma unroll
+      for (int k = 0; k < EPL; ++k) e[k] = i + k >= 0 && i + k < V ? value(e[k]) : -INFINITY;
+    }
+  }
+  __device__ float at(int i) const { return value(to_f32(x[i])); }
+  __device__ void load(u32x4 (&v)[kSamplePieces], int j0) const {
+#pragma unroll
+    for (int k = 0; k < kSamplePieces; ++k) v[k] = piece(j0 + k);
+  }
+  // f(v, first piece) over this thread's pieces, a part at a time, the next one in flight
+  template <typename F> __device__ void parts(F &&f) const {
+    u32x4 v0[kSamplePieces], v1[kSamplePieces];
+    load(v0, 0);
+    for (int j = 0;;) {
+      load(v1, j + kSamplePieces);
+      f(v0, j);
+      if ((j += kSamplePieces) >= per) break;
+      load(v0, j + kSamplePieces);
+      f(v1, j);
+      if ((j += kSamplePieces) >= per) break;
+    }
+  }
+  // f(e, id of e[0]) over this thread's pieces, to read the row again
+  template <typename F> __device__ void again(F &&f) const {
+#pragma unroll 1
+    for (int j0 = 0; j0 < per; j0 += kSamplePieces) {
+      u32x4 v[kSamplePieces];
+      load(v, j0);
+#pragma unroll
+      for (int k = 0; k < kSamplePieces; ++k) {
+        if (j0 + k >= per) break;
+        float e[EPL];
+        unpack(v[k], j0 + k, e);
+        f(e, id0(j0 + k));
+        __builtin_amdgcn_sched_barrier(0);  // one piece's 64-bit values in registers at a time
+      }
+    }
+  }
+};
+
+template <int THREADS> struct SampleShared {
+  static constexpr int WAVES = THREADS / kWave, SHARE = kSampleRaw / WAVES;
+  union {
+    uint64_t raw[WAVES][SHARE];  // as collected: the order of logits, then falling id
+    uint64_t bins[kSampleBins];
+  };
+  uint64_t found[kSampleMost];  // ranked
+  union {
+    struct {
+      double weight[kSampleMost], before[kSampleMost];  // of the ranked, and the sum before each
+    };
+    short unit[kSampleBins];
+  };
+  float tops[THREADS];
+  double wave_d[2][WAVES];
+  float wave_f[2][WAVES];
+  int wave_n[WAVES];
+  uint64_t sums[kWave];
+  int near[kWave];
+  double above;
+  int count, token, last, keep_p, keep_m;
+  unsigned lo, hi;
+};
+
+// Reductions over the workgroup with one barrier each: a reduction's slots are
+// written again two reductions later, past another barrier.
+template <int THREADS> struct SampleBlock {
+  static constexpr int WAVES = THREADS / kWave;
+  SampleShared<THREADS> &s;
+  int turn = 0;
+  __device__ double sum(double v) {
+    v = wave_sum(v);
+    turn ^= 1;
+    if ((threadIdx.x & (kWave - 1)) == 0) s.wave_d[turn][threadIdx.x / kWave] = v;
+    __syncthreads();
+    v = 0.0;
+    for (int w = 0; w < WAVES; ++w) v += s.wave_d[turn][w];
+    return v;
+  }
+  __device__ float max(float v) {
+    v = wave_max_dpp(v);
+    turn ^= 1;
+    if ((threadIdx.x & (kWave - 1)) == 0) s.wave_f[turn][threadIdx.x / kWave] = v;
+    __syncthreads();
+    v = s.wave_f[turn][0];
+    for (int w = 1; w < WAVES; ++w) v = fmaxf(v, s.wave_f[turn][w]);
+    return v;
+  }
+  // exclusive prefix over the threads
+  __device__ double scan(double v) {
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    double x = v;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+      const double y = __shfl_up(x, o, kWave);
+      if (lane >= o) x += y;
+    }
+    turn ^= 1;
+    if (lane == kWave - 1) s.wave_d[turn][wave] = x;
+    __syncthreads();
+    double before = 0.0;
+    for (int w = 0; w < wave; ++w) before += s.wave_d[turn][w];
+    double e = __shfl_up(x, 1, kWave);
+    if (lane == 0) e = 0.0;
+    return before + e;
+  }
+};
+
+// A bound that `want` of the threads' maxima in s.tops reach, and not many more:
+// halving between the least and the largest, in each wave for itself.  -FLT_MAX
+// where fewer are finite.
+template <int THREADS> __device__ __forceinline__ float sample_bound(const SampleShared<THREADS> &s, int want) {
+  constexpr int N = THREADS / kWave;
+  const int lane = threadIdx.x & (kWave - 1);
+  float v[N], lo = FLT_MAX, hi = -FLT_MAX;
+  int n = 0;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    v[k] = s.tops[k * kWave + lane];
+    n += __popcll(__ballot(v[k] >= -FLT_MAX));
+    lo = fminf(lo, v[k] >= -FLT_MAX ? v[k] : FLT_MAX);
+    hi = fmaxf(hi, v[k]);
+  }
+  if (n < want) return -FLT_MAX;
+  lo = -wave_max_dpp(-lo);
+  hi = fminf(wave_max_dpp(hi), FLT_MAX);
+#pragma unroll 1
+  for (int step = 0; step < 7; ++step) {
+    const float mid = 0.5f * lo + 0.5f * hi;
+    int reach = 0;
+#pragma unroll
+    for (int k = 0; k < N; ++k) reach += __popcll(__ballot(v[k] >= mid));
+    if (reach >= want) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// s.found[0 .. n) from the largest to the least: a bitonic network over the next
+// power of two.  A wave's 64 pairs up to 64 apart are 128 elements of its own, so
+// those steps need no barrier.
+template <int THREADS> __device__ __forceinline__ void sample_sort(SampleShared<THREADS> &s, int n) {
+  const int tid = threadIdx.x;
+  int size = 128;
+  while (size < n) size <<= 1;
+  for (int q = n + tid; q < size; q += THREADS) s.found[q] = 0;
+  __syncthreads();
+  volatile uint64_t *x = s.found;
+  for (int k = 2; k <= size; k <<= 1)
+    for (int j = k / 2; j > 0; j >>= 1) {
+      if (tid < size / 2) {
+        const int lo = 2 * tid - (tid & (j - 1)), hi = lo + j;
+        const uint64_t a = x[lo], b = x[hi];
+        if ((a < b) == ((lo & k) == 0 || k == size)) {
+          x[lo] = b;
+          x[hi] = a;
+        }
+      }
+      const int next = j > 1 ? j / 2 : k;  // the next step's distance
+      if (j > 64 || next > 64) __syncthreads();
+      else __builtin_amdgcn_wave_barrier();
+    }
+  __syncthreads();
+}
+
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4))) void sample_kernel(SampleArgs a) {
+  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+  constexpr int EPL = 16 / sizeof(T), WAVES = THREADS / kWave, SHARE = kSampleRaw / WAVES;
+  __shared__ SampleShared<THREADS> s;
+  SampleBlock<THREADS> block{s};
+  SampleRow<T, THREADS> x(a.logits, row * a.row_stride, a.vocab);
   const int V = a.vocab;
-  __shared__ double dscratch[kSampleWaves + 1];
-  __shared__ int iscratch[kSampleWaves + 1];
-  __shared__ int found;
 
   const float t_row = a.temperatures ? a.temperatures[row] : a.temperature;
   const float p_row = a.top_ps ? a.top_ps[row] : a.top_p;
   const float m_row = a.min_ps ? a.min_ps[row] : a.min_p;
   const int k_given = a.top_ks ? a.top_ks[row] : a.top_k;
   const bool greedy = !(t_row > 0.0f);
-  const int k_row = greedy ? 1 : k_given;
-  const double inv_t = greedy ? 1.0 : 1.0 / (double)t_row;
+  const int k_row = !greedy && k_given > 0 && k_given < V ? k_given : 0;
+  const bool by_p = !greedy && p_row < 1.0f, by_m = !greedy && m_row > 0.0f;
+  const double p = fmax((double)p_row, 0.0), m = fmin((double)m_row, 1.0);
+  const double c = greedy ? 0.0 : 1.4426950408889634074 / (double)t_row;
   const float uu = a.u[row];
   const double u = uu > 0.0f ? (double)fminf(uu, 1.0f) : 0.0;
+  float *probs = a.probs ? a.probs + row * a.probs_stride : nullptr;
 
-  auto key_at = [&](int i) { return sample_key(to_f32(x[i])); };
-  auto count_above = [&](unsigned k) {  // ids whose key is higher
-    int n = 0;
-    for (int i = tid; i < V; i += kSampleThreads) n += key_at(i) > k;
-    return block_sum(n, iscratch);
+  // ---- 1: the row once
+  // few: some hundred logits hold the cut, as far as can be said before the row is read
+  const bool few = !greedy && ((k_row > 0 && k_row <= kSampleTopK) || (k_row == 0 && (by_p || by_m)));
+  const int want = k_row > 0 ? k_row : kSampleGuess;
+  const bool weigh = !greedy && k_row == 0 && (by_p || !by_m);  // the sum of all weights is asked for
+  float top, bound;
+  double mass, base;  // this thread's weights against `base`
+  int top_j;          // this thread's first piece that has its largest logit
+  int collected;      // by this wave; past its share they are only counted
+  const auto collect = [&](const float(&e)[EPL], int i) {
+#pragma unroll
+    for (int q = 0; q < EPL; ++q) {
+      const uint64_t hits = __ballot(e[q] >= bound);
+      const int at = collected + (int)__builtin_amdgcn_mbcnt_hi((unsigned)(hits >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)hits, 0));
+      if (e[q] >= bound && at < SHARE) s.raw[wave][at] = (uint64_t)sample_key(e[q]) << 32 | (unsigned)~(i + q);
+      collected += __popcll(hits);
+    }
   };
-
-  unsigned top = 0;
-  for (int i = tid; i < V; i += kSampleThreads) top = max(top, key_at(i));
-  top = (unsigned)block_max((double)top, dscratch);
-  if (top <= kKeyNegInf) {  // no candidate
+  while (true) {
+    top = -INFINITY;
+    bound = INFINITY;
+    mass = base = 0.0;
+    top_j = collected = 0;
+    if (tid == 0) {
+      s.token = V;
+      s.last = -1;
+      s.keep_p = s.keep_m = 1;
+    }
+    x.parts([&](const u32x4(&v)[kSamplePieces], int j0) {
+      float part[kSamplePieces];
+#pragma unroll
+      for (int k = 0; k < kSamplePieces; ++k) {
+        part[k] = -INFINITY;
+        if (j0 + k < x.per) {
+          float e[EPL];
+          x.unpack(v[k], j0 + k, e);
+          part[k] = e[0];
+#pragma unroll
+          for (int q = 1; q < EPL; ++q) part[k] = fmaxf(part[k], e[q]);
+        }
+        if (part[k] > top) top_j = j0 + k;
+        top = fmaxf(top, part[k]);
+      }
+      if (j0 == 0 && (few || weigh)) {
+        // weights are taken against the largest logit of the first part: 64
+        // bits have room for what is larger after it
+        s.tops[tid] = top;
+        base = (double)block.max(top);
+        if (few) bound = sample_bound(s, want);
+      }
+      if (few) {
+#pragma unroll
+        for (int k = 0; k < kSamplePieces; ++k)
+          if (__any(part[k] >= bound)) {
+            float e[EPL];
+            x.unpack(v[k], j0 + k, e);
+            collect(e, x.id0(j0 + k));
+          }
+      }
+      if (weigh) {
+#pragma unroll
+        for (int k = 0; k < kSamplePieces; ++k) {
+          if (j0 + k >= x.per) break;
+          float e[EPL];
+          double w[EPL];
+          x.unpack(v[k], j0 + k, e);
+          sample_weights(e, base, c, w);
+#pragma unroll
+          for (int q = 0; q < EPL; ++q) mass += w[q];
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    });
+    const float own_top = top;
+    top = block.max(top);
+    if (few) {
+      s.tops[tid] = own_top;
+      if (lane == 0) s.wave_n[wave] = collected;
+    }
+    if (greedy && own_top == top && top > -INFINITY && top < INFINITY) {
+      float e[EPL];
+      x.unpack(x.piece(top_j), top_j, e);
+      int first = EPL;
+#pragma unroll
+      for (int q = EPL - 1; q >= 0; --q)
+        if (e[q] == top) first = q;
+      atomicMin(&s.token, x.id0(top_j) + first);
+    }
+    if (top < INFINITY) break;
+    x.infinite = true;  // its largest is 0 the next time
+    __syncthreads();
+  }
+  if (top == -INFINITY) {  // no candidate
     if (tid == 0) a.token[row] = -1;
-    if (a.probs)
-      for (int i = tid; i < V; i += kSampleThreads) a.probs[row * a.probs_stride + i] = 0.0f;
+    if (probs)
+      for (int i = tid; i < V; i += THREADS) probs[i] = 0.0f;
     return;
   }
-  auto mass_above = [&](unsigned k, Cut within) {  // weight of ids whose key is higher than both
-    double m = 0.0;
-    for (int i = tid; i < V; i += kSampleThreads) {
-      const unsigned key = key_at(i);
-      if (key > k && key > within.key) m += sample_weight(key, top, inv_t);
-    }
-    return block_sum(m, dscratch);
+  if (greedy) {
+    __syncthreads();
+    const int token = s.token;
+    if (tid == 0) a.token[row] = token;
+    if (probs)
+      for (int i = tid; i < V; i += THREADS) probs[i] = i == token ? 1.0f : 0.0f;
+    return;
+  }
+  const double dtop = (double)top;
+  // the weights of a cut's ids, of this thread
+  const auto weights_within = [&](Cut cut) {
+    double sum = 0.0;
+    x.again([&](const float(&e)[EPL], int i) {
+      double w[EPL];
+      sample_weights(e, dtop, c, w);
+#pragma unroll
+      for (int q = 0; q < EPL; ++q) sum += cut.keeps(e[q], i + q) ? w[q] : 0.0;
+    });
+    return sum;
   };
-
-  // top-k: the highest key that fewer than k ids are above of, less one, bounds it
-  Cut cut{kKeyNegInf, 0};  // every id of weight
-  if (k_row > 0 && k_row < V) {
-    unsigned lo = kKeyNegInf, hi = top;  // count_above(hi) < k; the answer is in [lo, hi]
-    while (lo < hi) {
-      const unsigned mid = lo + (hi - lo) / 2;
-      if (count_above(mid) < k_row) hi = mid;
-      else lo = mid + 1;
-    }
-    cut = Cut{lo, k_row - count_above(lo)};
-    if (lo <= kKeyNegInf) cut = Cut{kKeyNegInf, 0};
+  const Cut all_ids{-FLT_MAX, INT_MAX};
+  // against the row's largest now, or again where the first part was too far from it
+  if (weigh) {
+    const double up = (base - dtop) * c;
+    if (up > -900.0 && up <= 0.0) mass *= exp2(up);
+    else mass = weights_within(all_ids);
   }
-  const Cut first_k = cut;
-  if (!greedy && p_row < 1.0f) {
-    const double w_cut = sample_weight(first_k.key, top, inv_t);
-    const double total = mass_above(kKeyNegInf, first_k) + first_k.ties * (first_k.key > kKeyNegInf ? w_cut : 0.0);
-    const double want = fmax((double)p_row, 0.0) * total;
-    unsigned lo = first_k.key, hi = top;  // the least key whose mass above is short of `want`
-    while (lo < hi) {
-      const unsigned mid = lo + (hi - lo) / 2;
-      if (mass_above(mid, first_k) < want) hi = mid;
-      else lo = mid + 1;
-    }
-    if (lo > kKeyNegInf) {
-      // of the ids with that key, those before which the mass is short of it
-      const double above = mass_above(lo, first_k), w = sample_weight(lo, top, inv_t);
-      const double more = ceil((want - above) / w);
-      cut = shorter(cut, Cut{lo, (int)fmin(fmax(more, 1.0), 2147483647.0)});
-    }
-  }
-  if (!greedy && m_row > 0.0f) {
-    unsigned lo = kKeyNegInf + 1, hi = top;  // the least key of weight min_p
-    while (lo < hi) {
-      const unsigned mid = lo + (hi - lo) / 2;
-      if (sample_weight(mid, top, inv_t) >= (double)m_row) hi = mid;
-      else lo = mid + 1;
-    }
-    cut = shorter(cut, Cut{lo, 2147483647});
+  double total = weigh ? block.sum(mass) : 0.0;
+  // the least logit of weight m: (x - top) c >= log2 m
+  float m_bound = -FLT_MAX;
+  if (by_m) {
+    const double border = dtop + log2(m) / c;
+    m_bound = (float)fmax(border, (double)-FLT_MAX);
+    if ((double)m_bound < border) m_bound = sample_value(sample_key(m_bound) + 1);
   }
 
-  // ties before an id are counted in the order of ids: threads own whole ranges
-  const int per = (V + kSampleThreads - 1) / kSampleThreads;
-  const int i0 = min(V, tid * per), i1 = min(V, i0 + per);
-  int same = 0, all_same;
-  for (int i = i0; i < i1; ++i) same += key_at(i) == cut.key;
-  const int before = block_exclusive_scan(same, iscratch, &all_same);
-  auto walk = [&](auto &&each) {  // each(id, weight) over this thread's ids
-    int tie = before;
-    for (int i = i0; i < i1; ++i) {
-      const unsigned key = key_at(i);
-      const bool kept = key > cut.key || (key == cut.key && tie < cut.ties);
-      tie += key == cut.key;
-      each(i, kept ? sample_weight(key, top, inv_t) : 0.0);
+  constexpr double unit52 = 4503599627370496.0;
+  // Ranks the n of s.found, with weights and the sums before each.
+  const auto rank = [&](int n) {
+    sample_sort(s, n);
+    constexpr int N = kSampleMost / THREADS;
+    double w[N], sum = 0.0;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int r = N * tid + k;
+      w[k] = r < n ? sample_weight(sample_value((unsigned)(s.found[r] >> 32)), dtop, c) : 0.0;
+      sum += w[k];
+    }
+    double run = block.scan(sum);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      s.weight[N * tid + k] = w[k];
+      s.before[N * tid + k] = run;
+      run += w[k];
+    }
+    __syncthreads();
+  };
+  const auto sorted_x = [&](int r) { return sample_value((unsigned)(s.found[r] >> 32)); };
+  const auto sorted_id = [&](int r) { return (int)~(unsigned)s.found[r]; };
+  // Of the first n ranked, how many have a mass before them (with `above`) short
+  // of `goal`: into s.keep_p, which holds 1.
+  const auto short_of = [&](int n, double above, double goal) {
+    for (int r = tid; r < n; r += THREADS)
+      if (above + s.before[r] < goal && (r + 1 == n || above + s.before[r + 1] >= goal)) s.keep_p = r + 1;
+  };
+
+  // ---- 2: the cut among the collected
+  int keep = 0;  // ranked ids kept, where the cut is among them
+  if (few) {
+    __syncthreads();
+    // the collected that reach `bound` to s.found; their number, or more than kSampleMost
+    const auto gather = [&]() {
+      const int have = s.wave_n[wave];
+      const unsigned least = sample_key(bound);
+      int mine = 0;
+      if (have <= SHARE)
+        for (int r = lane; r - lane < have; r += kWave) mine += __popcll(__ballot(r < have && (unsigned)(s.raw[wave][r] >> 32) >= least));
+      else mine = kSampleMost + 1;
+      if (lane == 0) s.near[wave] = mine;
+      __syncthreads();
+      int at = 0, n = 0;
+      for (int w = 0; w < WAVES; ++w) {
+        if (w < wave) at += s.near[w];
+        n += s.near[w];
+      }
+      if (n <= kSampleMost)
+        for (int r = lane; r - lane < have; r += kWave) {
+          const bool in = r < have && (unsigned)(s.raw[wave][r] >> 32) >= least;
+          const uint64_t hits = __ballot(in);
+          if (in)
+            s.found[at + (int)__builtin_amdgcn_mbcnt_hi((unsigned)(hits >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)hits, 0))] =
+                s.raw[wave][r];
+          at += __popcll(hits);
+        }
+      return n;
+    };
+    // by the maxima of the whole row the bound of a top-k is a tighter one
+    if (k_row > 0) bound = fmaxf(bound, sample_bound(s, want));
+    int n = gather();
+    if (n > kSampleMost) {  // the first part was not like the rest: again, by the maxima of the whole row
+      bound = sample_bound(s, want);
+      collected = 0;
+      x.again(collect);
+      __syncthreads();
+      if (lane == 0) s.wave_n[wave] = collected;
+      __syncthreads();
+      n = gather();
+    }
+    if (n <= kSampleMost) {
+      rank(n);
+      const int upto = k_row > 0 ? min(k_row, n) : n;
+      const double all = s.before[upto - 1] + s.weight[upto - 1];
+      if (k_row > 0) total = all;
+      if (by_p) short_of(upto, 0.0, p * total);
+      if (by_m)
+        for (int r = tid; r < n; r += THREADS)
+          if (sorted_x(r) >= m_bound && (r + 1 == n || sorted_x(r + 1) < m_bound)) s.keep_m = r + 1;
+      __syncthreads();
+      // whether the ranked hold the cut
+      if (k_row > 0 || bound <= -FLT_MAX || (by_m && bound <= m_bound) || (by_p && all >= p * total))
+        keep = min(upto, min(by_p ? s.keep_p : n, by_m ? s.keep_m : n));
+    }
+  }
+
+  if (keep > 0) {
+    // the token among them: the 64th of the ids that the running sum passes the
+    // goal in, then the id.  The sums are integers, so their order does not matter.
+    const int shift = max(0, 26 - __clz(V));  // V >> shift < 64
+    if (tid < kWave) s.sums[tid] = 0;
+    if (tid == 0) s.count = 0;
+    __syncthreads();
+    for (int r = tid; r < keep; r += THREADS) {
+      atomicAdd((unsigned long long *)&s.sums[sorted_id(r) >> shift], (unsigned long long)(s.weight[r] * unit52));
+      if (u == 0.0) atomicMin(&s.token, sorted_id(r));  // the first, however little it weighs
+    }
+    __syncthreads();
+    uint64_t upto = s.sums[lane];
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+      const uint64_t y = __shfl_up((unsigned long long)upto, o, kWave);
+      if (lane >= o) upto += y;
+    }
+    const uint64_t whole = __shfl((unsigned long long)upto, kWave - 1, kWave);
+    const double goal = u * (double)whole;
+    const uint64_t past = __ballot((double)upto > goal), any = __ballot(s.sums[lane] > 0);
+    const int part = past ? __ffsll((unsigned long long)past) - 1 : 63 - __clzll((long long)any);
+    const uint64_t first = __shfl((unsigned long long)(upto - s.sums[lane]), part, kWave);
+    for (int q = tid; q < keep; q += THREADS) {
+      const int id = sorted_id(q);
+      if (id >> shift != part) continue;
+      uint64_t run = first;
+      for (int r = 0; r < keep; ++r) {
+        const int other = sorted_id(r);
+        run += other >> shift == part && other <= id ? (uint64_t)(s.weight[r] * unit52) : 0;
+      }
+      if (s.weight[q] * unit52 >= 1.0) atomicMax(&s.last, id);
+      if ((double)run > goal) atomicMin(&s.token, id);
+    }
+    if (probs)
+      for (int i = tid; i < V; i += THREADS) probs[i] = 0.0f;
+    __syncthreads();
+    if (tid == 0) a.token[row] = s.token < V ? s.token : s.last;
+    if (probs) {
+      const double inv = 1.0 / (s.before[keep - 1] + s.weight[keep - 1]);
+      for (int q = tid; q < keep; q += THREADS) probs[sorted_id(q)] = (float)(s.weight[q] * inv);
+    }
+    return;
+  }
+
+  // ---- 3: a cut by histograms
+  // The shortest prefix of the ids within `in` whose count (by_count) or mass
+  // reaches `goal`.
+  const auto locate = [&](bool by_count, double goal, Cut in) {
+    // the ranges cover lo .. hi; what weighs less than e^-30 shares the last one
+    float hi = top, lo = by_count ? 0.0f : (float)fmax(dtop - 43.3 / c, (double)-FLT_MAX);
+    if (by_count) {
+      float least = FLT_MAX;
+      x.again([&](const float(&e)[EPL], int i) {
+#pragma unroll
+        for (int q = 0; q < EPL; ++q)
+          if (e[q] >= -FLT_MAX) least = fminf(least, e[q]);
+      });
+      lo = -block.max(-least);
+    }
+    double above = 0.0;  // count or mass of what is larger than hi
+    const int bits = min(45, 30 + __clz(V));  // of a weight in a bin's sum, so that V of them fit
+    while (true) {
+      if (lo == hi) {
+        // equal logits: as many of them as it takes, in the order of ids
+        const double w = by_count ? 1.0 : sample_weight(hi, dtop, c);
+        const double need = fmax(1.0, ceil((goal - above) / w));
+        int from = 0, to = V - 1;
+        while (from < to) {  // the least id up to which there are that many
+          const int mid = from + (to - from) / 2;
+          int mine = 0;
+          x.again([&](const float(&e)[EPL], int i) {
+#pragma unroll
+            for (int q = 0; q < EPL; ++q) mine += e[q] == hi && i + q <= mid && in.keeps(e[q], i + q);
+          });
+          if (block.sum((double)mine) >= need) to = mid;
+          else from = mid + 1;
+        }
+        return shorter(in, Cut{hi, to});
+      }
+      const double step = ((double)hi - (double)lo) / kSampleBins;
+      const float scale = (float)(1.0 / step);
+      const auto bin_of = [&](float v) { return (int)fminf((hi - v) * scale, kSampleBins - 1.0f); };
+      // a bin's unit is the least power of two that the largest weight it can hold is
+      // below 2^bits of; what weighs less than 2^-900 is not told from nothing
+      for (int q = tid; q < kSampleBins; q += THREADS) {
+        s.bins[q] = 0;
+        s.unit[q] = (short)((int)ceil(fmax(((double)hi - q * step - dtop) * c, -900.0)) + 2 - bits);
+      }
+      __syncthreads();
+      x.again([&](const float(&e)[EPL], int i) {
+        double w[EPL];
+        if (!by_count) sample_weights(e, dtop, c, w);
+#pragma unroll
+        for (int q = 0; q < EPL; ++q)
+          if (e[q] <= hi && e[q] >= -FLT_MAX && in.keeps(e[q], i + q)) {
+            const int bin = bin_of(e[q]);
+            uint64_t add = 1;
+            if (!by_count) {
+              const double scaled = __hiloint2double(__double2hiint(w[q]) - ((int)s.unit[bin] << 20), __double2loint(w[q]));
+              add = __double_as_longlong(scaled + unit52) & 0xFFFFFFFFFFFFFull;
+            }
+            if (add) atomicAdd((unsigned long long *)&s.bins[bin], (unsigned long long)add);
+          }
+      });
+      __syncthreads();
+      // the first bin that the running sum reaches the goal in; where it falls
+      // short by a last bit of the whole, the last that holds anything
+      constexpr int N = kSampleBins / THREADS;
+      double w[N], sum = 0.0;
+#pragma unroll
+      for (int q = 0; q < N; ++q) {
+        const int bin = N * tid + q;
+        w[q] = by_count ? (double)s.bins[bin] : ldexp((double)s.bins[bin], s.unit[bin]);
+        sum += w[q];
+      }
+      double run = above + block.scan(sum);
+      if (tid == 0) {
+        s.count = 0;
+        s.lo = 0xFFFFFFFFu;
+        s.hi = 0;
+        s.last = -1;
+        s.token = INT_MAX;
+        s.keep_p = 1;
+      }
+      __syncthreads();
+      double before[N];
+#pragma unroll
+      for (int q = 0; q < N; ++q) {
+        before[q] = run;
+        run += w[q];
+        if (w[q] > 0.0) {
+          atomicMax(&s.last, N * tid + q);
+          if (run >= goal) atomicMin(&s.token, N * tid + q);
+        }
+      }
+      __syncthreads();
+      const int bin = min(s.token, s.last);
+#pragma unroll
+      for (int q = 0; q < N; ++q)
+        if (bin == N * tid + q) s.above = before[q];
+      __syncthreads();
+      above = s.above;
+      // its logits, if they can be ranked at once
+      x.again([&](const float(&e)[EPL], int i) {
+#pragma unroll
+        for (int q = 0; q < EPL; ++q)
+          if (e[q] <= hi && e[q] >= -FLT_MAX && in.keeps(e[q], i + q) && bin_of(e[q]) == bin) {
+            const int at = atomicAdd(&s.count, 1);
+            const unsigned key = sample_key(e[q]);
+            if (at < kSampleMost) s.found[at] = (uint64_t)key << 32 | (unsigned)~(i + q);  // ranked: in any order
+            atomicMin(&s.lo, key);
+            atomicMax(&s.hi, key);
+          }
+      });
+      __syncthreads();
+      const int n = s.count;
+      lo = sample_value(s.lo);
+      hi = sample_value(s.hi);
+      if (n <= kSampleMost) {
+        rank(n);
+        if (!by_count) short_of(n, above, goal);
+        __syncthreads();
+        const int last = min(n, by_count ? max(1, (int)(goal - above)) : s.keep_p) - 1;
+        return shorter(in, Cut{sorted_x(last), sorted_id(last)});
+      }
+      __syncthreads();
     }
   };
-  double mine = 0.0, total;
-  int last = -1;
-  walk([&](int i, double w) {
-    mine += w;
-    if (w > 0.0) last = i;
-  });
-  if (tid == 0) found = V;
-  double run = block_exclusive_scan(mine, dscratch, &total);
-  last = (int)block_max((double)last, dscratch);
-  const double want = u * total;
-  const double inv_total = 1.0 / total;
-  int hit = V;
-  walk([&](int i, double w) {
-    run += w;
-    if (w > 0.0 && run > want) hit = min(hit, i);
-    if (a.probs) a.probs[row * a.probs_stride + i] = (float)(w * inv_total);
-  });
-  if (hit < V) atomicMin(&found, hit);
+  Cut cut = all_ids;
+#pragma unroll 1
+  for (int turn = 0; turn < 2; ++turn) {  // top-k, then top-p within it
+    const bool by_count = turn == 0;
+    if (by_count ? k_row == 0 : !by_p) continue;
+    if (!by_count && k_row > 0) total = block.sum(weights_within(cut));
+    cut = locate(by_count, by_count ? (double)k_row : p * total, cut);
+    __syncthreads();
+  }
+  if (by_m) cut = shorter(cut, Cut{m_bound, INT_MAX});
+
+  // ---- 4: the range of the token, then the token
+  const bool every = cut.x <= -FLT_MAX && cut.id == INT_MAX;
+  if (!(every && weigh)) mass = weights_within(cut);
   __syncthreads();
-  if (tid == 0) a.token[row] = found < V ? found : last;
+  const double in_wave = wave_sum(mass);
+  if (tid == 0) {
+    s.token = V;
+    s.last = -1;
+  }
+  if (lane == 0) s.weight[wave] = in_wave;
+  __syncthreads();
+  total = 0.0;
+  for (int w = 0; w < WAVES; ++w) total += s.weight[w];
+  double goal = u * total, run = 0.0;
+  int range = -1, last_range = 0;
+  for (int w = 0; w < WAVES; ++w) {
+    const double in_w = s.weight[w];
+    if (in_w > 0.0) last_range = w;
+    if (range < 0 && run + in_w > goal) range = w;
+    if (range < 0) run += in_w;
+  }
+  if (range < 0) {  // u = 1: the last id that weighs
+    range = last_range;
+    goal = INFINITY;
+  }
+  const int64_t size = (int64_t)x.per * kWave * EPL;
+  const int lo = (int)max((int64_t)0, range * size - x.lead), hi = (int)min((int64_t)V, (range + 1) * size - x.lead);
+  const int each = (hi - lo + THREADS - 1) / THREADS;
+  const int i0 = min(hi, lo + tid * each), i1 = min(hi, i0 + each);
+  constexpr int AT = 6;  // of a thread's ids at once
+  const auto ids = [&](int i, double(&w)[AT]) {
+    float e[AT];
+#pragma unroll
+    for (int k = 0; k < AT; ++k) e[k] = i + k < i1 ? x.at(i + k) : -INFINITY;
+    sample_weights(e, dtop, c, w);
+#pragma unroll
+    for (int k = 0; k < AT; ++k) w[k] = cut.keeps(e[k], i + k) ? w[k] : 0.0;
+  };
+  double mine = 0.0, w[AT];
+  for (int i = i0; i < i1; i += AT) {
+    ids(i, w);
+#pragma unroll
+    for (int k = 0; k < AT; ++k) mine += w[k];
+  }
+  double at = run + block.scan(mine);
+  // the threads whose ids the sum passes the goal in, or nearly
+  if (goal == INFINITY || (at <= goal * (1.0 + 1e-12) && (at + mine) * (1.0 + 1e-12) >= goal)) {
+    for (int i = i0; i < i1; i += AT) {
+      ids(i, w);
+#pragma unroll
+      for (int k = 0; k < AT; ++k) {
+        at += w[k];
+        if (w[k] > 0.0) {
+          atomicMax(&s.last, i + k);
+          if (at > goal) atomicMin(&s.token, i + k);
+        }
+      }
+    }
+  }
+  __syncthreads();
+  if (tid == 0) a.token[row] = s.token < V ? s.token : s.last;
+  if (probs) {
+    const double inv = 1.0 / total;
+    x.again([&](const float(&e)[EPL], int i) {
+      double w[EPL];
+      sample_weights(e, dtop, c, w);
+#pragma unroll
+      for (int q = 0; q < EPL; ++q)
+        if (i + q >= 0 && i + q < V) probs[i + q] = cut.keeps(e[q], i + q) ? (float)(w[q] * inv) : 0.0f;
+    });
+  }
+}
+
+// A row is a compute unit's work while there are units for every row, else two share one.
+template <typename T> int launch_sample(const SampleArgs &a, int64_t rows, hipStream_t s) {
+  if (rows <= cu_count()) sample_kernel<T, 1024><<<(unsigned)rows, 1024, 0, s>>>(a);
+  else sample_kernel<T, 512><<<(unsigned)rows, 512, 0, s>>>(a);
+  return launch_status();
 }
 
 }  // namespace specdec
@@ -204,8 +849,6 @@ SPECDEC_API int specdec_sample(const void *logits, int dtype, int64_t rows, int6
     return SPECDEC_EUNSUPPORTED;
   SampleArgs a{logits, row_stride, (int)vocab, u, temperature, top_p, min_p, top_k, temperatures, top_ps, min_ps, top_ks,
                token, probs, probs_stride};
-  const dim3 grid((unsigned)rows), block(kSampleThreads);
-  if (dtype == SPECDEC_F32) sample_kernel<float><<<grid, block, 0, as_stream(stream)>>>(a);
-  else sample_kernel<__hip_bfloat16><<<grid, block, 0, as_stream(stream)>>>(a);
-  return launch_status();
+  if (dtype == SPECDEC_F32) return launch_sample<float>(a, rows, as_stream(stream));
+  return launch_sample<__hip_bfloat16>(a, rows, as_stream(stream));
 }
