@@ -37,7 +37,6 @@ namespace specdec {
 
 constexpr int kSamplePieces = 6;    // pieces of 16 bytes of a part; the next part's are in flight
 constexpr int kSampleRaw = 2048;    // logits that are collected, each wave its share
-constexpr int kSampleMost = 1024;   // logits that are ranked at once
 constexpr int kSampleBins = 2048;
 constexpr int kSampleTopK = 400;    // the largest top_k that is bounded by the threads' maxima
 constexpr int kSampleGuess = 128;   // reach the bound in the first part, for a nucleus of unknown size
@@ -210,10 +209,10 @@ template <int THREADS> struct SampleShared {
     uint64_t raw[WAVES][SHARE];  // as collected: the order of logits, then falling id
     uint64_t bins[kSampleBins];
   };
-  uint64_t found[kSampleMost];  // ranked
+  uint64_t found[THREADS];      // ranked, as many at once
   union {
     struct {
-      double weight[kSampleMost], before[kSampleMost];  // of the ranked, and the sum before each
+      double weight[THREADS], before[THREADS];  // of the ranked, and the sum before each
     };
     short unit[kSampleBins];
   };
@@ -224,6 +223,7 @@ template <int THREADS> struct SampleShared {
   uint64_t sums[kWave];
   int near[kWave];
   double above;
+  float bound;
   int count, token, last, keep_p, keep_m;
   unsigned lo, hi;
 };
@@ -273,60 +273,79 @@ template <int THREADS> struct SampleBlock {
 };
 
 // A bound that `want` of the threads' maxima in s.tops reach, and not many more:
-// halving between the least and the largest, in each wave for itself.  -FLT_MAX
-// where fewer are finite.
-template <int THREADS> __device__ __forceinline__ float sample_bound(const SampleShared<THREADS> &s, int want) {
+// halving between the least and the largest, in wave 0.  -FLT_MAX where fewer are
+// finite.  With its barrier; the caller's stands between the maxima and this.
+template <int THREADS> __device__ __forceinline__ float sample_bound(SampleShared<THREADS> &s, int want) {
   constexpr int N = THREADS / kWave;
-  const int lane = threadIdx.x & (kWave - 1);
-  float v[N], lo = FLT_MAX, hi = -FLT_MAX;
-  int n = 0;
+  const int lane = threadIdx.x;
+  if (lane < kWave) {
+    float v[N], lo = FLT_MAX, hi = -FLT_MAX;
+    int n = 0;
 #pragma unroll
-  for (int k = 0; k < N; ++k) {
-    v[k] = s.tops[k * kWave + lane];
-    n += __popcll(__ballot(v[k] >= -FLT_MAX));
-    lo = fminf(lo, v[k] >= -FLT_MAX ? v[k] : FLT_MAX);
-    hi = fmaxf(hi, v[k]);
-  }
-  if (n < want) return -FLT_MAX;
-  lo = -wave_max_dpp(-lo);
-  hi = fminf(wave_max_dpp(hi), FLT_MAX);
+    for (int k = 0; k < N; ++k) {
+      v[k] = s.tops[k * kWave + lane];
+      n += __popcll(__ballot(v[k] >= -FLT_MAX));
+      lo = fminf(lo, v[k] >= -FLT_MAX ? v[k] : FLT_MAX);
+      hi = fmaxf(hi, v[k]);
+    }
+    lo = -wave_max_dpp(-lo);
+    hi = fminf(wave_max_dpp(hi), FLT_MAX);
 #pragma unroll 1
-  for (int step = 0; step < 7; ++step) {
-    const float mid = 0.5f * lo + 0.5f * hi;
-    int reach = 0;
+    for (int step = 0; step < 7; ++step) {
+      const float mid = 0.5f * lo + 0.5f * hi;
+      int reach = 0;
 #pragma unroll
-    for (int k = 0; k < N; ++k) reach += __popcll(__ballot(v[k] >= mid));
-    if (reach >= want) lo = mid;
-    else hi = mid;
+      for (int k = 0; k < N; ++k) reach += __popcll(__ballot(v[k] >= mid));
+      if (reach >= want) lo = mid;
+      else hi = mid;
+    }
+    if (lane == 0) s.bound = n < want ? -FLT_MAX : lo;
   }
-  return lo;
+  __syncthreads();
+  return s.bound;
 }
 
-// s.found[0 .. n) from the largest to the least: a bitonic network over the next
-// power of two.  A wave's 64 pairs up to 64 apart are 128 elements of its own, so
-// those steps need no barrier.
-template <int THREADS> __device__ __forceinline__ void sample_sort(SampleShared<THREADS> &s, int n) {
+// The other half of a pair `distance` (a power of two under 64) lanes away.
+__device__ __forceinline__ uint64_t sample_partner(uint64_t v, int distance) {
+  const int lo = (int)v, hi = (int)(v >> 32);
+  int a, b;
+  if (distance == 1) a = dpp_move<0xB1>(lo), b = dpp_move<0xB1>(hi);
+  else if (distance == 2) a = dpp_move<0x4E>(lo), b = dpp_move<0x4E>(hi);
+  else a = __shfl_xor(lo, distance, kWave), b = __shfl_xor(hi, distance, kWave);
+  return (uint64_t)(unsigned)b << 32 | (unsigned)a;
+}
+
+// s.found[0 .. n), n <= THREADS, from the largest to the least: a bitonic network
+// over the next power of two, an element a thread; pairs less than 64 apart are
+// within a wave and need no barrier.
+template <int THREADS> __device__ __forceinline__ uint64_t sample_sort(SampleShared<THREADS> &s, int n) {
   const int tid = threadIdx.x;
   int size = 128;
   while (size < n) size <<= 1;
-  for (int q = n + tid; q < size; q += THREADS) s.found[q] = 0;
-  __syncthreads();
-  volatile uint64_t *x = s.found;
-  for (int k = 2; k <= size; k <<= 1)
-    for (int j = k / 2; j > 0; j >>= 1) {
-      if (tid < size / 2) {
-        const int lo = 2 * tid - (tid & (j - 1)), hi = lo + j;
-        const uint64_t a = x[lo], b = x[hi];
-        if ((a < b) == ((lo & k) == 0 || k == size)) {
-          x[lo] = b;
-          x[hi] = a;
-        }
-      }
-      const int next = j > 1 ? j / 2 : k;  // the next step's distance
-      if (j > 64 || next > 64) __syncthreads();
-      else __builtin_amdgcn_wave_barrier();
+  uint64_t mine = tid < n ? s.found[tid] : 0;
+#pragma unroll 1
+  for (int k = 2; k <= size; k <<= 1) {
+    const bool down = (tid & k) == 0 || k == size;
+#pragma unroll 1
+    for (int j = k / 2; j >= kWave; j >>= 1) {
+      __syncthreads();
+      s.found[tid] = mine;
+      __syncthreads();
+      const uint64_t other = s.found[tid ^ j];
+      mine = ((other > mine) == (down == ((tid & j) == 0))) ? other : mine;
     }
+    if (tid < size) {
+#pragma unroll
+      for (int j = kWave / 2; j > 0; j >>= 1) {
+        if (j >= k) continue;
+        const uint64_t other = sample_partner(mine, j);
+        mine = ((other > mine) == (down == ((tid & j) == 0))) ? other : mine;
+      }
+    }
+  }
   __syncthreads();
+  s.found[tid] = mine;
+  return mine;
 }
 
 template <typename T, int THREADS>
@@ -473,7 +492,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
   // against the row's largest now, or again where the first part was too far from it
   if (weigh) {
     const double up = (base - dtop) * c;
-    if (up > -900.0 && up <= 0.0) mass *= exp2(up);
+    if (up > -900.0 && up <= 0.0) mass *= sample_weight((float)base, dtop, c);
     else mass = weights_within(all_ids);
   }
   double total = weigh ? block.sum(mass) : 0.0;
@@ -488,21 +507,34 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
   constexpr double unit52 = 4503599627370496.0;
   // Ranks the n of s.found, with weights and the sums before each.
   const auto rank = [&](int n) {
-    sample_sort(s, n);
-    constexpr int N = kSampleMost / THREADS;
-    double w[N], sum = 0.0;
+    if (n <= kWave) {  // in wave 0, by counting
+      if (wave == 0) {
+        const uint64_t mine = lane < n ? s.found[lane] : 0;
+        int above = lane < n ? 0 : lane;
+        for (int r = 0; r < n; ++r) {
+          const uint64_t other = (uint64_t)(unsigned)__builtin_amdgcn_readlane((int)(mine >> 32), r) << 32 |
+                                 (unsigned)__builtin_amdgcn_readlane((int)mine, r);
+          above += lane < n && other > mine;
+        }
+        s.found[above] = mine;
+        __builtin_amdgcn_wave_barrier();
+        const float v = sample_value((unsigned)(s.found[lane] >> 32));
+        const double w = lane < n ? sample_weight(v, dtop, c) : 0.0;
+        double run = w;
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const int r = N * tid + k;
-      w[k] = r < n ? sample_weight(sample_value((unsigned)(s.found[r] >> 32)), dtop, c) : 0.0;
-      sum += w[k];
-    }
-    double run = block.scan(sum);
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      s.weight[N * tid + k] = w[k];
-      s.before[N * tid + k] = run;
-      run += w[k];
+        for (int o = 1; o < kWave; o <<= 1) {
+          const double y = __shfl_up(run, o, kWave);
+          if (lane >= o) run += y;
+        }
+        const double before = __shfl_up(run, 1, kWave);
+        s.weight[lane] = w;
+        s.before[lane] = lane ? before : 0.0;
+      }
+    } else {
+      const uint64_t mine = sample_sort(s, n);
+      const double w = tid < n ? sample_weight(sample_value((unsigned)(mine >> 32)), dtop, c) : 0.0;
+      s.before[tid] = block.scan(w);
+      s.weight[tid] = w;
     }
     __syncthreads();
   };
@@ -519,14 +551,14 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
   int keep = 0;  // ranked ids kept, where the cut is among them
   if (few) {
     __syncthreads();
-    // the collected that reach `bound` to s.found; their number, or more than kSampleMost
+    // the collected that reach `bound` to s.found; their number, or more than THREADS
     const auto gather = [&]() {
       const int have = s.wave_n[wave];
       const unsigned least = sample_key(bound);
       int mine = 0;
       if (have <= SHARE)
         for (int r = lane; r - lane < have; r += kWave) mine += __popcll(__ballot(r < have && (unsigned)(s.raw[wave][r] >> 32) >= least));
-      else mine = kSampleMost + 1;
+      else mine = THREADS + 1;
       if (lane == 0) s.near[wave] = mine;
       __syncthreads();
       int at = 0, n = 0;
@@ -534,7 +566,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
         if (w < wave) at += s.near[w];
         n += s.near[w];
       }
-      if (n <= kSampleMost)
+      if (n <= THREADS)
         for (int r = lane; r - lane < have; r += kWave) {
           const bool in = r < have && (unsigned)(s.raw[wave][r] >> 32) >= least;
           const uint64_t hits = __ballot(in);
@@ -543,12 +575,13 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
                 s.raw[wave][r];
           at += __popcll(hits);
         }
+      __syncthreads();
       return n;
     };
     // by the maxima of the whole row the bound of a top-k is a tighter one
     if (k_row > 0) bound = fmaxf(bound, sample_bound(s, want));
     int n = gather();
-    if (n > kSampleMost) {  // the first part was not like the rest: again, by the maxima of the whole row
+    if (n > THREADS) {  // the first part was not like the rest: again, by the maxima of the whole row
       bound = sample_bound(s, want);
       collected = 0;
       x.again(collect);
@@ -557,7 +590,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
       __syncthreads();
       n = gather();
     }
-    if (n <= kSampleMost) {
+    if (n <= THREADS) {
       rank(n);
       const int upto = k_row > 0 ? min(k_row, n) : n;
       const double all = s.before[upto - 1] + s.weight[upto - 1];
@@ -573,6 +606,35 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
     }
   }
 
+  if (keep > 0 && keep <= kWave) {
+    // the token among them: the running sum up to each id, in wave 0
+    if (probs)
+      for (int i = tid; i < V; i += THREADS) probs[i] = 0.0f;
+    total = s.before[keep - 1] + s.weight[keep - 1];
+    if (wave == 0) {
+      const int id = lane < keep ? sorted_id(lane) : INT_MAX;
+      const double w = lane < keep ? s.weight[lane] : 0.0;
+      double run = 0.0, all = 0.0;
+      for (int r = 0; r < keep; ++r) {
+        const int other = __builtin_amdgcn_readlane(id, r);
+        const double v = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(w), r),
+                                          __builtin_amdgcn_readlane(__double2loint(w), r));
+        all += v;
+        run += other <= id ? v : 0.0;
+      }
+      if (lane < keep) {
+        atomicMax(&s.last, id);
+        if (run > u * all) atomicMin(&s.token, id);
+      }
+      __builtin_amdgcn_wave_barrier();
+      if (lane == 0) a.token[row] = s.token < V ? s.token : s.last;
+    }
+    if (probs) {
+      __syncthreads();
+      if (tid < keep) probs[sorted_id(tid)] = (float)(s.weight[tid] / total);
+    }
+    return;
+  }
   if (keep > 0) {
     // the token among them: the 64th of the ids that the running sum passes the
     // goal in, then the id.  The sums are integers, so their order does not matter.
@@ -723,7 +785,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
           if (e[q] <= hi && e[q] >= -FLT_MAX && in.keeps(e[q], i + q) && bin_of(e[q]) == bin) {
             const int at = atomicAdd(&s.count, 1);
             const unsigned key = sample_key(e[q]);
-            if (at < kSampleMost) s.found[at] = (uint64_t)key << 32 | (unsigned)~(i + q);  // ranked: in any order
+            if (at < THREADS) s.found[at] = (uint64_t)key << 32 | (unsigned)~(i + q);  // ranked: in any order
             atomicMin(&s.lo, key);
             atomicMax(&s.hi, key);
           }
@@ -732,7 +794,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
       const int n = s.count;
       lo = sample_value(s.lo);
       hi = sample_value(s.hi);
-      if (n <= kSampleMost) {
+      if (n <= THREADS) {
         rank(n);
         if (!by_count) short_of(n, above, goal);
         __syncthreads();
@@ -801,7 +863,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
   // the threads whose ids the sum passes the goal in, or nearly
   if (goal == INFINITY || (at <= goal * (1.0 + 1e-12) && (at + mine) * (1.0 + 1e-12) >= goal)) {
     for (int i = i0; i < i1; i += AT) {
-      ids(i, w);
+      if (each > AT) ids(i, w);
 #pragma unroll
       for (int k = 0; k < AT; ++k) {
         at += w[k];
