@@ -35,8 +35,11 @@
 
 namespace specdec {
 
+// a lambda that is called keeps what it captures in memory
+#define SAMPLE_INLINE __attribute__((always_inline))
+
 constexpr int kSamplePieces = 6;    // pieces of 16 bytes of a part; the next part's are in flight
-constexpr int kSampleRaw = 2048;    // logits that are collected, each wave its share
+constexpr int kSampleRaw = 4096;    // logits that are collected, each wave its share
 constexpr int kSampleBins = 2048;
 constexpr int kSampleTopK = 400;    // the largest top_k that is bounded by the threads' maxima
 constexpr int kSampleGuess = 128;   // reach the bound in the first part, for a nucleus of unknown size
@@ -140,22 +143,22 @@ template <typename T, int THREADS> struct SampleRow {
   unsigned offset;   // of this thread's first piece
   bool infinite;     // the row has +inf: those weigh the same, the others nothing
 
-  __device__ SampleRow(const void *logits, int64_t first, int vocab) : x((const T *)logits + first), V(vocab), infinite(false) {
+  __device__ __forceinline__ SampleRow(const void *logits, int64_t first, int vocab) : x((const T *)logits + first), V(vocab), infinite(false) {
     lead = (int)((uintptr_t)x % 16 / sizeof(T));
     const int pieces = (lead + V + EPL - 1) / EPL;
     per = (pieces + THREADS - 1) / THREADS;
     rows = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(x - lead), 0, pieces * 16, 0x00020000);
     offset = ((threadIdx.x / kWave) * per * kWave + (threadIdx.x & (kWave - 1))) * 16u;
   }
-  __device__ int id0(int j) const { return (int)(offset / 16 + j * kWave) * EPL - lead; }  // id of the first element of piece j
-  __device__ u32x4 piece(int j) const {
+  __device__ __forceinline__ int id0(int j) const { return (int)(offset / 16 + j * kWave) * EPL - lead; }  // id of the first element of piece j
+  __device__ __forceinline__ u32x4 piece(int j) const {
     return __builtin_amdgcn_raw_buffer_load_b128(rows, j < per ? offset + j * (kWave * 16u) : 0xFFFFFF00u, 0, 0);
   }
-  __device__ float value(float v) const {
+  __device__ __forceinline__ float value(float v) const {
     v = fmaxf(v, -INFINITY);  // a NaN is -inf
     return infinite ? (v == INFINITY ? 0.0f : -INFINITY) : v;
   }
-  __device__ void unpack(u32x4 v, int j, float (&e)[EPL]) const {
+  __device__ __forceinline__ void unpack(u32x4 v, int j, float (&e)[EPL]) const {
 #pragma unroll
     for (int k = 0; k < EPL; ++k) {
       if constexpr (sizeof(T) == 4) e[k] = fmaxf(__uint_as_float(v[k]), -INFINITY);
@@ -167,13 +170,18 @@ template <typename T, int THREADS> struct SampleRow {
       for (int k = 0; k < EPL; ++k) e[k] = i + k >= 0 && i + k < V ? value(e[k]) : -INFINITY;
     }
   }
-  __device__ float at(int i) const { return value(to_f32(x[i])); }
-  __device__ void load(u32x4 (&v)[kSamplePieces], int j0) const {
+  // the logit of an id of the row, or anything
+  __device__ __forceinline__ float at(int i) const {
+    const unsigned at = (unsigned)(lead + i) * (unsigned)sizeof(T);
+    if constexpr (sizeof(T) == 4) return value(__uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rows, at, 0, 0)));
+    else return value(__uint_as_float((unsigned)__builtin_amdgcn_raw_buffer_load_b16(rows, at, 0, 0) << 16));
+  }
+  __device__ __forceinline__ void load(u32x4 (&v)[kSamplePieces], int j0) const {
 #pragma unroll
     for (int k = 0; k < kSamplePieces; ++k) v[k] = piece(j0 + k);
   }
   // f(v, first piece) over this thread's pieces, a part at a time, the next one in flight
-  template <typename F> __device__ void parts(F &&f) const {
+  template <typename F> __device__ __forceinline__ void parts(F &&f) const {
     u32x4 v0[kSamplePieces], v1[kSamplePieces];
     load(v0, 0);
     for (int j = 0;;) {
@@ -186,7 +194,7 @@ template <typename T, int THREADS> struct SampleRow {
     }
   }
   // f(e, id of e[0]) over this thread's pieces, to read the row again
-  template <typename F> __device__ void again(F &&f) const {
+  template <typename F> __device__ __forceinline__ void again(F &&f) const {
 #pragma unroll 1
     for (int j0 = 0; j0 < per; j0 += kSamplePieces) {
       u32x4 v[kSamplePieces];
@@ -205,10 +213,8 @@ template <typename T, int THREADS> struct SampleRow {
 
 template <int THREADS> struct SampleShared {
   static constexpr int WAVES = THREADS / kWave, SHARE = kSampleRaw / WAVES;
-  union {
-    uint64_t raw[WAVES][SHARE];  // as collected: the order of logits, then falling id
-    uint64_t bins[kSampleBins];
-  };
+  uint64_t raw[WAVES][SHARE];   // as collected: the order of logits, then falling id
+  uint64_t bins[kSampleBins];
   uint64_t found[THREADS];      // ranked, as many at once
   union {
     struct {
@@ -234,7 +240,7 @@ template <int THREADS> struct SampleBlock {
   static constexpr int WAVES = THREADS / kWave;
   SampleShared<THREADS> &s;
   int turn = 0;
-  __device__ double sum(double v) {
+  __device__ __forceinline__ double sum(double v) {
     v = wave_sum(v);
     turn ^= 1;
     if ((threadIdx.x & (kWave - 1)) == 0) s.wave_d[turn][threadIdx.x / kWave] = v;
@@ -243,7 +249,7 @@ template <int THREADS> struct SampleBlock {
     for (int w = 0; w < WAVES; ++w) v += s.wave_d[turn][w];
     return v;
   }
-  __device__ float max(float v) {
+  __device__ __forceinline__ float max(float v) {
     v = wave_max_dpp(v);
     turn ^= 1;
     if ((threadIdx.x & (kWave - 1)) == 0) s.wave_f[turn][threadIdx.x / kWave] = v;
@@ -253,7 +259,7 @@ template <int THREADS> struct SampleBlock {
     return v;
   }
   // exclusive prefix over the threads
-  __device__ double scan(double v) {
+  __device__ __forceinline__ double scan(double v) {
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     double x = v;
 #pragma unroll
@@ -379,7 +385,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
   double mass, base;  // this thread's weights against `base`
   int top_j;          // this thread's first piece that has its largest logit
   int collected;      // by this wave; past its share they are only counted
-  const auto collect = [&](const float(&e)[EPL], int i) {
+  const auto collect = [&](const float(&e)[EPL], int i) SAMPLE_INLINE {
 #pragma unroll
     for (int q = 0; q < EPL; ++q) {
       const uint64_t hits = __ballot(e[q] >= bound);
@@ -398,7 +404,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
       s.last = -1;
       s.keep_p = s.keep_m = 1;
     }
-    x.parts([&](const u32x4(&v)[kSamplePieces], int j0) {
+    x.parts([&](const u32x4(&v)[kSamplePieces], int j0) SAMPLE_INLINE {
       float part[kSamplePieces];
 #pragma unroll
       for (int k = 0; k < kSamplePieces; ++k) {
@@ -478,9 +484,9 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
   }
   const double dtop = (double)top;
   // the weights of a cut's ids, of this thread
-  const auto weights_within = [&](Cut cut) {
+  const auto weights_within = [&](Cut cut) SAMPLE_INLINE {
     double sum = 0.0;
-    x.again([&](const float(&e)[EPL], int i) {
+    x.again([&](const float(&e)[EPL], int i) SAMPLE_INLINE {
       double w[EPL];
       sample_weights(e, dtop, c, w);
 #pragma unroll
@@ -506,7 +512,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
 
   constexpr double unit52 = 4503599627370496.0;
   // Ranks the n of s.found, with weights and the sums before each.
-  const auto rank = [&](int n) {
+  const auto rank = [&](int n) SAMPLE_INLINE {
     if (n <= kWave) {  // in wave 0, by counting
       if (wave == 0) {
         const uint64_t mine = lane < n ? s.found[lane] : 0;
@@ -538,11 +544,11 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
     }
     __syncthreads();
   };
-  const auto sorted_x = [&](int r) { return sample_value((unsigned)(s.found[r] >> 32)); };
-  const auto sorted_id = [&](int r) { return (int)~(unsigned)s.found[r]; };
+  const auto sorted_x = [&](int r) SAMPLE_INLINE { return sample_value((unsigned)(s.found[r] >> 32)); };
+  const auto sorted_id = [&](int r) SAMPLE_INLINE { return (int)~(unsigned)s.found[r]; };
   // Of the first n ranked, how many have a mass before them (with `above`) short
   // of `goal`: into s.keep_p, which holds 1.
-  const auto short_of = [&](int n, double above, double goal) {
+  const auto short_of = [&](int n, double above, double goal) SAMPLE_INLINE {
     for (int r = tid; r < n; r += THREADS)
       if (above + s.before[r] < goal && (r + 1 == n || above + s.before[r + 1] >= goal)) s.keep_p = r + 1;
   };
@@ -552,7 +558,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
   if (few) {
     __syncthreads();
     // the collected that reach `bound` to s.found; their number, or more than THREADS
-    const auto gather = [&]() {
+    const auto gather = [&]() SAMPLE_INLINE {
       const int have = s.wave_n[wave];
       const unsigned least = sample_key(bound);
       int mine = 0;
@@ -680,15 +686,142 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
     return;
   }
 
-  // ---- 3: a cut by histograms
+  // ---- 3: a nucleus of thousands
+  // The shortest prefix whose mass reaches `goal`, and this thread's part of that
+  // mass.  A few pieces of every thread say where the cut about is: by the weight
+  // below it, of which many ids have little each, so that a sample holds a like
+  // share of it.  The row read once more gives the mass above that range of
+  // logits and the ids in it, among which the cut is; false where it is not.
+  const auto nucleus = [&](double goal, Cut &cut) SAMPLE_INLINE {
+    constexpr int PARTS = 8192 / (THREADS * EPL);  // pieces of a thread in the sample
+    if (x.per < 2 * PARTS || !(c > 0.0)) return false;
+    const float lo = (float)fmax(dtop - 43.3 / c, (double)-FLT_MAX);
+    if (!(lo < top)) return false;
+    const float scale = (float)(kSampleBins / ((double)top - (double)lo)), c32 = (float)c;
+    const auto bin_of = [&](float v) SAMPLE_INLINE { return (int)fminf((top - v) * scale, kSampleBins - 1.0f); };
+    for (int q = tid; q < kSampleBins; q += THREADS) s.bins[q] = 0;
+    __syncthreads();
+    constexpr float unit40 = 1099511627776.0f;
+    u32x4 v[PARTS];
+#pragma unroll
+    for (int k = 0; k < PARTS; ++k) v[k] = x.piece((2 * k + 1) * x.per / (2 * PARTS));
+#pragma unroll
+    for (int k = 0; k < PARTS; ++k) {
+      float e[EPL];
+      x.unpack(v[k], (2 * k + 1) * x.per / (2 * PARTS), e);
+#pragma unroll
+      for (int q = 0; q < EPL; ++q) {
+        const float w = __builtin_amdgcn_exp2f((e[q] - top) * c32);
+        if (e[q] >= -FLT_MAX) atomicAdd((unsigned long long *)&s.bins[bin_of(e[q])], (unsigned long long)(w * unit40));
+      }
+    }
+    if (tid == 0) {
+      s.near[0] = 0;
+      s.near[1] = kSampleBins - 1;
+    }
+    __syncthreads();
+    constexpr int N = kSampleBins / THREADS;
+    double w[N], sum = 0.0;
+#pragma unroll
+    for (int q = 0; q < N; ++q) sum += w[q] = (double)s.bins[kSampleBins - 1 - (N * tid + q)];
+    double below = block.scan(sum);  // from the least weight up
+    const double aim = (total - goal) * PARTS / x.per * unit40;
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+      const int bin = kSampleBins - 1 - (N * tid + q);
+      if (below < 0.94 * aim && below + w[q] >= 0.94 * aim) s.near[1] = bin;  // the range ends here
+      if (below < 1.06 * aim && below + w[q] >= 1.06 * aim) s.near[0] = bin;  // .. and begins here
+      below += w[q];
+    }
+    __syncthreads();
+    // logits of bins near[0] .. near[1], and one more either way
+    const float from = top - (float)(s.near[1] + 2) / scale, to = top - (float)(s.near[0] - 1) / scale;
+    if (!(from < to)) return false;
+    bound = from;
+    collected = 0;
+    mass = 0.0;
+    x.again([&](const float(&e)[EPL], int i) SAMPLE_INLINE {
+      double w[EPL];
+      sample_weights(e, dtop, c, w);
+      float in[EPL];
+#pragma unroll
+      for (int q = 0; q < EPL; ++q) {
+        mass += e[q] > to ? w[q] : 0.0;
+        in[q] = e[q] > to ? -INFINITY : e[q];
+      }
+      collect(in, i);
+    });
+    const double above = block.sum(mass);
+    if (lane == 0) s.wave_n[wave] = collected;
+    const int have = collected;
+    // the collected by 2048 ranges again, of weights in units that the largest is 2^45 of
+    const double step = ((double)to - (double)from) / kSampleBins;
+    const float fine = (float)(1.0 / step);
+    const auto fine_of = [&](float v) SAMPLE_INLINE { return (int)fmaxf(0.0f, fminf((to - v) * fine, kSampleBins - 1.0f)); };
+    const double unit = 35184372088832.0 / sample_weight(to, dtop, c);
+    for (int q = tid; q < kSampleBins; q += THREADS) s.bins[q] = 0;
+    if (tid == 0) {
+      s.count = 0;
+      s.last = -1;
+      s.token = INT_MAX;
+      s.keep_p = 1;
+    }
+    __syncthreads();
+    int most = 0;
+    for (int w = 0; w < WAVES; ++w) most = max(most, s.wave_n[w]);
+    if (most > SHARE || !(above < goal)) return false;
+    const auto mine = [&](int r) SAMPLE_INLINE { return sample_value((unsigned)(s.raw[wave][r] >> 32)); };
+    for (int r = lane; r < have; r += kWave) {
+      const float v = mine(r);
+      atomicAdd((unsigned long long *)&s.bins[fine_of(v)], (unsigned long long)(sample_weight(v, dtop, c) * unit));
+    }
+    __syncthreads();
+    double in_bin[N];
+    sum = 0.0;
+#pragma unroll
+    for (int q = 0; q < N; ++q) sum += in_bin[q] = (double)s.bins[N * tid + q] / unit;
+    double run = above + block.scan(sum);
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+      // the first bin that the sum passes the goal in, by more than the units round
+      if (run < goal && run + in_bin[q] >= goal) {
+        s.token = N * tid + q;
+        s.above = run;
+      }
+      run += in_bin[q];
+    }
+    __syncthreads();
+    const int bin = s.token;
+    if (bin == INT_MAX) return false;
+    for (int r = lane; r < have; r += kWave)
+      if (fine_of(mine(r)) == bin) {
+        const int at = atomicAdd(&s.count, 1);
+        if (at < THREADS) s.found[at] = s.raw[wave][r];
+      }
+    __syncthreads();
+    const int n = s.count;
+    if (n > THREADS) return false;
+    const double before = s.above;
+    rank(n);
+    short_of(n, before, goal);
+    __syncthreads();
+    cut = Cut{sorted_x(s.keep_p - 1), sorted_id(s.keep_p - 1)};
+    for (int r = lane; r < have; r += kWave) {
+      const float v = mine(r);
+      if (cut.keeps(v, (int)~(unsigned)s.raw[wave][r])) mass += sample_weight(v, dtop, c);
+    }
+    return true;
+  };
+
+  // .. or any other cut, by histograms
   // The shortest prefix of the ids within `in` whose count (by_count) or mass
   // reaches `goal`.
-  const auto locate = [&](bool by_count, double goal, Cut in) {
+  const auto locate = [&](bool by_count, double goal, Cut in) SAMPLE_INLINE {
     // the ranges cover lo .. hi; what weighs less than e^-30 shares the last one
     float hi = top, lo = by_count ? 0.0f : (float)fmax(dtop - 43.3 / c, (double)-FLT_MAX);
     if (by_count) {
       float least = FLT_MAX;
-      x.again([&](const float(&e)[EPL], int i) {
+      x.again([&](const float(&e)[EPL], int i) SAMPLE_INLINE {
 #pragma unroll
         for (int q = 0; q < EPL; ++q)
           if (e[q] >= -FLT_MAX) least = fminf(least, e[q]);
@@ -706,7 +839,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
         while (from < to) {  // the least id up to which there are that many
           const int mid = from + (to - from) / 2;
           int mine = 0;
-          x.again([&](const float(&e)[EPL], int i) {
+          x.again([&](const float(&e)[EPL], int i) SAMPLE_INLINE {
 #pragma unroll
             for (int q = 0; q < EPL; ++q) mine += e[q] == hi && i + q <= mid && in.keeps(e[q], i + q);
           });
@@ -717,7 +850,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
       }
       const double step = ((double)hi - (double)lo) / kSampleBins;
       const float scale = (float)(1.0 / step);
-      const auto bin_of = [&](float v) { return (int)fminf((hi - v) * scale, kSampleBins - 1.0f); };
+      const auto bin_of = [&](float v) SAMPLE_INLINE { return (int)fminf((hi - v) * scale, kSampleBins - 1.0f); };
       // a bin's unit is the least power of two that the largest weight it can hold is
       // below 2^bits of; what weighs less than 2^-900 is not told from nothing
       for (int q = tid; q < kSampleBins; q += THREADS) {
@@ -725,7 +858,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
         s.unit[q] = (short)((int)ceil(fmax(((double)hi - q * step - dtop) * c, -900.0)) + 2 - bits);
       }
       __syncthreads();
-      x.again([&](const float(&e)[EPL], int i) {
+      x.again([&](const float(&e)[EPL], int i) SAMPLE_INLINE {
         double w[EPL];
         if (!by_count) sample_weights(e, dtop, c, w);
 #pragma unroll
@@ -779,7 +912,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
       __syncthreads();
       above = s.above;
       // its logits, if they can be ranked at once
-      x.again([&](const float(&e)[EPL], int i) {
+      x.again([&](const float(&e)[EPL], int i) SAMPLE_INLINE {
 #pragma unroll
         for (int q = 0; q < EPL; ++q)
           if (e[q] <= hi && e[q] >= -FLT_MAX && in.keeps(e[q], i + q) && bin_of(e[q]) == bin) {
@@ -805,19 +938,23 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
     }
   };
   Cut cut = all_ids;
+  bool summed = weigh && !by_p;  // `mass` is that of the cut
+  if (by_p && k_row == 0) summed = nucleus(p * total, cut);
 #pragma unroll 1
   for (int turn = 0; turn < 2; ++turn) {  // top-k, then top-p within it
     const bool by_count = turn == 0;
-    if (by_count ? k_row == 0 : !by_p) continue;
+    if (by_count ? k_row == 0 : !by_p || summed) continue;
     if (!by_count && k_row > 0) total = block.sum(weights_within(cut));
     cut = locate(by_count, by_count ? (double)k_row : p * total, cut);
     __syncthreads();
   }
-  if (by_m) cut = shorter(cut, Cut{m_bound, INT_MAX});
+  if (by_m && cut.x < m_bound) {
+    cut = Cut{m_bound, INT_MAX};
+    summed = false;
+  }
 
   // ---- 4: the range of the token, then the token
-  const bool every = cut.x <= -FLT_MAX && cut.id == INT_MAX;
-  if (!(every && weigh)) mass = weights_within(cut);
+  if (!summed) mass = weights_within(cut);
   __syncthreads();
   const double in_wave = wave_sum(mass);
   if (tid == 0) {
@@ -845,13 +982,13 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
   const int each = (hi - lo + THREADS - 1) / THREADS;
   const int i0 = min(hi, lo + tid * each), i1 = min(hi, i0 + each);
   constexpr int AT = 6;  // of a thread's ids at once
-  const auto ids = [&](int i, double(&w)[AT]) {
+  const auto ids = [&](int i, double(&w)[AT]) SAMPLE_INLINE {
     float e[AT];
 #pragma unroll
-    for (int k = 0; k < AT; ++k) e[k] = i + k < i1 ? x.at(i + k) : -INFINITY;
+    for (int k = 0; k < AT; ++k) e[k] = x.at(i + k);
     sample_weights(e, dtop, c, w);
 #pragma unroll
-    for (int k = 0; k < AT; ++k) w[k] = cut.keeps(e[k], i + k) ? w[k] : 0.0;
+    for (int k = 0; k < AT; ++k) w[k] = i + k < i1 && cut.keeps(e[k], i + k) ? w[k] : 0.0;
   };
   double mine = 0.0, w[AT];
   for (int i = i0; i < i1; i += AT) {
@@ -878,7 +1015,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
   if (tid == 0) a.token[row] = s.token < V ? s.token : s.last;
   if (probs) {
     const double inv = 1.0 / total;
-    x.again([&](const float(&e)[EPL], int i) {
+    x.again([&](const float(&e)[EPL], int i) SAMPLE_INLINE {
       double w[EPL];
       sample_weights(e, dtop, c, w);
 #pragma unroll
