@@ -570,8 +570,13 @@ inline TreeCut tree_cut(int batch, int queries, int H, int Hkv, int d, int dtype
   cut.groups = (need + cut.tiles - 1) / cut.tiles;
   const int ck = dtype == SPECDEC_BF16 ? 32 : 16, chunks = (max_kv + ck - 1) / ck;
   const int64_t units = (int64_t)batch * Hkv * cut.groups;
-  int64_t splits = (1024 + units - 1) / units;
-  splits = splits < chunks / kTreeWaves ? splits : chunks / kTreeWaves;
+  // two workgroups a compute unit, what the registers of most variants let in at
+  // once, and four chunks a wave, below which the second launch costs more than it
+  // gives (measured: 8 rows of 32 nodes at 4096 keys 55.9 / 56.8 / 64.5 us in 1 / 2 /
+  // 4 splits, one row of 16 at 300 keys 7.6 / 9.8 in 1 / 2, four fp32 rows of 13 at
+  // 1500 keys 34.5 / 26.4 / 26.6 / 34.8 in 1 / 2 / 4 / 8)
+  int64_t splits = 512 / units;
+  splits = splits < chunks / (4 * kTreeWaves) ? splits : chunks / (4 * kTreeWaves);
   cut.splits = (int)(splits < 1 ? 1 : splits > 64 ? 64 : splits);
   return cut;
 }

@@ -6,6 +6,8 @@ computes on the CPU: inputs that are not on a GPU are an error.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from specdec._lib import lib
@@ -1257,45 +1259,64 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
 TREE_NODES = 256  # nodes of a tree, at most
 
 
-def _tree_side(dev: torch.device, dtype: torch.dtype, cos, sin, k_pool, v_pool, tables, layered: int) -> tuple[int, ...]:
+def _tree_side(dev: torch.device, index: int, dtype: torch.dtype, cos, sin, k_pool, v_pool, tables, layered: int):
     """(blocks, kv heads, block size, head_dim) of the paged pools [(layers,)
     blocks, kv heads, block size, head_dim] (V with the last two swapped), and
     the checks of what else a tree's kernels read the cache with."""
-    shape = k_pool.shape
-    if len(shape) != 4 + layered or v_pool.shape != (*shape[:-2], shape[-1], shape[-2]):
+    shape, vshape, cshape, tshape = k_pool.shape, v_pool.shape, cos.shape, tables.shape
+    if len(shape) != 4 + layered or len(vshape) != 4 + layered or shape[:-2] != vshape[:-2] or shape[-1] != vshape[-2] \
+            or shape[-2] != vshape[-1]:
         raise ValueError(f"the pools must be {'[layers, ' if layered else '['}blocks, kv heads, block size, head_dim] and "
-                         f"the same with the last two swapped (got {list(shape)} and {list(v_pool.shape)})")
-    _on(dev, k_pool, "k_pool", dtype, True)
-    _on(dev, v_pool, "v_pool", dtype, True)
-    _on(dev, cos, "cos", torch.float32, True)
-    _on(dev, sin, "sin", torch.float32, True)
-    if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] * 2 != shape[-1]:
-        raise ValueError(f"cos and sin must be [positions, {shape[-1] // 2}] (got {list(cos.shape)} and {list(sin.shape)})")
-    _on(dev, tables, "tables", torch.int32)
-    if tables.dim() != 2 or tables.stride(1) != 1 or tables.shape[0] > 1 and tables.stride(0) < tables.shape[1]:
+                         f"the same with the last two swapped (got {list(shape)} and {list(vshape)})")
+    if (k_pool.get_device() != index or v_pool.get_device() != index or cos.get_device() != index
+            or sin.get_device() != index or tables.get_device() != index or k_pool.dtype is not dtype
+            or v_pool.dtype is not dtype or cos.dtype is not torch.float32 or sin.dtype is not torch.float32
+            or tables.dtype is not torch.int32 or not k_pool.is_contiguous() or not v_pool.is_contiguous()
+            or not cos.is_contiguous() or not sin.is_contiguous()):
+        _on(dev, k_pool, "k_pool", dtype, True)
+        _on(dev, v_pool, "v_pool", dtype, True)
+        _on(dev, cos, "cos", torch.float32, True)
+        _on(dev, sin, "sin", torch.float32, True)
+        _on(dev, tables, "tables", torch.int32)
+    if len(cshape) != 2 or cshape != sin.shape or cshape[1] * 2 != shape[-1]:
+        raise ValueError(f"cos and sin must be [positions, {shape[-1] // 2}] (got {list(cshape)} and {list(sin.shape)})")
+    if len(tshape) != 2 or not tables.is_contiguous() and (tables.stride(1) != 1 or tshape[0] > 1
+                                                          and tables.stride(0) < tshape[1]):
         raise ValueError("block tables must be int32 [rows, capacity] with unit inner stride")
     return shape[-4:]
 
 
-def _tree_rows(qkv: torch.Tensor, kv_heads: int, head_dim: int) -> int:
+def _tree_rows(qkv: torch.Tensor, shape, strides, kv_heads: int, head_dim: int) -> int:
     """Query heads of projection rows [..., (H + 2 Hkv) * head_dim]."""
-    heads = qkv.shape[-1] // head_dim - 2 * kv_heads
-    if heads <= 0 or (heads + 2 * kv_heads) * head_dim != qkv.shape[-1]:
-        raise ValueError(f"qkv rows of {qkv.shape[-1]} values do not hold q, k and v of {kv_heads} kv heads of {head_dim}")
-    if qkv.stride(-1) != 1 or qkv.shape[-2] > 1 and qkv.stride(-2) < qkv.shape[-1]:
+    row = shape[-1]
+    heads = row // head_dim - 2 * kv_heads
+    if heads <= 0 or (heads + 2 * kv_heads) * head_dim != row:
+        raise ValueError(f"qkv rows of {row} values do not hold q, k and v of {kv_heads} kv heads of {head_dim}")
+    if strides[-1] != 1 or shape[-2] > 1 and strides[-2] < row:
         raise ValueError("qkv needs unit inner stride and rows that do not overlap")
     return heads
 
 
-def _per_tree(dev: torch.device, t: torch.Tensor, batch: int, shape: tuple, dtype: torch.dtype, name: str) -> int:
-    """Batch stride of t [batch or 1, *shape], 0 where one tree serves every row."""
-    _on(dev, t, name, dtype)
-    got = t.shape
-    if len(got) != 1 + len(shape) or got[0] not in (1, batch) or got[1:] != shape:
+def _per_tree(dev: torch.device, index: int, t: torch.Tensor, batch: int, shape: tuple, dtype: torch.dtype,
+              name: str) -> tuple[int, ...]:
+    """Strides of t [batch or 1, *shape], the batch's 0 where one tree serves every row."""
+    if t.get_device() != index or t.dtype is not dtype:
+        _on(dev, t, name, dtype)
+    got, strides = t.shape, t.stride()
+    if len(got) != 1 + len(shape) or got[1:] != shape or got[0] != batch and got[0] != 1:
         raise ValueError(f"{name} must be [{batch} or 1, {', '.join(map(str, shape))}] (got {list(got)})")
-    if t.stride(-1) != 1 and shape[-1] > 1:
+    if strides[-1] != 1 and shape[-1] > 1:
         raise ValueError(f"{name} needs unit inner stride")
-    return 0 if got[0] == 1 else t.stride(0)
+    return strides if got[0] != 1 else (0, *strides[1:])
+
+
+@functools.lru_cache(maxsize=1024)
+def _tree_floats(*sizes) -> int:
+    import ctypes
+
+    floats = ctypes.c_int64()
+    _check(lib().specdec_tree_attention_workspace(*sizes, ctypes.byref(floats)), "tree_attention")
+    return floats.value
 
 
 def tree_attention(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
@@ -1315,53 +1336,51 @@ def tree_attention(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_po
     keeps a layer's; the cache is read only (tree_commit writes it).  head_dim 64
     or 128.  max_kv_len is the cached length the launch is laid out for; longer
     rows are right too, and slower."""
-    if not qkv.is_cuda:
+    index = qkv.get_device()
+    if index < 0:
         gpu(qkv, "qkv")
-    dev, dt = qkv.device, _FP8_INPUTS.get(qkv.dtype)
+    dev, dtype, shape, strides = qkv.device, qkv.dtype, qkv.shape, qkv.stride()
+    dt = _FP8_INPUTS.get(dtype)
     if dt is None:
-        raise TypeError(f"qkv must be bf16 or fp32 (got {qkv.dtype})")
-    if qkv.dim() != 3:
-        raise ValueError(f"qkv must be [B, N, (H + 2 Hkv) * head_dim] (got {list(qkv.shape)})")
-    blocks, kv_heads, bs, d = _tree_side(dev, qkv.dtype, cos, sin, k_pool, v_pool, tables, 0)
-    batch, nodes, _ = qkv.shape
-    if _tree_rows(qkv, kv_heads, d) != n_heads:
-        raise ValueError(f"qkv rows of {qkv.shape[2]} values do not hold {n_heads} query and {kv_heads} kv heads of {d}")
+        raise TypeError(f"qkv must be bf16 or fp32 (got {dtype})")
+    if len(shape) != 3:
+        raise ValueError(f"qkv must be [B, N, (H + 2 Hkv) * head_dim] (got {list(shape)})")
+    blocks, kv_heads, bs, d = _tree_side(dev, index, dtype, cos, sin, k_pool, v_pool, tables, 0)
+    batch, nodes, row = shape
+    if _tree_rows(qkv, shape, strides, kv_heads, d) != n_heads:
+        raise ValueError(f"qkv rows of {row} values do not hold {n_heads} query and {kv_heads} kv heads of {d}")
     if not 0 <= first <= nodes or nodes > TREE_NODES:
         raise ValueError(f"a tree has at most {TREE_NODES} nodes, first among them (got {nodes}, {first})")
-    _on(dev, meta, "meta", torch.int32, True, 3 * batch)
-    words, width = -(-nodes // 64), nodes - first
-    if mask.dim() == 2 and words == 1:
+    if meta.get_device() != index or meta.dtype is not torch.int32 or meta.numel() != 3 * batch or not meta.is_contiguous():
+        _on(dev, meta, "meta", torch.int32, True, 3 * batch)
+    words, width = (nodes + 63) // 64, nodes - first
+    if words == 1 and mask.dim() == 2:
         mask = mask[:, :, None]
-    mask_stride = _per_tree(dev, mask, batch, (width, words), torch.int64, "mask")
-    depth_stride = _per_tree(dev, depth, batch, (nodes,), torch.int32, "depth")
+    mask_strides = _per_tree(dev, index, mask, batch, (width, words), torch.int64, "mask")
+    depth_strides = _per_tree(dev, index, depth, batch, (nodes,), torch.int32, "depth")
     if out is None:
-        out = torch.empty(batch, width, n_heads * d, dtype=qkv.dtype, device=dev)
+        out = torch.empty(batch, width, n_heads * d, dtype=dtype, device=dev)
+        s0, s1 = width * n_heads * d, n_heads * d
     else:
-        _on(dev, out, "out", qkv.dtype)
+        if out.get_device() != index or out.dtype is not dtype:
+            _on(dev, out, "out", dtype)
         if out.shape != (batch, width, n_heads * d):
             raise ValueError(f"out must be {[batch, width, n_heads * d]} (got {list(out.shape)})")
         s0, s1, s2 = out.stride()
         if s2 != 1 or width > 1 and s1 < n_heads * d or batch > 1 and s0 < (width - 1) * s1 + n_heads * d:
             raise ValueError("out needs unit inner stride and rows that do not overlap")
-    ws = _tree_workspace(dev, batch, nodes, first, n_heads, kv_heads, d, dt, bs, max_kv_len)
-    st = _launch(dev.index, lib().specdec_tree_attention, qkv.data_ptr(), dt, qkv.stride(0), qkv.stride(1), cos.data_ptr(),
+    # split partials: memory of the call's own, from torch's allocator, so calls on
+    # several streams or in several graphs share none
+    floats = _tree_floats(batch, nodes, first, n_heads, kv_heads, d, dt, bs, max_kv_len)
+    ws = torch.empty(floats, dtype=torch.float32, device=dev) if floats else None
+    st = _launch(index, lib().specdec_tree_attention, qkv.data_ptr(), dt, strides[0], strides[1], cos.data_ptr(),
                  sin.data_ptr(), cos.shape[0], k_pool.data_ptr(), v_pool.data_ptr(), blocks, tables.data_ptr(),
-                 tables.stride(0), tables.shape[0], tables.shape[1], meta.data_ptr(), mask.data_ptr(), mask_stride,
-                 mask.stride(1), depth.data_ptr(), depth_stride, batch, nodes, first, n_heads, kv_heads, d, bs, scale,
-                 max_kv_len, ptr(ws), 0 if ws is None else ws.numel(), out.data_ptr(), out.stride(0), out.stride(1))
+                 tables.stride(0), tables.shape[0], tables.shape[1], meta.data_ptr(), mask.data_ptr(), mask_strides[0],
+                 mask_strides[1], depth.data_ptr(), depth_strides[0], batch, nodes, first, n_heads, kv_heads, d, bs, scale,
+                 max_kv_len, None if ws is None else ws.data_ptr(), floats, out.data_ptr(), s0, s1)
     if st:
         _check(st, "tree_attention")
     return out
-
-
-def _tree_workspace(dev: torch.device, *sizes) -> torch.Tensor | None:
-    """A call's split partials: memory of the call's own, from torch's
-    allocator, so calls on several streams or in several graphs share none."""
-    import ctypes
-
-    floats = ctypes.c_int64()
-    _check(lib().specdec_tree_attention_workspace(*sizes, ctypes.byref(floats)), "tree_attention")
-    return torch.empty(floats.value, dtype=torch.float32, device=dev) if floats.value else None
 
 
 def tree_commit(tokens: torch.Tensor, parents: torch.Tensor, sampled: torch.Tensor, meta: torch.Tensor,
@@ -1385,42 +1404,48 @@ def tree_commit(tokens: torch.Tensor, parents: torch.Tensor, sampled: torch.Tens
     blocks of `room` slots past each row's cached length.  The path has at most
     `room` nodes (N where not given).  A row without a live node or a slot gets n =
     -1 and token -1."""
-    if not tokens.is_cuda:
+    index = tokens.get_device()
+    if index < 0:
         gpu(tokens, "tokens")
-    dev = tokens.device
-    if tokens.dim() != 2:
-        raise ValueError(f"tokens must be [B, N] (got {list(tokens.shape)})")
-    batch, nodes = tokens.shape
+    dev, shape = tokens.device, tokens.shape
+    if len(shape) != 2:
+        raise ValueError(f"tokens must be [B, N] (got {list(shape)})")
+    batch, nodes = shape
     if not 0 < nodes <= TREE_NODES:
         raise ValueError(f"a tree has 1 to {TREE_NODES} nodes (got {nodes})")
-    room = nodes if room is None else room
-    if room < 1:
+    if room is None:
+        room = nodes
+    elif room < 1:
         raise ValueError(f"room must be at least 1, for node 0 (got {room})")
-    tokens_stride = _per_tree(dev, tokens, batch, (nodes,), torch.int64, "tokens")
-    sampled_stride = _per_tree(dev, sampled, batch, (nodes,), torch.int64, "sampled")
-    if sampled.shape[0] != batch:
+    if sampled.shape != shape:
         raise ValueError(f"sampled must be [{batch}, {nodes}] (got {list(sampled.shape)})")
-    parents_stride = _per_tree(dev, parents, batch, (nodes,), torch.int32, "parents")
-    _on(dev, meta, "meta", torch.int32, True, 3 * batch)
-    cache = [None, F32, 0, 0, 0, 0, None, None, 0, 0, 0, 0, 0, None, None, 0, None, 0, 0, 0]
+    tokens_stride = _per_tree(dev, index, tokens, batch, (nodes,), torch.int64, "tokens")[0]
+    sampled_stride = _per_tree(dev, index, sampled, batch, (nodes,), torch.int64, "sampled")[0]
+    parents_stride = _per_tree(dev, index, parents, batch, (nodes,), torch.int32, "parents")[0]
+    if meta.get_device() != index or meta.dtype is not torch.int32 or meta.numel() != 3 * batch or not meta.is_contiguous():
+        _on(dev, meta, "meta", torch.int32, True, 3 * batch)
     if qkv is not None:
-        dt = _FP8_INPUTS.get(qkv.dtype)
+        dtype, qshape, strides = qkv.dtype, qkv.shape, qkv.stride()
+        dt = _FP8_INPUTS.get(dtype)
         if dt is None:
-            raise TypeError(f"qkv must be bf16 or fp32 (got {qkv.dtype})")
-        _on(dev, qkv, "qkv")
-        blocks, kv_heads, bs, d = _tree_side(dev, qkv.dtype, cos, sin, k_pool, v_pool, tables, 1)
-        if qkv.dim() != 4 or qkv.shape[:3] != (k_pool.shape[0], batch, nodes):
-            raise ValueError(f"qkv must be [{k_pool.shape[0]}, {batch}, {nodes}, (H + 2 Hkv) * head_dim] (got "
-                             f"{list(qkv.shape)})")
-        heads = _tree_rows(qkv, kv_heads, d)
-        cache = [qkv.data_ptr(), dt, qkv.shape[0], qkv.stride(0), qkv.stride(1), qkv.stride(2), cos.data_ptr(),
-                 sin.data_ptr(), cos.shape[0], heads, kv_heads, d, bs, k_pool.data_ptr(), v_pool.data_ptr(), blocks,
-                 tables.data_ptr(), tables.stride(0), tables.shape[0], tables.shape[1]]
+            raise TypeError(f"qkv must be bf16 or fp32 (got {dtype})")
+        if qkv.get_device() != index:
+            _on(dev, qkv, "qkv")
+        blocks, kv_heads, bs, d = _tree_side(dev, index, dtype, cos, sin, k_pool, v_pool, tables, 1)
+        layers = k_pool.shape[0]
+        if len(qshape) != 4 or qshape[:3] != (layers, batch, nodes):
+            raise ValueError(f"qkv must be [{layers}, {batch}, {nodes}, (H + 2 Hkv) * head_dim] (got {list(qshape)})")
+        heads = _tree_rows(qkv, qshape, strides, kv_heads, d)
+        cache = (qkv.data_ptr(), dt, layers, strides[0], strides[1], strides[2], cos.data_ptr(), sin.data_ptr(),
+                 cos.shape[0], heads, kv_heads, d, bs, k_pool.data_ptr(), v_pool.data_ptr(), blocks, tables.data_ptr(),
+                 tables.stride(0), tables.shape[0], tables.shape[1])
     elif k_pool is not None or v_pool is not None:
         raise ValueError("a commit to a cache needs the layers' qkv")
-    verdict = torch.empty(nodes + 1, batch, dtype=torch.int64, device=dev)
-    path = torch.empty(batch, nodes, dtype=torch.int32, device=dev)
-    st = _launch(dev.index, lib().specdec_tree_commit, tokens.data_ptr(), tokens_stride, parents.data_ptr(), parents_stride,
+    else:
+        cache = (None, F32, 0, 0, 0, 0, None, None, 0, 0, 0, 0, 0, None, None, 0, None, 0, 0, 0)
+    verdict = torch.empty_strided((nodes + 1, batch), (batch, 1), dtype=torch.int64, device=dev)
+    path = torch.empty_strided((batch, nodes), (nodes, 1), dtype=torch.int32, device=dev)
+    st = _launch(index, lib().specdec_tree_commit, tokens.data_ptr(), tokens_stride, parents.data_ptr(), parents_stride,
                  sampled.data_ptr(), sampled_stride, meta.data_ptr(), batch, nodes, room, verdict.data_ptr(),
                  path.data_ptr(), *cache)
     if st:
