@@ -128,10 +128,12 @@ class KVCache:
         self.allocator.flush()
 
     # -- append --------------------------------------------------------------
-    def append(self, seq_ids: list[int], n_new: list[int]) -> PagedStep:
+    def append(self, seq_ids: list[int], n_new: list[int], nodes: list[int] | None = None) -> PagedStep:
         """Reserve slots for n_new[b] tokens on each row; lengths advance now.
         Rows grow in order and an OutOfBlocks leaves earlier rows grown, as in
-        cache/kv.py:83-85."""
+        cache/kv.py:83-85.  With `nodes` the step is that of a tree of nodes[b]
+        drafted tokens, of which n_new[b] at most are kept: the metadata's third
+        row holds the nodes (ops.tree_attention, ops.tree_commit)."""
         width = max(n_new)
         past = [self.tables[s].length for s in seq_ids]
         pops: list[tuple[int, int, int]] = []
@@ -149,7 +151,7 @@ class KVCache:
                 table._n += needed
             table.length += n
         rows = [self.tables[s].row for s in seq_ids]
-        host = rows + past + list(n_new)
+        host = rows + past + list(n_new if nodes is None else nodes)
         meta = alloc._plan(self._store, pops, tail=host)  # one upload for the plan and the metadata
         if failure is not None:
             raise failure

@@ -37,6 +37,7 @@ import torch.nn.functional as F
 
 from cache.kv import KVCache
 from lm.model import Llama, as_llama
+from lm.tree import TreeStep
 from specdec import ops
 
 
@@ -121,7 +122,7 @@ def _project_add(hidden: torch.Tensor, x: torch.Tensor, w: torch.Tensor, gemv: b
 def forward_core(llama: Llama, cache: KVCache, meta: torch.Tensor, ids: torch.Tensor, max_kv_len: int,
                  last: torch.Tensor | None = None, workspace: ops.AttentionWorkspace | None = None,
                  split_tokens: int = 0, temperature: float | None = None, out: torch.Tensor | None = None,
-                 index_out: torch.Tensor | None = None) -> torch.Tensor:
+                 index_out: torch.Tensor | None = None, tree: TreeStep | None = None) -> torch.Tensor:
     """Device-only forward of ids [B, T] whose rows were appended with `meta`
     (int32 [3, B] on the device).  `max_kv_len` bounds every row's cached
     length after the append; `last` (int64 [B]) selects one row per batch
@@ -131,7 +132,9 @@ def forward_core(llama: Llama, cache: KVCache, meta: torch.Tensor, ids: torch.Te
     bits need not match other calls, which also lets single-row projections
     run as matrix-vector products).  With a `temperature` the result is the
     probabilities of the logits instead (`out`, `index_out` as in
-    `probabilities`)."""
+    `probabilities`).  With a `tree` the ids are nodes of a tree of drafted
+    tokens: its attention takes the place of the causal one, and nothing is
+    appended to the cache (lm/tree.py)."""
     cfg = llama.config
     gemv = split_tokens != 0
     b, t = ids.shape
@@ -141,12 +144,12 @@ def forward_core(llama: Llama, cache: KVCache, meta: torch.Tensor, ids: torch.Te
     layers = llama.layers
     hidden = F.embedding(ids, llama.embed)
     if llama.is_fp8:
-        x = _fp8_layers(llama, cache, meta, hidden, max_kv_len, workspace, split_tokens)
+        x = _fp8_layers(llama, cache, meta, hidden, max_kv_len, workspace, split_tokens, tree)
         return _project_out(llama, x, last, temperature, out, index_out)
     x = torch.empty_like(hidden)
     # the attention finishes the input norm for decode-sized calls; else a
     # weightless norm kernel writes x and the projection reads that
-    in_attn = ops.norm_in_attention(hidden.dtype, cache.block_size, t)
+    in_attn = tree is None and ops.norm_in_attention(hidden.dtype, cache.block_size, t)
     if not in_attn:
         ops.add_rmsnorm(hidden, None, llama.unit_norm, x, eps)
     attn = torch.empty(b, t, h * d, dtype=hidden.dtype, device=hidden.device)
@@ -165,6 +168,9 @@ def forward_core(llama: Llama, cache: KVCache, meta: torch.Tensor, ids: torch.Te
                                            norm_of=hidden, eps=eps)
             ops.linear_attn_parts(parts, b, h, _linear_weight(attn, layer.wo, layer.wo_t), hidden.view(b, -1),
                                   accumulate=True)
+        elif tree is not None:
+            tree.attend(i, qkv, llama, cache, meta, attn)
+            _project_add(hidden, attn, layer.wo, gemv, layer.wo_t)
         else:
             ops.rope_paged_attention(qkv, llama.rope_cos, llama.rope_sin, cache.k[i], cache.v[i], tables, meta, b, t,
                                      h, hk, d, cache.block_size, llama.scaling, max_kv_len, attn, attn.stride(1),
@@ -198,7 +204,7 @@ def _project_out(llama: Llama, x: torch.Tensor, last: torch.Tensor | None, tempe
 
 
 def _fp8_layers(llama: Llama, cache: KVCache, meta: torch.Tensor, hidden: torch.Tensor, max_kv_len: int,
-                workspace: ops.AttentionWorkspace | None, split_tokens: int) -> torch.Tensor:
+                workspace: ops.AttentionWorkspace | None, split_tokens: int, tree: TreeStep | None = None) -> torch.Tensor:
     """The decoder layers of a model with 8-bit projections over hidden [B, T,
     hidden], and the final norm.  Nine launches a layer: each projection reads
     rows in 8 bits that the norm before it, the attention's output or the MLP's
@@ -214,9 +220,12 @@ def _fp8_layers(llama: Llama, cache: KVCache, meta: torch.Tensor, hidden: torch.
     x = ops.add_rmsnorm_fp8(hidden, None, ones, eps)
     for i, layer in enumerate(llama.layers):
         qkv = ops.linear_fp8(*x, *layer.wqkv)
-        ops.rope_paged_attention(qkv, llama.rope_cos, llama.rope_sin, cache.k[i], cache.v[i], tables, meta, b, t, h, hk,
-                                 d, cache.block_size, llama.scaling, max_kv_len, attn, attn.stride(1), workspace,
-                                 split_tokens)
+        if tree is not None:
+            tree.attend(i, qkv, llama, cache, meta, attn)
+        else:
+            ops.rope_paged_attention(qkv, llama.rope_cos, llama.rope_sin, cache.k[i], cache.v[i], tables, meta, b, t, h,
+                                     hk, d, cache.block_size, llama.scaling, max_kv_len, attn, attn.stride(1), workspace,
+                                     split_tokens)
         ops.linear_fp8(*ops.quantize_fp8(attn), *layer.wo, out=hidden, add=hidden)
         gate_up = ops.linear_fp8(*ops.add_rmsnorm_fp8(hidden, None, ones, eps), *layer.wgu)
         act = ops.silu_mul_fp8(gate_up)

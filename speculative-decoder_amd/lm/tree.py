@@ -6,7 +6,11 @@ in the reference, which drafts a chain (spec/draft.py).
 """
 from __future__ import annotations
 
+from dataclasses import dataclass
+
 import torch
+
+from specdec import ops
 
 
 def plan(parents: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -33,3 +37,34 @@ def plan(parents: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         depth = depth + depth.gather(1, up)
         up = up.gather(1, up)
     return mask.contiguous(), depth.int()
+
+
+@dataclass(frozen=True)
+class TreeStep:
+    """What a forward over tree nodes needs beside a chain's: the masks int64 [B
+    or 1, N - first, ..] of the nodes that it runs, first .. N - 1, the depths
+    int32 [B or 1, N] of all, and `qkv` [layers, B, N, ..], where each layer's
+    projections of the nodes are kept for the levels after them and for the
+    commit.  `past` bounds the rows' cached lengths."""
+
+    mask: torch.Tensor
+    depth: torch.Tensor
+    qkv: torch.Tensor
+    past: int
+    first: int = 0
+
+    @staticmethod
+    def store(llama, batch: int, nodes: int) -> torch.Tensor:
+        """An empty `qkv` for `nodes` nodes of `batch` rows."""
+        cfg = llama.config
+        row = (cfg.num_attention_heads + 2 * cfg.num_key_value_heads) * cfg.head_dim
+        return torch.empty(len(llama.layers), batch, nodes, row, dtype=llama.embed.dtype, device=llama.embed.device)
+
+    def attend(self, layer: int, qkv: torch.Tensor, llama, cache, meta: torch.Tensor, out: torch.Tensor) -> None:
+        """The attention of this step's nodes in one layer, from their
+        projections qkv [B, N - first, ..], into out."""
+        kept = self.qkv[layer]
+        kept[:, self.first:].copy_(qkv)
+        ops.tree_attention(kept, llama.rope_cos, llama.rope_sin, cache.k[layer], cache.v[layer], cache.table_tensor, meta,
+                           self.mask, self.depth, llama.config.num_attention_heads, llama.scaling, self.past, self.first,
+                           out)
