@@ -53,8 +53,9 @@ __device__ __forceinline__ TreeRow tree_row(const TreeArgs &a, int b) {
 }
 
 // One wave a (query node, head): a lane a key, 64 keys at a time, in fp32.  For
-// any block size, stride and alignment; what it is bound by is its scattered
-// reads.
+// what the tiles below do not take: blocks that are no multiple of 16 bytes of
+// keys, rows that are not 16-byte aligned.  Bound by its scattered reads (8 rows of
+// 32 nodes at 4096 keys, 32 heads: 4.1 ms).
 template <typename T, int D>
 __global__ __launch_bounds__(kWave) void tree_attention_any_kernel(TreeArgs a) {
   const int lane = threadIdx.x, b = blockIdx.z, h = blockIdx.y, i = blockIdx.x, node = a.first + i;
@@ -162,6 +163,9 @@ __global__ __launch_bounds__(kWave) void tree_attention_any_kernel(TreeArgs a) {
 // end, where the workgroup's waves fold their (m, l, O).
 // A lane's row of K holds pieces j and j + NP / 2 of a rotated pair of dims, so the
 // tree's own keys are rotated in the registers that they arrive in.
+// Bound by memory: 8 rows of 32 nodes at 4096 keys, 32 heads of 64, 55 us for 241 MB
+// (85% of a copy's rate); by the dependent round trips of metadata, tables, nodes
+// and keys where these are few (one row of 16 nodes at 300 keys 7.1 us).
 constexpr int kTreeWaves = 4;
 
 template <typename T, int D> struct TreeTile {
@@ -240,6 +244,7 @@ __device__ __forceinline__ void tree_row_pieces(const TreeArgs &a, const T *row,
 // rows, splits over the cached keys.
 struct TreeCut {
   int tiles, groups, splits;
+  bool shared;  // the grid whose waves share their keys
   __host__ __device__ int64_t rows() const { return (int64_t)groups * tiles * 16; }  // of a kv head, with padding
 };
 
@@ -252,8 +257,9 @@ __host__ __device__ inline TreeParts tree_parts(float *ws, int64_t unit, int64_t
   return TreeParts{ws + unit * rows * 2, ws + units * rows * 2 + unit * rows * d};
 }
 
-// Waves a SIMD that a variant's registers are held to.
-constexpr int tree_waves(int d, int tiles) { return d == 64 ? (tiles == 1 ? 3 : tiles == 2 ? 2 : 1) : (tiles == 1 ? 2 : 1); }
+// Waves a SIMD that a variant's registers are held to: 168, 256 and 512 of them
+// for q, O, two chunks of K and V and the tree's tables.
+constexpr int tree_waves(int d, int tiles) { return (d == 64 ? 4 : 3) - tiles; }
 
 template <typename T, int D, int NT>
 __global__ __launch_bounds__(kTreeWaves *kWave)
@@ -537,6 +543,328 @@ __global__ __launch_bounds__(kTreeWaves *kWave)
   }
 }
 
+// The same for more than 32 query rows a kv head: NW waves share a chunk of 2 CK
+// keys through LDS, each with up to NT tiles of its own, so the keys are read once
+// for 16 NT NW query rows and no wave's state has to be folded with another's.
+// The next chunk is in flight in registers while this one is used; one barrier a
+// chunk, two buffers.  Against the grid above with four tiles a wave: 8 rows of 64
+// nodes at 4096 keys, one query head a kv head, 85 -> 65 us (73% of the bytes at a
+// copy's rate); 4 rows of 64 nodes at 8000 keys, four query heads a kv head of 64,
+// 72 -> 46, and of 128, where that grid has room for two tiles, 116 -> 76.  There it
+// is bound by its instructions: 11.5 k vector and 1.8 k matrix instructions a SIMD
+// are some 31 of the 60 us, with two waves a SIMD to hide the rest; the splits'
+// partials (34 MB) and their fold are most of the others.
+// K is kept in the order of the score tiles' rows, rows of 4 NP pieces; V as in the
+// cache, rows of 8 pieces; a piece's place in its row is its number xor the row's
+// low bits, so that the lanes of a read fall on different banks.
+template <typename T, int D, int NW> struct TreeShared {
+  using L = TreeTile<T, D>;
+  static constexpr int KC = 2 * L::CK, PR = 4 * L::NP, THREADS = NW * kWave;
+  static constexpr int KS = KC * PR / THREADS, VS = D * 8 / THREADS;  // pieces that a thread brings
+  static_assert(KS > 0 && VS > 0 && KS * THREADS == KC * PR && VS * THREADS == D * 8, "whole pieces a thread");
+  u32x4 k[2][KC * PR], v[2][D * 8];
+  int odd;  // a value of the tree is no number
+  static __device__ __forceinline__ int k_at(int key, int p) {  // of a chunk's key, piece p of its row
+    const int in = key % L::CK, row = (key / L::CK * L::NTK + in % L::EPL / 4) * 16 + in / L::EPL * 4 + in % 4;
+    return row * PR + (p ^ (row & 7));
+  }
+  static __device__ __forceinline__ int v_at(int d, int p) { return d * 8 + (p ^ (d & 7)); }
+};
+
+template <typename T, int D, int NW, int NT>
+__global__ __launch_bounds__(NW *kWave) __attribute__((amdgpu_waves_per_eu(NT == 1 ? 4 : 2, NT == 1 ? 4 : 2))) void
+tree_attention_shared_kernel(TreeArgs a, TreeCut cut, int shift, float *ws) {
+  using L = TreeTile<T, D>;
+  using S = TreeShared<T, D, NW>;
+  constexpr int EPL = L::EPL, CK = L::CK, NTK = L::NTK, NP = L::NP, ND = L::ND, KC = S::KC, PR = S::PR;
+  __shared__ S sh;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, c = lane & 15, g = lane / 16;
+  const int units = a.batch * a.Hkv * cut.splits;
+  int unit = blockIdx.x, qg = 0;
+  if (cut.groups > 1) {  // as above: query groups of one unit on one XCD
+    const int rest = unit / 8;
+    qg = rest % cut.groups;
+    unit = rest / cut.groups * 8 + unit % 8;
+    if (unit >= units) return;
+  }
+  const int split = unit % cut.splits, bh = unit / cut.splits, hk = bh % a.Hkv, b = bh / a.Hkv;
+  const int G = a.H / a.Hkv;
+  const TreeRow r = tree_row(a, b);
+  const int row0 = qg * cut.tiles * 16, nrows = (r.live - a.first) * G;
+  if (row0 >= nrows) return;
+  bool bad = !r.fits;
+  const int past = r.fits ? r.past : 0, live = r.live;
+  const T *rows = (const T *)a.qkv + b * a.batch_stride;
+  const int32_t *depth = a.depth + b * a.depth_batch_stride;
+  const int32_t *table = a.tables + (r.fits ? r.row * a.table_stride : 0);
+  const auto first_row = [&](int t) { return row0 + 16 * (wave + NW * t); };  // of this wave's tile t
+  int tiles = 0;
+
+  u32x4 q[NT][NP];
+  f32x4 o[NT][ND];
+  float m[NT], l[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    if (first_row(t) < nrows) tiles = t + 1;
+    const int qr = min(first_row(t) + c, nrows - 1), node = a.first + qr / G;
+    tree_row_pieces<T, D>(a, rows + node * a.token_stride + (int64_t)(hk * G + qr % G) * D, (int64_t)r.past + depth[node], g,
+                          q[t]);
+    m[t] = -INFINITY;
+    l[t] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const float sc = a.scale * 1.4426950408889634f;
+
+  // half a chunk (CK keys) of buffer `buf` against this wave's tiles; hide(t, s) puts
+  // the scores of keys that a query does not see to -inf
+  const auto use = [&](int buf, int half, bool odd, int keys, auto &&hide) __attribute__((always_inline)) {
+    if (tiles == 0) return;
+    float s[NT][EPL];
+#pragma unroll
+    for (int tk = 0; tk < NTK; ++tk) {
+      const int row = (half * NTK + tk) * 16 + c;
+      u32x4 k[NP];
+#pragma unroll
+      for (int j = 0; j < NP; ++j) k[j] = sh.k[buf][row * PR + ((4 * j + g) ^ (row & 7))];
+      f32x4 acc[NT];  // a tile that the wave does not have costs less than the branches around it
+#pragma unroll
+      for (int t = 0; t < NT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < NP; ++j)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[t] = tree_mma(T(), k[j], q[t][j], acc[t]);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[t][4 * tk + i] = acc[t][i];
+    }
+    // K's registers are free before V's are taken: all at once are spilled, and a
+    // reload waits for the chunk in flight
+    __builtin_amdgcn_sched_barrier(0);
+    constexpr int VN = ND < 4 ? ND : 4;
+    u32x4 v[VN], p[NT];
+    const auto take = [&](int d0) __attribute__((always_inline)) {
+#pragma unroll
+      for (int d = 0; d < VN; ++d) v[d] = sh.v[buf][S::v_at(16 * (d0 + d) + c, half * 4 + g)];
+    };
+    take(0);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      hide(t, s[t]);
+      float top = s[t][0];
+#pragma unroll
+      for (int e = 1; e < EPL; ++e) top = fmaxf(top, s[t][e]);
+      top *= sc;
+      if (__any(top > m[t] + 8.0f)) {  // as above
+        top = fmaxf(top, __shfl_xor(top, 16, kWave));
+        top = fmaxf(top, __shfl_xor(top, 32, kWave));
+        const float m_new = fmaxf(m[t], top);
+        const float f = m[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[t] - m_new);
+        m[t] = m_new;
+        l[t] *= f;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[t][d] *= f;
+      }
+      const float base = m[t] == -INFINITY ? 0.0f : m[t];
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) {
+        s[t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e], sc, -base));
+        l[t] += s[t][e];
+      }
+      p[t] = tree_pack(s[t]);
+      if (odd) {
+        for (int key = 0; key < keys; ++key) {  // 0 times what is no number is left out
+          float pk = 0.0f;
+#pragma unroll
+          for (int e = 0; e < EPL; ++e) pk = key % EPL == e ? s[t][e] : pk;
+          pk = __shfl(pk, key / EPL * 16 + c, kWave);
+          if (pk == 0.0f) continue;
+#pragma unroll
+          for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              o[t][d][i] += pk * to_f32(((const T *)&sh.v[buf][S::v_at(16 * d + 4 * g + i, half * 4 + key / EPL)])[key % EPL]);
+        }
+      }
+    }
+    if (odd) return;
+#pragma unroll
+    for (int d0 = 0; d0 < ND; d0 += VN) {
+      if (d0 > 0) {
+        take(d0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int d = 0; d < VN; ++d)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) o[t][d0 + d] = tree_mma(T(), v[d], p[t], o[t][d0 + d]);
+    }
+  };
+
+  // ---- the tree's own keys, chunks dealt over the splits
+  for (int n0 = split * KC; n0 < live; n0 += cut.splits * KC) {
+    __syncthreads();
+    if (tid == 0) sh.odd = 0;
+    __syncthreads();
+    for (int i = tid; i < KC * PR / 2; i += S::THREADS) {
+      const int key = i / (PR / 2), p = i % (PR / 2), node = min(n0 + key, live - 1);
+      const int64_t pos = (int64_t)r.past + depth[node];
+      const bool in = pos >= 0 && pos < a.positions;
+      const T *row = rows + node * a.token_stride + (int64_t)(a.H + hk) * D + EPL * p;
+      u32x4 lo = *(const u32x4 *)row, hi = *(const u32x4 *)(row + D / 2);
+      float co[EPL], si[EPL];
+#pragma unroll
+      for (int e = 0; e < EPL; e += 4) {
+        *(f32x4 *)&co[e] = *(const f32x4 *)(a.cos_t + (in ? pos : 0) * (D / 2) + EPL * p + e);
+        *(f32x4 *)&si[e] = *(const f32x4 *)(a.sin_t + (in ? pos : 0) * (D / 2) + EPL * p + e);
+      }
+      tree_rotate<EPL>(lo, hi, co, si, in);
+      sh.k[0][S::k_at(key, p)] = lo;
+      sh.k[0][S::k_at(key, p + PR / 2)] = hi;
+    }
+    for (int i = tid; i < KC * PR; i += S::THREADS) {
+      const int key = i / PR, p = i % PR, node = min(n0 + key, live - 1);
+      const u32x4 v = *(const u32x4 *)(rows + node * a.token_stride + (int64_t)(a.H + a.Hkv + hk) * D + EPL * p);
+      float x[EPL];
+      tree_unpack(v, x);
+      bool finite = true;
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) {
+        finite &= fabsf(x[e]) < INFINITY;
+        ((T *)&sh.v[0][S::v_at(EPL * p + e, key / EPL)])[key % EPL] = from_f32<T>(x[e]);
+      }
+      if (!finite) sh.odd = 1;
+    }
+    __syncthreads();
+    const bool odd = sh.odd != 0;
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half)
+      use(0, half, odd, min(CK, max(0, live - n0 - half * CK)), [&](int t, float(&s)[EPL]) __attribute__((always_inline)) {
+        const int key = n0 + half * CK + EPL * g, qr = min(first_row(t) + c, nrows - 1);
+        const uint64_t word = key < live ? a.mask[b * a.mask_batch_stride + qr / G * a.mask_row_stride + key / 64] : 0;
+        const unsigned seen = (unsigned)(word >> (key % 64));
+#pragma unroll
+        for (int e = 0; e < EPL; ++e)
+          if (!(seen >> e & 1) || key + e >= live) s[e] = -INFINITY;
+      });
+  }
+
+  // ---- the cached keys: this split's chunks
+  const int chunks = (past + KC - 1) / KC, per = (chunks + cut.splits - 1) / cut.splits;
+  const int begin = split * per, end = min(chunks, begin + per);
+  const int64_t tile = (int64_t)a.bs * D, stride = tile * a.Hkv;
+  const T *kp = (const T *)a.k_pool + hk * tile, *vp = (const T *)a.v_pool + hk * tile;
+  const unsigned most = a.num_blocks - 1;
+  struct Ids {
+    int k[S::KS], v[S::VS];
+  };
+  struct Brought {
+    u32x4 k[S::KS], v[S::VS];
+  };
+  const auto page = [&](int key) { return shift >= 0 ? key >> shift : key / a.bs; };
+  const auto k_key = [&](int ch, int i) { return min(ch * KC + (tid + i * S::THREADS) / PR, past - 1); };
+  const auto v_key = [&](int ch, int i) {
+    return min(ch * KC + (tid + i * S::THREADS) % 8 * EPL, (past - 1) & ~(EPL - 1));
+  };
+  const auto look = [&](int ch, Ids &w) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < S::KS; ++i) w.k[i] = table[page(k_key(ch, i))];
+#pragma unroll
+    for (int i = 0; i < S::VS; ++i) w.v[i] = table[page(v_key(ch, i))];
+  };
+  const auto bring = [&](int ch, const Ids &w, Brought &x) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < S::KS; ++i) {
+      bad |= (unsigned)w.k[i] > most;
+      const int key = k_key(ch, i);
+      x.k[i] = *(const u32x4 *)(kp + min((unsigned)w.k[i], most) * stride + (int64_t)(key - page(key) * a.bs) * D +
+                                (tid + i * S::THREADS) % PR * EPL);
+    }
+#pragma unroll
+    for (int i = 0; i < S::VS; ++i) {
+      bad |= (unsigned)w.v[i] > most;
+      const int key = v_key(ch, i);
+      x.v[i] = *(const u32x4 *)(vp + min((unsigned)w.v[i], most) * stride + (int64_t)((tid + i * S::THREADS) / 8) * a.bs + key -
+                                page(key) * a.bs);
+    }
+  };
+  const auto put = [&](int ch, int buf, Brought &x) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < S::KS; ++i) sh.k[buf][S::k_at((tid + i * S::THREADS) / PR, (tid + i * S::THREADS) % PR)] = x.k[i];
+#pragma unroll
+    for (int i = 0; i < S::VS; ++i) {
+      const int p = (tid + i * S::THREADS) % 8, left = past - ch * KC - p * EPL;
+      if (left < EPL) {  // slots behind the cached length hold anything at all
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          if constexpr (sizeof(T) == 2)
+            x.v[i][w] = 2 * w + 1 < left ? x.v[i][w] : 2 * w < left ? x.v[i][w] & 0xFFFFu : 0u;
+          else
+            x.v[i][w] = w < left ? x.v[i][w] : 0u;
+        }
+      }
+      sh.v[buf][S::v_at((tid + i * S::THREADS) / 8, p)] = x.v[i];
+    }
+  };
+  if (begin < end) {
+    Ids w;
+    Brought x;
+    look(begin, w);
+    bring(begin, w, x);
+    look(min(begin + 1, end - 1), w);
+    __syncthreads();  // the tree's chunk has been used
+    put(begin, 0, x);
+    __syncthreads();
+    for (int ch = begin; ch < end; ++ch) {
+      const int buf = (ch - begin) & 1;
+      if (ch + 1 < end) {
+        bring(ch + 1, w, x);
+        look(min(ch + 2, end - 1), w);
+      }
+#pragma unroll 1
+      for (int half = 0; half < 2; ++half)
+        use(buf, half, false, 0, [&](int, float(&s)[EPL]) __attribute__((always_inline)) {
+          const int left = past - ch * KC - half * CK - EPL * g;
+          if (left < EPL) {
+#pragma unroll
+            for (int e = 0; e < EPL; ++e)
+              if (e >= left) s[e] = -INFINITY;
+          }
+        });
+      if (ch + 1 < end) put(ch + 1, buf ^ 1, x);
+      __syncthreads();
+    }
+  }
+  bad = __syncthreads_or(bad);
+
+  const TreeParts parts = tree_parts(ws, unit, units, cut.rows(), D);
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    if (t >= tiles) break;
+    float sum = l[t] + __shfl_xor(l[t], 16, kWave);
+    sum += __shfl_xor(sum, 32, kWave);
+    if (bad) sum = NAN;
+    const int qr = first_row(t) + c;
+    if (qr >= nrows) continue;
+    if (cut.splits > 1) {
+      if (g == 0) {
+        parts.ml[qr * 2] = m[t];
+        parts.ml[qr * 2 + 1] = sum;
+      }
+#pragma unroll
+      for (int d = 0; d < ND; ++d) *(f32x4 *)&parts.o[(int64_t)qr * D + 16 * d + 4 * g] = o[t][d];
+    } else {
+      T *out = (T *)a.out + b * a.out_batch_stride + qr / G * a.out_token_stride + (int64_t)(hk * G + qr % G) * D + 4 * g;
+      const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out[16 * d + i] = from_f32<T>(sum != 0.0f ? o[t][d][i] * inv : 0.0f);
+    }
+  }
+}
+
 // Folds the splits' partials, D / 4 lanes a query row.
 template <typename T, int D> __global__ __launch_bounds__(256) void tree_fold_kernel(TreeArgs a, TreeCut cut, float *ws) {
   constexpr int LANES = D / 4, PER = 256 / LANES;
@@ -566,7 +894,8 @@ template <typename T, int D> __global__ __launch_bounds__(256) void tree_fold_ke
 inline TreeCut tree_cut(int batch, int queries, int H, int Hkv, int d, int dtype, int max_kv) {
   const int rows = queries * (H / Hkv), need = (rows + 15) / 16;
   TreeCut cut;
-  cut.tiles = need <= 1 ? 1 : need <= 2 || d == 128 ? 2 : 4;
+  cut.shared = need > 2;
+  cut.tiles = cut.shared ? (need <= 8 ? 8 : 16) : need;
   cut.groups = (need + cut.tiles - 1) / cut.tiles;
   const int ck = dtype == SPECDEC_BF16 ? 32 : 16, chunks = (max_kv + ck - 1) / ck;
   const int64_t units = (int64_t)batch * Hkv * cut.groups;
@@ -575,8 +904,9 @@ inline TreeCut tree_cut(int batch, int queries, int H, int Hkv, int d, int dtype
   // gives (measured: 8 rows of 32 nodes at 4096 keys 55.9 / 56.8 / 64.5 us in 1 / 2 /
   // 4 splits, one row of 16 at 300 keys 7.6 / 9.8 in 1 / 2, four fp32 rows of 13 at
   // 1500 keys 34.5 / 26.4 / 26.6 / 34.8 in 1 / 2 / 4 / 8)
-  int64_t splits = 512 / units;
-  splits = splits < chunks / (4 * kTreeWaves) ? splits : chunks / (4 * kTreeWaves);
+  int64_t splits = (cut.tiles == 16 ? 256 : 512) / units;
+  const int least = cut.shared ? 8 : 4 * kTreeWaves;
+  splits = splits < chunks / least ? splits : chunks / least;
   cut.splits = (int)(splits < 1 ? 1 : splits > 64 ? 64 : splits);
   return cut;
 }
@@ -744,9 +1074,12 @@ template <typename T, int D> int launch_tree_tiles(const TreeArgs &a, const Tree
   while (1 << shift < a.bs) ++shift;
   if (1 << shift != a.bs) shift = -1;
   const dim3 block(kTreeWaves * kWave);
-  if (cut.tiles == 1) tree_attention_kernel<T, D, 1><<<(unsigned)grid, block, 0, s>>>(a, cut, shift, ws);
-  else if (cut.tiles == 2) tree_attention_kernel<T, D, 2><<<(unsigned)grid, block, 0, s>>>(a, cut, shift, ws);
-  else if constexpr (D == 64) tree_attention_kernel<T, D, 4><<<(unsigned)grid, block, 0, s>>>(a, cut, shift, ws);
+  constexpr int NT = D / 64;  // of 8 tiles: what the registers of four waves a SIMD hold, or of two
+  if (cut.tiles == 16) tree_attention_shared_kernel<T, D, 8, 2><<<(unsigned)grid, 8 * kWave, 0, s>>>(a, cut, shift, ws);
+  else if (cut.tiles == 8)
+    tree_attention_shared_kernel<T, D, 8 / NT, NT><<<(unsigned)grid, 8 / NT * kWave, 0, s>>>(a, cut, shift, ws);
+  else if (cut.tiles == 1) tree_attention_kernel<T, D, 1><<<(unsigned)grid, block, 0, s>>>(a, cut, shift, ws);
+  else tree_attention_kernel<T, D, 2><<<(unsigned)grid, block, 0, s>>>(a, cut, shift, ws);
   if (cut.splits > 1) {
     const int rows = (a.nodes - a.first) * (a.H / a.Hkv), per = 256 / (D / 4);
     tree_fold_kernel<T, D><<<dim3((rows + per - 1) / per, a.Hkv, a.batch), 256, 0, s>>>(a, cut, ws);
