@@ -42,6 +42,7 @@ constexpr int kSamplePieces = 6;    // pieces of 16 bytes of a part; the next pa
 constexpr int kSampleRaw = 4096;    // logits that are collected, each wave its share
 constexpr int kSampleBins = 2048;
 constexpr int kSampleTopK = 400;    // the largest top_k that is bounded by the threads' maxima
+constexpr double kSampleOff = 1.0 / (1 << 17);
 constexpr int kSampleGuess = 128;   // reach the bound in the first part, for a nucleus of unknown size
 
 struct SampleArgs {
@@ -230,7 +231,7 @@ template <int THREADS> struct SampleShared {
   int near[kWave];
   double above;
   float bound;
-  int count, token, last, keep_p, keep_m;
+  int count, token, last, keep_p, keep_q, keep_m;
   unsigned lo, hi;
 };
 
@@ -402,7 +403,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
     if (tid == 0) {
       s.token = V;
       s.last = -1;
-      s.keep_p = s.keep_m = 1;
+      s.keep_p = s.keep_q = s.keep_m = 1;
     }
     x.parts([&](const u32x4(&v)[kSamplePieces], int j0) SAMPLE_INLINE {
       float part[kSamplePieces];
@@ -440,11 +441,18 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
         for (int k = 0; k < kSamplePieces; ++k) {
           if (j0 + k >= x.per) break;
           float e[EPL];
-          double w[EPL];
           x.unpack(v[k], j0 + k, e);
-          sample_weights(e, base, c, w);
+          if (by_p) {
+            float sum = 0.0f;
 #pragma unroll
-          for (int q = 0; q < EPL; ++q) mass += w[q];
+            for (int q = 0; q < EPL; ++q) sum += __builtin_amdgcn_exp2f((e[q] - (float)base) * (float)c);
+            mass += (double)sum;
+          } else {
+            double w[EPL];
+            sample_weights(e, base, c, w);
+#pragma unroll
+            for (int q = 0; q < EPL; ++q) mass += w[q];
+          }
           __builtin_amdgcn_sched_barrier(0);
         }
       }
@@ -496,10 +504,18 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
   };
   const Cut all_ids{-FLT_MAX, INT_MAX};
   // against the row's largest now, or again where the first part was too far from it
+  // For a nucleus the sum is that of 32-bit exponentials, a third of the work: they
+  // are off by 2^-23 and 2^-23 |y| of their powers y, |y| < 40 where they weigh at
+  // all, so by less than kSampleOff together.  Where that leaves a choice the sum is
+  // taken again in 64 bits.
+  bool sure = !by_p;
   if (weigh) {
     const double up = (base - dtop) * c;
-    if (up > -900.0 && up <= 0.0) mass *= sample_weight((float)base, dtop, c);
-    else mass = weights_within(all_ids);
+    if (up > (by_p ? -100.0 : -900.0) && up <= 0.0) mass *= sample_weight((float)base, dtop, c);
+    else {
+      mass = weights_within(all_ids);
+      sure = true;
+    }
   }
   double total = weigh ? block.sum(mass) : 0.0;
   // the least logit of weight m: (x - top) c >= log2 m
@@ -547,10 +563,10 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
   const auto sorted_x = [&](int r) SAMPLE_INLINE { return sample_value((unsigned)(s.found[r] >> 32)); };
   const auto sorted_id = [&](int r) SAMPLE_INLINE { return (int)~(unsigned)s.found[r]; };
   // Of the first n ranked, how many have a mass before them (with `above`) short
-  // of `goal`: into s.keep_p, which holds 1.
-  const auto short_of = [&](int n, double above, double goal) SAMPLE_INLINE {
+  // of `goal`: into `keep`, which holds 1.
+  const auto short_of = [&](int n, double above, double goal, int &keep) SAMPLE_INLINE {
     for (int r = tid; r < n; r += THREADS)
-      if (above + s.before[r] < goal && (r + 1 == n || above + s.before[r + 1] >= goal)) s.keep_p = r + 1;
+      if (above + s.before[r] < goal && (r + 1 == n || above + s.before[r + 1] >= goal)) keep = r + 1;
   };
 
   // ---- 2: the cut among the collected
@@ -600,12 +616,25 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
       rank(n);
       const int upto = k_row > 0 ? min(k_row, n) : n;
       const double all = s.before[upto - 1] + s.weight[upto - 1];
-      if (k_row > 0) total = all;
-      if (by_p) short_of(upto, 0.0, p * total);
+      if (k_row > 0) {
+        total = all;
+        sure = true;
+      }
+      const double off = sure ? 0.0 : kSampleOff;
+      if (by_p) short_of(upto, 0.0, p * total * (1.0 - off), s.keep_p);
+      if (by_p && !sure) short_of(upto, 0.0, p * total * (1.0 + off), s.keep_q);
       if (by_m)
         for (int r = tid; r < n; r += THREADS)
           if (sorted_x(r) >= m_bound && (r + 1 == n || sorted_x(r + 1) < m_bound)) s.keep_m = r + 1;
       __syncthreads();
+      if (by_p && !sure && (s.keep_p != s.keep_q || (all >= p * total * (1.0 - off) && all < p * total * (1.0 + off)))) {
+        total = block.sum(weights_within(all_ids));
+        sure = true;
+        if (tid == 0) s.keep_p = 1;
+        __syncthreads();
+        short_of(upto, 0.0, p * total, s.keep_p);
+        __syncthreads();
+      }
       // whether the ranked hold the cut
       if (k_row > 0 || bound <= -FLT_MAX || (by_m && bound <= m_bound) || (by_p && all >= p * total))
         keep = min(upto, min(by_p ? s.keep_p : n, by_m ? s.keep_m : n));
@@ -692,7 +721,8 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
   // below it, of which many ids have little each, so that a sample holds a like
   // share of it.  The row read once more gives the mass above that range of
   // logits and the ids in it, among which the cut is; false where it is not.
-  const auto nucleus = [&](double goal, Cut &cut) SAMPLE_INLINE {
+  const auto nucleus = [&](Cut &cut) SAMPLE_INLINE {
+    double goal = p * total;
     constexpr int PARTS = 8192 / (THREADS * EPL);  // pieces of a thread in the sample
     if (x.per < 2 * PARTS || !(c > 0.0)) return false;
     const float lo = (float)fmax(dtop - 43.3 / c, (double)-FLT_MAX);
@@ -740,18 +770,23 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
     bound = from;
     collected = 0;
     mass = 0.0;
+    double whole = 0.0;
     x.again([&](const float(&e)[EPL], int i) SAMPLE_INLINE {
       double w[EPL];
       sample_weights(e, dtop, c, w);
       float in[EPL];
 #pragma unroll
       for (int q = 0; q < EPL; ++q) {
+        whole += w[q];
         mass += e[q] > to ? w[q] : 0.0;
         in[q] = e[q] > to ? -INFINITY : e[q];
       }
       collect(in, i);
     });
     const double above = block.sum(mass);
+    total = block.sum(whole);
+    sure = true;
+    goal = p * total;
     if (lane == 0) s.wave_n[wave] = collected;
     const int have = collected;
     // the collected by 2048 ranges again, of weights in units that the largest is 2^45 of
@@ -803,7 +838,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
     if (n > THREADS) return false;
     const double before = s.above;
     rank(n);
-    short_of(n, before, goal);
+    short_of(n, before, goal, s.keep_p);
     __syncthreads();
     cut = Cut{sorted_x(s.keep_p - 1), sorted_id(s.keep_p - 1)};
     for (int r = lane; r < have; r += kWave) {
@@ -929,7 +964,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
       hi = sample_value(s.hi);
       if (n <= THREADS) {
         rank(n);
-        if (!by_count) short_of(n, above, goal);
+        if (!by_count) short_of(n, above, goal, s.keep_p);
         __syncthreads();
         const int last = min(n, by_count ? max(1, (int)(goal - above)) : s.keep_p) - 1;
         return shorter(in, Cut{sorted_x(last), sorted_id(last)});
@@ -939,7 +974,10 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
   };
   Cut cut = all_ids;
   bool summed = weigh && !by_p;  // `mass` is that of the cut
-  if (by_p && k_row == 0) summed = nucleus(p * total, cut);
+  if (by_p && k_row == 0) {
+    summed = nucleus(cut);
+    if (!sure) total = block.sum(weights_within(all_ids));
+  }
 #pragma unroll 1
   for (int turn = 0; turn < 2; ++turn) {  // top-k, then top-p within it
     const bool by_count = turn == 0;
