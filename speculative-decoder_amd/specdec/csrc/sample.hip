@@ -81,6 +81,21 @@ __device__ __forceinline__ double sample_fma(double a, double b, double c) {
 // the 8th power through (2^f - 1) / f at the 9 Chebyshev points, so 2^0 is 1.  N
 // side by side: the chain of one takes its latency 17 times.
 template <int N> __device__ __forceinline__ void sample_weights(const float (&e)[N], double base, double c, double (&w)[N]) {
+  if constexpr (N > 6) {  // .. of up to six: more at once are spilled
+    constexpr int A = N / 2;
+    float e1[A], e2[N - A];
+    double w1[A], w2[N - A];
+#pragma unroll
+    for (int k = 0; k < A; ++k) e1[k] = e[k];
+#pragma unroll
+    for (int k = A; k < N; ++k) e2[k - A] = e[k];
+    sample_weights(e1, base, c, w1);
+    __builtin_amdgcn_sched_barrier(0);
+    sample_weights(e2, base, c, w2);
+#pragma unroll
+    for (int k = 0; k < N; ++k) w[k] = k < A ? w1[k] : w2[k - A];
+    return;
+  }
   constexpr double magic = 6755399441055744.0;  // 1.5 2^52: n in the low bits of a sum
   double f[N];
   int n[N];
