@@ -294,34 +294,46 @@ template <int THREADS> struct SampleBlock {
   }
 };
 
-// A bound that `want` of the threads' maxima in s.tops reach, and not many more:
-// halving between the least and the largest, in wave 0.  -FLT_MAX where fewer are
-// finite.  With its barrier; the caller's stands between the maxima and this.
+// Halves lo .. hi towards the largest bound that `want` of v (N a lane) reach.
+template <int N> __device__ __forceinline__ float sample_halve(const float (&v)[N], int want) {
+  float lo = FLT_MAX, hi = -FLT_MAX;
+  int n = 0;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    n += __popcll(__ballot(v[k] >= -FLT_MAX));
+    lo = fminf(lo, v[k] >= -FLT_MAX ? v[k] : FLT_MAX);
+    hi = fmaxf(hi, v[k]);
+  }
+  if (n < want) return -FLT_MAX;
+  lo = -wave_max_dpp(-lo);
+  hi = fminf(wave_max_dpp(hi), FLT_MAX);
+#pragma unroll 1
+  for (int step = 0; step < 7; ++step) {
+    const float mid = 0.5f * lo + 0.5f * hi;
+    int reach = 0;
+#pragma unroll
+    for (int k = 0; k < N; ++k) reach += __popcll(__ballot(v[k] >= mid));
+    if (reach >= want) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// A bound that `want` of the threads' maxima in s.tops reach, and not many more;
+// -FLT_MAX where fewer are finite.  In wave 0, of every four threads the larger
+// where that leaves four times as many as are wanted.  With its barrier; the caller's
+// stands between the maxima and this.
 template <int THREADS> __device__ __forceinline__ float sample_bound(SampleShared<THREADS> &s, int want) {
   constexpr int N = THREADS / kWave;
   const int lane = threadIdx.x;
   if (lane < kWave) {
-    float v[N], lo = FLT_MAX, hi = -FLT_MAX;
-    int n = 0;
+    float v[N], four[N / 4];
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-      v[k] = s.tops[k * kWave + lane];
-      n += __popcll(__ballot(v[k] >= -FLT_MAX));
-      lo = fminf(lo, v[k] >= -FLT_MAX ? v[k] : FLT_MAX);
-      hi = fmaxf(hi, v[k]);
-    }
-    lo = -wave_max_dpp(-lo);
-    hi = fminf(wave_max_dpp(hi), FLT_MAX);
-#pragma unroll 1
-    for (int step = 0; step < 7; ++step) {
-      const float mid = 0.5f * lo + 0.5f * hi;
-      int reach = 0;
+    for (int k = 0; k < N; ++k) v[k] = s.tops[k * kWave + lane];
 #pragma unroll
-      for (int k = 0; k < N; ++k) reach += __popcll(__ballot(v[k] >= mid));
-      if (reach >= want) lo = mid;
-      else hi = mid;
-    }
-    if (lane == 0) s.bound = n < want ? -FLT_MAX : lo;
+    for (int k = 0; k < N / 4; ++k) four[k] = fmaxf(fmaxf(v[4 * k], v[4 * k + 1]), fmaxf(v[4 * k + 2], v[4 * k + 3]));
+    const float bound = 4 * want <= N / 4 * kWave ? sample_halve(four, want) : sample_halve(v, want);
+    if (lane == 0) s.bound = bound;
   }
   __syncthreads();
   return s.bound;
@@ -441,6 +453,9 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
         s.tops[tid] = top;
         base = (double)block.max(top);
         if (few) bound = sample_bound(s, want);
+        // the least logit of weight m is no lower than against the largest so far; a
+        // top-p within a top-k needs the whole of that
+        if (few && by_m && (k_row == 0 || !by_p)) bound = fmaxf(bound, (float)fmax(base + log2(m) / c, (double)-FLT_MAX));
       }
       if (few) {
 #pragma unroll

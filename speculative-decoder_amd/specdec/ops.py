@@ -1202,7 +1202,8 @@ def _per_row(v, dev: torch.device, rows: int, dtype: torch.dtype, name: str, lo:
 def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
            out: torch.Tensor | None = None, probs: torch.Tensor | None = None) -> torch.Tensor:
     """A token for each row of logits [..., V] (fp32 or bf16) from the row's
-    uniform u [...] (fp32): int64 [...], in `out` where given.
+    uniform u [...] (fp32): int64 [...], in `out` where given.  At most 2^24 ids
+    a row.
 
     Ids are ordered by falling logit, ties by the lower id, with weights w =
     exp((x - max) / temperature).  Kept is the shortest of three prefixes of
@@ -1215,8 +1216,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
 
     temperature, top_p and min_p are numbers or fp32 tensors of a value a row,
     top_k an int or an int32 tensor.  `probs` (fp32 [..., V], rows of any
-    stride) receives the distribution that the token was drawn from, for an
-    accept-reject against it; zeros in a row without a token."""
+    stride, apart from the logits) receives the distribution that the token was
+    drawn from, for an accept-reject against it; zeros in a row without a token."""
     if not logits.is_cuda:
         gpu(logits, "logits")
     dt = _FP8_INPUTS.get(logits.dtype)
@@ -1335,7 +1336,7 @@ def tree_attention(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_po
     nodes are not written, one that sees nothing gets zeros.  Pools as KVCache
     keeps a layer's; the cache is read only (tree_commit writes it).  head_dim 64
     or 128.  max_kv_len is the cached length the launch is laid out for; longer
-    rows are right too, and slower."""
+    rows are right too, and slower.  out and the inputs may not overlap."""
     index = qkv.get_device()
     if index < 0:
         gpu(qkv, "qkv")
@@ -1431,6 +1432,8 @@ def tree_commit(tokens: torch.Tensor, parents: torch.Tensor, sampled: torch.Tens
             raise TypeError(f"qkv must be bf16 or fp32 (got {dtype})")
         if qkv.get_device() != index:
             _on(dev, qkv, "qkv")
+        if cos is None or sin is None or k_pool is None or v_pool is None or tables is None:
+            raise ValueError("a commit to a cache needs qkv, cos, sin, both pools and the tables")
         blocks, kv_heads, bs, d = _tree_side(dev, index, dtype, cos, sin, k_pool, v_pool, tables, 1)
         layers = k_pool.shape[0]
         if len(qshape) != 4 or qshape[:3] != (layers, batch, nodes):
@@ -1440,7 +1443,7 @@ def tree_commit(tokens: torch.Tensor, parents: torch.Tensor, sampled: torch.Tens
                  cos.shape[0], heads, kv_heads, d, bs, k_pool.data_ptr(), v_pool.data_ptr(), blocks, tables.data_ptr(),
                  tables.stride(0), tables.shape[0], tables.shape[1])
     elif k_pool is not None or v_pool is not None:
-        raise ValueError("a commit to a cache needs the layers' qkv")
+        raise ValueError("a commit to a cache needs qkv, cos, sin, both pools and the tables")
     else:
         cache = (None, F32, 0, 0, 0, 0, None, None, 0, 0, 0, 0, 0, None, None, 0, None, 0, 0, 0)
     verdict = torch.empty_strided((nodes + 1, batch), (batch, 1), dtype=torch.int64, device=dev)

@@ -405,7 +405,8 @@ def test_commit_wrapper_refuses():
         (ValueError, dict(sampled=gpu["sampled"][:1])), (ValueError, dict(sampled=gpu["sampled"][:, :11])),
         (TypeError, dict(parents=gpu["parents"].long())), (ValueError, dict(room=0)), (ValueError, dict(meta=gpu["meta"][:2])),
         (ValueError, dict(qkv=gpu["qkv"][0])), (ValueError, dict(qkv=gpu["qkv"][:2])), (TypeError, dict(qkv=gpu["qkv"].half())),
-        (ValueError, dict(qkv=None)), (ValueError, dict(k_pool=gpu["k_pool"][0])), (TypeError, dict(v_pool=gpu["v_pool"].float())),
+        (ValueError, dict(qkv=None)), (ValueError, dict(cos=None)), (ValueError, dict(v_pool=None)),
+        (ValueError, dict(tables=None)), (ValueError, dict(k_pool=gpu["k_pool"][0])), (TypeError, dict(v_pool=gpu["v_pool"].float())),
         (ValueError, dict(cos=gpu["cos"][:, :4])), (TypeError, dict(tables=gpu["tables"].long())),
     ]
     for kind, change in wrong:
