@@ -39,7 +39,7 @@ namespace specdec {
 #define SAMPLE_INLINE __attribute__((always_inline))
 
 constexpr int kSamplePieces = 6;    // pieces of 16 bytes of a part; the next part's are in flight
-constexpr int kSampleRaw = 4096;    // logits that are collected, each wave its share
+constexpr int kSampleShare = 512;   // logits that a wave collects
 constexpr int kSampleBins = 2048;
 constexpr int kSampleTopK = 400;    // the largest top_k that is bounded by the threads' maxima
 constexpr double kSampleOff = 1.0 / (1 << 17);
@@ -228,7 +228,7 @@ template <typename T, int THREADS> struct SampleRow {
 };
 
 template <int THREADS> struct SampleShared {
-  static constexpr int WAVES = THREADS / kWave, SHARE = kSampleRaw / WAVES;
+  static constexpr int WAVES = THREADS / kWave, SHARE = kSampleShare;
   uint64_t raw[WAVES][SHARE];   // as collected: the order of logits, then falling id
   uint64_t bins[kSampleBins];
   uint64_t found[THREADS];      // ranked, as many at once
@@ -385,7 +385,7 @@ template <int THREADS> __device__ __forceinline__ uint64_t sample_sort(SampleSha
 template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4))) void sample_kernel(SampleArgs a) {
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-  constexpr int EPL = 16 / sizeof(T), WAVES = THREADS / kWave, SHARE = kSampleRaw / WAVES;
+  constexpr int EPL = 16 / sizeof(T), WAVES = THREADS / kWave, SHARE = kSampleShare;
   __shared__ SampleShared<THREADS> s;
   SampleBlock<THREADS> block{s};
   SampleRow<T, THREADS> x(a.logits, row * a.row_stride, a.vocab);
@@ -753,9 +753,11 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
   // logits and the ids in it, among which the cut is; false where it is not.
   const auto nucleus = [&](Cut &cut) SAMPLE_INLINE {
     double goal = p * total;
-    constexpr int PARTS = 8192 / (THREADS * EPL);  // pieces of a thread in the sample
+    constexpr int PARTS = 16 / EPL;  // pieces of a thread in the sample: 16 ids
+    // four times what a sum over some half of so many ids is off by
+    constexpr double margin = THREADS == 1024 ? 0.043 : 0.06;
     if (x.per < 2 * PARTS || !(c > 0.0)) return false;
-    const float lo = (float)fmax(dtop - 43.3 / c, (double)-FLT_MAX);
+    const float lo = (float)fmax(dtop - 31.7 / c, (double)-FLT_MAX);  // e^-22: what weighs less shares the last range
     if (!(lo < top)) return false;
     const float scale = (float)(kSampleBins / ((double)top - (double)lo)), c32 = (float)c;
     const auto bin_of = [&](float v) SAMPLE_INLINE { return (int)fminf((top - v) * scale, kSampleBins - 1.0f); };
@@ -789,8 +791,8 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
 #pragma unroll
     for (int q = 0; q < N; ++q) {
       const int bin = kSampleBins - 1 - (N * tid + q);
-      if (below < 0.94 * aim && below + w[q] >= 0.94 * aim) s.near[1] = bin;  // the range ends here
-      if (below < 1.06 * aim && below + w[q] >= 1.06 * aim) s.near[0] = bin;  // .. and begins here
+      if (below < (1.0 - margin) * aim && below + w[q] >= (1.0 - margin) * aim) s.near[1] = bin;  // the range ends here
+      if (below < (1.0 + margin) * aim && below + w[q] >= (1.0 + margin) * aim) s.near[0] = bin;  // .. and begins here
       below += w[q];
     }
     __syncthreads();

@@ -62,6 +62,46 @@ def test_top_p(spread, top_p, dtype):
     check(*rows_of(7, 2, 20011, dtype, spread), top_p=top_p)
 
 
+def flat_rows(seed, rows, vocab, dtype, steep):
+    """Rows whose nucleus holds thousands of ids: probability falls as rank^-steep."""
+    g = torch.Generator().manual_seed(seed)
+    rank = torch.stack([torch.randperm(vocab, generator=g) for _ in range(rows)]).float() + 1
+    x = 12 - steep * rank.log() + 0.5 * torch.randn(rows, vocab, generator=g)
+    return x.to(dtype), torch.rand(rows, generator=g)
+
+
+@pytest.mark.parametrize("vocab", [16411, 49152, 65537, 128001])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("steep,kw", [(0.9, dict(top_p=0.9)), (1.0, dict(top_p=0.5, temperature=1.3)),
+                                      (0.8, dict(top_p=0.98, min_p=0.0005)), (0.9, dict(top_p=0.7, top_k=6000)),
+                                      (1.1, dict(top_p=0.9999))])
+def test_wide_nuclei(vocab, dtype, steep, kw):
+    check(*flat_rows(vocab, 3, vocab, dtype, steep), **kw)
+
+
+@pytest.mark.parametrize("vocab,rows", [(1003, 700), (20000, 300), (49152, 270)])
+@pytest.mark.parametrize("kw", [dict(top_p=0.9), dict(top_k=40, top_p=0.9), dict(), dict(min_p=0.02, top_p=0.95),
+                                dict(temperature=0.0)])
+def test_more_rows_than_compute_units(vocab, rows, kw):
+    x, u = flat_rows(rows, rows, vocab, torch.float32, 1.0)
+    x[::2] *= 2.0  # every other row peaked
+    check(x, u, **kw)
+
+
+def test_wide_nuclei_that_no_sample_shows():
+    """Rows of one value; of two; weights that only a stretch of ids has; ids in falling and rising order."""
+    v = 49152
+    x = torch.zeros(6, v)
+    x[1, ::3] = -0.01
+    x[2] = -30.0
+    x[2, 7000:7400] = torch.randn(400, generator=torch.Generator().manual_seed(1))
+    x[3] = -torch.arange(v) * (8.0 / v)
+    x[4] = torch.arange(v) * (8.0 / v)
+    x[5, : v // 2] = -20.0
+    for top_p in (0.9, 0.5, 0.999):
+        check(x, torch.tensor([0.3, 0.7, 0.5, 0.99, 0.01, 0.6]), top_p=top_p)
+
+
 @pytest.mark.parametrize("min_p", [0.0, 1e-30, 0.01, 0.1, 0.5, 1.0])
 def test_min_p(min_p):
     check(*rows_of(8, 3, 9001), min_p=min_p, temperature=1.3)

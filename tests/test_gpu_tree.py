@@ -67,6 +67,34 @@ def test_many_query_rows(heads, kv, nodes):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,kv,nodes,first", [(4, 2, 24, 0), (8, 2, 40, 0), (8, 1, 65, 3), (2, 2, 100, 40)])
+@pytest.mark.parametrize("past", [[63, 64], [2000, 1], [4097, 900]])
+def test_many_query_rows_at_any_length(dtype, dim, heads, kv, nodes, first, past):
+    """48 to 496 query rows a kv head, splits of one and several chunks, ends inside chunks and pages."""
+    check(Case(nodes + past[0], past, nodes, heads, kv, dim, dtype=dtype, first=first, bs=16 if dim == 64 else 24))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("nodes", [12, 50, 90])
+def test_values_that_are_no_numbers_reach_who_sees_them(dtype, nodes):
+    """An infinite value of a node makes the outputs of the queries that see it
+    infinite, and no others'."""
+    case = Case(30, [40, 700], nodes, 8, 2, dtype=dtype)
+    want, spread, reach = case.reference()
+    at = (8 + 2) * 64 + 5  # v of kv head 0, dim 5
+    case.qkv[0, 3, at] = float("inf")
+    case.qkv[0, 3, at + 64] = float("nan")  # kv head 1
+    got = case.call(ops).cpu().double().view(2, nodes, 8, 64)
+    sees = case.seen[0, :, 3]
+    assert bool((got[0, sees, :4, 5] == float("inf")).all()) and bool(got[0, sees, 4:, 5].isnan().all())
+    ok = torch.ones(2, nodes, 8, 64, dtype=torch.bool)
+    ok[0, sees, :, 5] = False
+    off = (got - want.view_as(got)).abs()
+    assert bool((off <= case.tolerance(want, spread, reach).view_as(got))[ok].all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_rows_of_different_sizes(dtype):
     """Ragged lengths, rows of few live nodes and of none."""
     check(Case(5, [0, 1, 700, 64, 33, 128], 20, 4, 4, live=[20, 1, 7, 0, 19, 20], dtype=dtype))
@@ -86,9 +114,10 @@ def test_masks_that_leave_nothing(dtype):
     assert bool((got[0, 5] == 0).all()) and bool((got[1, 69] == 0).all())
 
 
-def test_nan_and_infinity_where_nothing_looks():
+@pytest.mark.parametrize("more", [0, 40])
+def test_nan_and_infinity_where_nothing_looks(more):
     """Values behind the cached length, of nodes that are not live or not seen, and of other rows' blocks."""
-    case = Case(8, [37, 20], 12, 4, 2, live=[12, 9])
+    case = Case(8, [37, 20], 12 + more, 4, 2, live=[12 + more, 9])
     seen_by_none = 7
     case.seen[0, :, seen_by_none] = False
     case.seen[0, seen_by_none, seen_by_none] = False
@@ -156,10 +185,11 @@ def test_max_kv_len_is_a_layout_only():
         check(case, max_kv_len=most)
 
 
-def test_bad_metadata_reads_nothing_out_of_range():
+@pytest.mark.parametrize("nodes,bs", [(5, 16), (5, 10), (60, 16)])
+def test_bad_metadata_reads_nothing_out_of_range(nodes, bs):
     """A table row, past or block id outside the tables and the pool, a position
     outside the rotation's tables: NaN in the rows concerned, the others right."""
-    case = Case(13, [40, 40, 40, 40, 40, 40, 40], 5, 4, 2)
+    case = Case(13, [40, 40, 40, 40, 40, 40, 40], nodes, 4, 2, bs=bs)
     want = case.call(ops).cpu()
     meta, tables, depth = case.meta.clone(), case.tables.clone(), case.depth.clone()
     meta[0, 0] = 1000
