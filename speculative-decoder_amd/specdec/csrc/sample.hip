@@ -11,22 +11,31 @@
 // up to that id.  No row is sorted as a whole.  One workgroup takes a row:
 //   1. It reads the row once, a wave a contiguous range.  The largest logits of
 //      its threads in the first part bound the k-th largest of the row from below
-//      (k of them are k logits), so what reaches that bound is collected in LDS on
-//      the way, together with the maximum and the sum of weights.
-//   2. The few hundred collected are ranked by counting; running sums over them
-//      give the cuts, and over their ids the token.  Most rows end here.
-//   3. A cut that is not among them (a nucleus of thousands of ids, a large
-//      top-k) is found by a histogram of the row over 2048 ranges of x, of counts
-//      or of weights, then by ranking the range that the cut falls into; the
-//      row is read again for each, mostly from the last-level cache.
-//   4. Without a cut, or past one, the sums of the waves' ranges say which range
-//      the token is in, and a scan of that range which id it is.
+//      (k of them are k logits), and min_p bounds by itself; what reaches the bound
+//      is collected in LDS on the way, together with the maximum and the sum of
+//      weights.
+//   2. The few hundred collected are ranked; running sums over them give the cuts,
+//      and over their ids the token.  Most rows end here.
+//   3. A nucleus of thousands of ids is found from a sample of the row and one more
+//      pass; a cut that is not found so (a large top_k, thousands of equal logits)
+//      by histograms of the row over 2048 ranges, of counts or of weights, and by
+//      ranking the range that it falls into.
+//   4. Without a cut, or past one of thousands, the sums of the waves' ranges say
+//      which range the token is in, and a scan of that range which id it is.
 //
 // Weights and their sums are held in 64 bits: a token is a comparison of u's
 // multiple of the total with a running sum of up to 2^18 weights, and in 32 bits
 // about one row in a hundred of a wide distribution would get the token beside.
-// A histogram's sums are integers, so their order does not matter: a weight in
-// units of 2^-45 of the largest that its range can hold.
+// Sums that atomics make are of integers, so their order does not matter: weights
+// in units of 2^-52, or of 2^-45 of the largest that a range can hold.
+//
+// What bounds it: greedy rows of 49152 the memory (512 rows 20.0 us, a copy's rate;
+// one row 6.5); otherwise a compute unit's vector instructions, 0.32 us for each
+// one an id of such a row, some 26 of them for a 64-bit weight: one row of the whole
+// softmax 22 us, 512 rows 43; top-k 50 20 and 37; min-p 0.05 13 and 30; a nucleus of
+// tens of ids 25 and 57, of 20000 57 and 102.  Rows fill one compute unit each, so a
+// call of few rows leaves the others idle; spreading a row over several needs a
+// second launch, whose cost on the host (3 us) and the GPU is what it would gain.
 #include "common.h"
 
 #include <float.h>
