@@ -29,13 +29,14 @@
 // Sums that atomics make are of integers, so their order does not matter: weights
 // in units of 2^-52, or of 2^-45 of the largest that a range can hold.
 //
-// What bounds it: greedy rows of 49152 the memory (512 rows 20.0 us, a copy's rate;
-// one row 6.5); otherwise a compute unit's vector instructions, 0.32 us for each
-// one an id of such a row, some 26 of them for a 64-bit weight: one row of the whole
-// softmax 22 us, 512 rows 43; top-k 50 20 and 37; min-p 0.05 13 and 30; a nucleus of
-// tens of ids 25 and 57, of 20000 57 and 102.  Rows fill one compute unit each, so a
-// call of few rows leaves the others idle; spreading a row over several needs a
-// second launch, whose cost on the host (3 us) and the GPU is what it would gain.
+// What bounds it: many greedy rows of 49152 fp32 logits the memory (512 rows 20.2
+// us, a copy's rate; one row 6.4).  Otherwise a compute unit's vector instructions:
+// by their issue rate each one an id of such a row is 0.32 us.  One row and 512 of
+// them, us: the whole softmax 22 and 44, top-k 50 21 and 37, min-p 0.05 13 and 30, a
+// nucleus of some ten ids 26 and 58, of some 16000 59 and 103.  Nuclei of 100 to 500
+// ids are the slowest of 512 rows: those that leave no row past 64 ids 58 us, those
+// with up to 256 as well 148; 512 copies of a row of 433 ids 190.  A call of few rows
+// leaves most compute units idle.
 #include "common.h"
 
 #include <float.h>
