@@ -733,13 +733,17 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
     const uint64_t past = __ballot((double)upto > goal), any = __ballot(s.sums[lane] > 0);
     const int part = past ? __ffsll((unsigned long long)past) - 1 : 63 - __clzll((long long)any);
     const uint64_t first = __shfl((unsigned long long)(upto - s.sums[lane]), part, kWave);
-    for (int q = tid; q < keep; q += THREADS) {
-      const int id = sorted_id(q);
-      if (id >> shift != part) continue;
+    // that 64th's ids by themselves: of hundreds kept a few
+    for (int q = tid; q < keep; q += THREADS)
+      if (sorted_id(q) >> shift == part) s.bins[atomicAdd(&s.count, 1)] = q;
+    __syncthreads();
+    const int members = s.count;
+    for (int i = tid; i < members; i += THREADS) {
+      const int q = (int)s.bins[i], id = sorted_id(q);
       uint64_t run = first;
-      for (int r = 0; r < keep; ++r) {
-        const int other = sorted_id(r);
-        run += other >> shift == part && other <= id ? (uint64_t)(s.weight[r] * unit52) : 0;
+      for (int j = 0; j < members; ++j) {
+        const int r = (int)s.bins[j];
+        run += sorted_id(r) <= id ? (uint64_t)(s.weight[r] * unit52) : 0;
       }
       if (s.weight[q] * unit52 >= 1.0) atomicMax(&s.last, id);
       if ((double)run > goal) atomicMin(&s.token, id);
