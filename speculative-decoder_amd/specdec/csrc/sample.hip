@@ -765,11 +765,10 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
   // below it, of which many ids have little each, so that a sample holds a like
   // share of it.  The row read once more gives the mass above that range of
   // logits and the ids in it, among which the cut is; false where it is not.
-  const auto nucleus = [&](Cut &cut) SAMPLE_INLINE {
+  bool crowded = false;  // more near the cut than a wave collects
+  const auto nucleus = [&](Cut &cut, double margin) SAMPLE_INLINE {
     double goal = p * total;
     constexpr int PARTS = 16 / EPL;  // pieces of a thread in the sample: 16 ids
-    // four times what a sum over some half of so many ids is off by
-    constexpr double margin = THREADS == 1024 ? 0.043 : 0.06;
     if (x.per < 2 * PARTS || !(c > 0.0)) return false;
     const float lo = (float)fmax(dtop - 31.7 / c, (double)-FLT_MAX);  // e^-22: what weighs less shares the last range
     if (!(lo < top)) return false;
@@ -850,7 +849,8 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
     __syncthreads();
     int most = 0;
     for (int w = 0; w < WAVES; ++w) most = max(most, s.wave_n[w]);
-    if (most > SHARE || !(above < goal)) return false;
+    crowded = most > SHARE;
+    if (crowded || !(above < goal)) return false;
     const auto mine = [&](int r) SAMPLE_INLINE { return sample_value((unsigned)(s.raw[wave][r] >> 32)); };
     for (int r = lane; r < have; r += kWave) {
       const float v = mine(r);
@@ -1021,7 +1021,16 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
   Cut cut = all_ids;
   bool summed = weigh && !by_p;  // `mass` is that of the cut
   if (by_p && k_row == 0) {
-    summed = nucleus(cut);
+    // four times what a sum over some half of the sample's ids is off by; where few ids
+    // hold much of the rest it is off by more, and few are near the cut, so there is
+    // room for a range that is wider
+    // four times what a sum over some half of the sample's ids is off by.  Where few ids
+    // hold much of the rest it is off by more, and few are near the cut: once more with
+    // room for that, before the histograms (512 rows of 49152, 142 -> 102 us; as a loop
+    // over the margins it spilled, and wide rows took 115 for 103).
+    constexpr double margin = THREADS == 1024 ? 0.043 : 0.06;
+    summed = nucleus(cut, margin);
+    if (!summed && !crowded) summed = nucleus(cut, 5 * margin);
     if (!sure) total = block.sum(weights_within(all_ids));
   }
 #pragma unroll 1

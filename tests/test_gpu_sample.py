@@ -88,6 +88,14 @@ def test_more_rows_than_compute_units(vocab, rows, kw):
     check(x, u, **kw)
 
 
+@pytest.mark.parametrize("rows", [5, 300])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("steep", [1.15, 1.3, 1.45])
+def test_nuclei_of_hundreds(steep, dtype, rows):
+    """More than a wave ranks, and few ids that hold much of what the nucleus leaves."""
+    check(*flat_rows(int(100 * steep), rows, 16411, dtype, steep), top_p=0.9)
+
+
 def test_wide_nuclei_that_no_sample_shows():
     """Rows of one value; of two; weights that only a stretch of ids has; ids in falling and rising order."""
     v = 49152
