@@ -33,10 +33,10 @@
 // us, a copy's rate; one row 6.4).  Otherwise a compute unit's vector instructions:
 // by their issue rate each one an id of such a row is 0.32 us.  One row and 512 of
 // them, us: the whole softmax 22 and 44, top-k 50 21 and 37, min-p 0.05 13 and 30, a
-// nucleus of some ten ids 26 and 58, of some 16000 59 and 103.  Nuclei of 100 to 500
-// ids are the slowest of 512 rows: those that leave no row past 64 ids 58 us, those
-// with up to 256 as well 148; 512 copies of a row of 433 ids 190.  A call of few rows
-// leaves most compute units idle.
+// nucleus of some ten ids 26 and 58, of some 16000 58 and 103.  Slower are rows that
+// the first sample is off for (512 copies of one of 433 ids 138), and bf16 rows with
+// wide nuclei, which spill (65 and 116).  A call of few rows leaves most compute
+// units idle.
 #include "common.h"
 
 #include <float.h>
