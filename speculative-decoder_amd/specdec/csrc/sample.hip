@@ -38,6 +38,7 @@
 // wide nuclei, which spill (65 and 116).  A call of few rows leaves most compute
 // units idle.
 #include "common.h"
+#include "sample_ranges.h"
 
 #include <float.h>
 #include <limits.h>
@@ -50,7 +51,6 @@ namespace specdec {
 
 constexpr int kSamplePieces = 6;    // pieces of 16 bytes of a part; the next part's are in flight
 constexpr int kSampleShare = 512;   // logits that a wave collects
-constexpr int kSampleBins = 2048;
 constexpr int kSampleTopK = 400;    // the largest top_k that is bounded by the threads' maxima
 constexpr double kSampleOff = 1.0 / (1 << 17);
 constexpr int kSampleGuess = 128;   // reach the bound in the first part, for a nucleus of unknown size
@@ -930,8 +930,8 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
         return shorter(in, Cut{hi, to});
       }
       const double step = ((double)hi - (double)lo) / kSampleBins;
-      const float scale = (float)(1.0 / step);
-      const auto bin_of = [&](float v) SAMPLE_INLINE { return (int)fminf((hi - v) * scale, kSampleBins - 1.0f); };
+      const SampleRanges ranges(lo, hi);
+      const auto bin_of = [&](float v) SAMPLE_INLINE { return ranges.of(v); };
       // a bin's unit is the least power of two that the largest weight it can hold is
       // below 2^bits of; what weighs less than 2^-900 is not told from nothing
       for (int q = tid; q < kSampleBins; q += THREADS) {
