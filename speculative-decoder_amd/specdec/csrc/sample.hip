@@ -545,13 +545,16 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
   const Cut all_ids{-FLT_MAX, INT_MAX};
   // against the row's largest now, or again where the first part was too far from it
   // For a nucleus the sum is that of 32-bit exponentials, a third of the work: they
-  // are off by 2^-23 and 2^-23 |y| of their powers y, |y| < 40 where they weigh at
-  // all, so by less than kSampleOff together.  Where that leaves a choice the sum is
-  // taken again in 64 bits.
+  // are off by 2^-23 and some 2^-23 |y| of their powers y of two, from the roundings
+  // of c, the difference and the product.  The largest power is at most 40 here, and
+  // what is 40 below it weighs next to nothing, so they are off by 41 2^-23 or less,
+  // with their sums' roundings by less than kSampleOff (64 2^-23).  Where that leaves
+  // a choice the sum is taken again in 64 bits, and at once where the largest power is
+  // more.
   bool sure = !by_p;
   if (weigh) {
     const double up = (base - dtop) * c;
-    if (up > (by_p ? -100.0 : -900.0) && up <= 0.0) mass *= sample_weight((float)base, dtop, c);
+    if (up > (by_p ? -40.0 : -900.0) && up <= 0.0) mass *= sample_weight((float)base, dtop, c);
     else {
       mass = weights_within(all_ids);
       sure = true;
