@@ -410,6 +410,9 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
   const bool by_p = !greedy && p_row < 1.0f, by_m = !greedy && m_row > 0.0f;
   const double p = fmax((double)p_row, 0.0), m = fmin((double)m_row, 1.0);
   const double c = greedy ? 0.0 : 1.4426950408889634074 / (double)t_row;
+  // powers in 32 bits: c is an fp32 number of full precision, and a difference that is
+  // none is a power past all that counts
+  const bool single = c > 1e-30 && c < 1e38;
   const float uu = a.u[row];
   const double u = uu > 0.0f ? (double)fminf(uu, 1.0f) : 0.0;
   float *probs = a.probs ? a.probs + row * a.probs_stride : nullptr;
@@ -550,11 +553,11 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
   // what is 40 below it weighs next to nothing, so they are off by 41 2^-23 or less,
   // with their sums' roundings by less than kSampleOff (64 2^-23).  Where that leaves
   // a choice the sum is taken again in 64 bits, and at once where the largest power is
-  // more.
+  // more or 32 bits do not hold c and the differences.
   bool sure = !by_p;
   if (weigh) {
     const double up = (base - dtop) * c;
-    if (up > (by_p ? -40.0 : -900.0) && up <= 0.0) mass *= sample_weight((float)base, dtop, c);
+    if (up > (by_p ? -40.0 : -900.0) && up <= 0.0 && (single || !by_p)) mass *= sample_weight((float)base, dtop, c);
     else {
       mass = weights_within(all_ids);
       sure = true;
@@ -772,7 +775,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
   const auto nucleus = [&](Cut &cut, double margin) SAMPLE_INLINE {
     double goal = p * total;
     constexpr int PARTS = 16 / EPL;  // pieces of a thread in the sample: 16 ids
-    if (x.per < 2 * PARTS || !(c > 0.0)) return false;
+    if (x.per < 2 * PARTS || !single) return false;
     const float lo = (float)fmax(dtop - 31.7 / c, (double)-FLT_MAX);  // e^-22: what weighs less shares the last range
     if (!(lo < top)) return false;
     const float scale = (float)(kSampleBins / ((double)top - (double)lo)), c32 = (float)c;

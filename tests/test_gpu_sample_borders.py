@@ -76,3 +76,57 @@ def test_the_largest_logits_past_the_first_part(top_p, kept):
     probs = torch.empty_like(x, device="cuda")
     ops.sample(x.cuda(), u.cuda(), t.cuda(), top_p=top_p, probs=probs)
     assert (probs > 0).sum(1).tolist() == [kept] * 48
+
+
+def check_near(x, u, temperature, top_k=0, top_p=1.0, min_p=0.0):
+    """As check, where a cut may lie so near to a border that 64 bits do not tell:
+    34 weights of 1 and 33 of e^-34 are 34 or 34 + 6e-14 by the order of their sum,
+    and half of that is 17 of them or 18.  Sums of n weights are off by n 2^-53, a
+    weight by 1e-13 at most (4e-14 in the kernel and the rounding of its power of at
+    most 62 where it counts), so a goal this near to a prefix's mass may be on either
+    side of it; the token and the distribution have to be those of the prefix taken."""
+    f32 = lambda v: float(torch.tensor(v, dtype=torch.float32))
+    temperature, top_p, min_p = f32(temperature), f32(top_p), f32(min_p)
+    probs = torch.full(x.shape, 9.0, device="cuda")
+    got = ops.sample(x.cuda(), u.cuda(), temperature, top_k, top_p, min_p, probs=probs).cpu()
+    probs = probs.cpu().double()
+    n = x.shape[1]
+    off = 4 * n * 2.0 ** -53 + 1e-13
+    for r in range(len(x)):
+        ids = torch.argsort(x[r].double(), descending=True, stable=True)
+        if top_k:
+            ids = ids[:top_k]
+        e = x[r].double()[ids]
+        w = torch.where(e == e[0], 1.0, torch.exp((e - e[0]) / temperature))
+        mass, ends = w.cumsum(0), []
+        for side in (-1, 1):
+            keep = len(ids)
+            if top_p < 1:
+                keep = min(keep, int((mass < (top_p + side * off) * mass[-1]).sum()) + 1)
+            if min_p > 0:
+                keep = min(keep, max(1, int((w >= min_p * (1 - side * off)).sum())))
+            ends.append(keep)
+        keep = min(max(int((probs[r] > 0).sum()), ends[0]), ends[1])
+        p = torch.zeros(n, dtype=torch.float64)
+        p[ids[:keep]] = w[:keep] / w[:keep].sum()
+        assert torch.equal(probs[r] > 0, p.float() > 0), (r, ends)
+        assert bool(((probs[r] - p).abs() <= p * 2.0 ** -23 + 2.0 ** -149).all()), r
+        run = p.cumsum(0)
+        token = int(((run > float(u[r])) & (p > 0)).nonzero()[0])
+        assert int(got[r]) == token or float((run - float(u[r])).abs().min()) < off, (r, int(got[r]), token)
+
+
+@pytest.mark.parametrize("vocab", [100, 3001])
+@pytest.mark.parametrize("kw", [dict(top_p=0.5), dict(top_p=0.9, min_p=0.3), dict(top_k=60, top_p=0.7), dict(min_p=0.6), {}])
+@pytest.mark.parametrize("temperature", [1e-45, 1e-40, 1e-39, 1e-37, 1e-32, 1e32, 1e37, 3.3e38])
+def test_temperatures_at_the_ends_of_fp32(temperature, kw, vocab):
+    """Powers of two that no fp32 product of a difference and 1 / temperature
+    holds: rows of one value, of values that weigh alike at this temperature, and of
+    values that weigh next to nothing beside the first."""
+    g = torch.Generator().manual_seed(vocab)
+    x = torch.zeros(5, vocab)
+    x[1] = (torch.randn(vocab, generator=g).double() * min(temperature, 1e37)).float()
+    x[2] = torch.randn(vocab, generator=g)
+    x[3] = torch.tensor([-MOST, 0.0, MOST])[torch.randint(0, 3, (vocab,), generator=g)]
+    x[4] = (torch.randint(-3, 1, (vocab,), generator=g).double() * min(temperature, 1e38)).float()
+    check_near(x, torch.rand(5, generator=g), temperature, **kw)
