@@ -152,6 +152,15 @@ def verify_tree(target, cache: KVCache, seq_ids: list[int], contexts: list[list[
     return verdict
 
 
+def _drawn(req: _Request, n: int, tokens: list[int]) -> None:
+    """Raises for a row that has no token to go on with, which a next forward would
+    look up as id -1: its logits hold no number (ops.sample), or its path no slot
+    (ops.tree_commit, n = -1)."""
+    if n < 0 or tokens[-1] < 0:
+        raise RuntimeError(f"seq {req.seq_id}: no token after {len(req.context)} tokens; the target's logits there are "
+                           "no numbers, or the cache has no slot for them")
+
+
 @torch.no_grad()
 def generate_tree(target, cache: KVCache, drafter: TreeDrafter, prompts: list[list[int]], max_new_tokens: int,
                   temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0,
@@ -161,7 +170,8 @@ def generate_tree(target, cache: KVCache, drafter: TreeDrafter, prompts: list[li
     prompt's new tokens and the statistics.  Every token is a draw from the
     target's distribution under temperature, top-k, top-p and min-p, with
     uniforms from `generator`: one a row for the first token, then one a node
-    and round.  Events as `spec.loop.generate`'s."""
+    and round.  A row whose logits hold no number is an error.  Events as
+    `spec.loop.generate`'s."""
     gen = generator if generator is not None else torch.Generator().manual_seed(0)
     event = on_event if on_event is not None else (lambda name: None)
     stats = TreeStats()
@@ -173,6 +183,8 @@ def generate_tree(target, cache: KVCache, drafter: TreeDrafter, prompts: list[li
     logits = run(target, cache, seq_ids, prompts)
     firsts = draw(logits, uniforms(len(prompts)), temperature, top_k, top_p, min_p).tolist()
     event("first_token")
+    for req, token in zip(requests, firsts):
+        _drawn(req, 0, [token])
     drafter.prefill(seq_ids, [r.context for r in requests])
     event("draft_prefilled")
     live = []
@@ -193,6 +205,7 @@ def generate_tree(target, cache: KVCache, drafter: TreeDrafter, prompts: list[li
         survivors = []
         for req, (n, after, *drafted) in zip(live, verdict):
             kept = _cut(drafted[:n] + [after], max_new_tokens - len(req.output), eos_id)
+            _drawn(req, n, kept)
             stats.drafted += tokens.shape[1] - 1
             stats.accepted += n
             stats.emitted_per_round.append(len(kept))
