@@ -130,25 +130,40 @@ def verify_tree(target, cache: KVCache, seq_ids: list[int], contexts: list[list[
     on the GPU.  tokens int64 [B, N]; parents [B or 1, N] on the host; u fp32 [B,
     N].  The cache holds the contexts but their last tokens on entry, and room
     for each row's longest path on return: the caller truncates it to the past
-    and the n + 1 nodes that the verdict keeps."""
+    and the n + 1 nodes that the verdict keeps.  A call that raises leaves its
+    lengths as they were."""
     for seq_id, ctx in zip(seq_ids, contexts):
         if cache.length(seq_id) != len(ctx) - 1:
             raise RuntimeError(f"seq {seq_id}: target cache holds {cache.length(seq_id)}, expected {len(ctx) - 1}")
-    b, n = tokens.shape
+    b = len(seq_ids)
+    if tokens.dim() != 2 or tokens.shape[0] != b or len(contexts) != b or not 0 < tokens.shape[1] <= ops.TREE_NODES:
+        raise ValueError(f"tokens must be [{b}, N] of at most {ops.TREE_NODES} nodes for {len(contexts)} contexts "
+                         f"(got {list(tokens.shape)})")
+    n = tokens.shape[1]
+    if parents.dim() != 2 or parents.shape[0] not in (1, b) or parents.shape[1] != n:
+        raise ValueError(f"parents must be [{b} or 1, {n}] (got {list(parents.shape)})")
+    if u.numel() != b * n:
+        raise ValueError(f"u must be [{b}, {n}], a uniform a node (got {list(u.shape)})")
     llama = as_llama(target, cache.device)
     mask, depth = trees.plan(parents)
     room = int(depth.max()) + 1
-    step = cache.append(seq_ids, [room] * b, nodes=[n] * b)
-    llama.ensure_positions(step.max_total)
-    tokens = tokens.to(cache.device, torch.int64)
-    up = parents.to(torch.int32).to(cache.device, non_blocking=True)
-    past = max(step.past)
-    tree = TreeStep(mask.to(cache.device, non_blocking=True), depth.to(cache.device, non_blocking=True),
-                    TreeStep.store(llama, b, n), past)
-    logits = forward_core(llama, cache, step.meta, tokens, past, tree=tree)
-    sampled = draw(logits, u, temperature, top_k, top_p, min_p)
-    verdict, _ = ops.tree_commit(tokens, up, sampled, step.meta, room, tree.qkv, llama.rope_cos, llama.rope_sin, cache.k,
-                                 cache.v, cache.table_tensor)
+    try:
+        step = cache.append(seq_ids, [room] * b, nodes=[n] * b)
+        llama.ensure_positions(step.max_total)
+        tokens = tokens.to(cache.device, torch.int64)
+        up = parents.to(torch.int32).to(cache.device, non_blocking=True)
+        past = max(step.past)
+        tree = TreeStep(mask.to(cache.device, non_blocking=True), depth.to(cache.device, non_blocking=True),
+                        TreeStep.store(llama, b, n), past)
+        logits = forward_core(llama, cache, step.meta, tokens, past, tree=tree)
+        sampled = draw(logits, u, temperature, top_k, top_p, min_p)
+        verdict, _ = ops.tree_commit(tokens, up, sampled, step.meta, room, tree.qkv, llama.rope_cos, llama.rope_sin, cache.k,
+                                     cache.v, cache.table_tensor)
+    except Exception:
+        # rows that have grown, too few blocks for the rest among the reasons
+        for seq_id, ctx in zip(seq_ids, contexts):
+            cache.truncate(seq_id, len(ctx) - 1)
+        raise
     return verdict
 
 

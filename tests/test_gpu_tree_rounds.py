@@ -35,3 +35,39 @@ def test_logits_that_are_no_numbers_end_the_rounds(monkeypatch):
             generate_tree(target, cache_for(target), drafter, prompts, 9, temperature=0.8)
         assert len(calls) == good + 1
     torch.cuda.synchronize()
+
+
+def test_a_verify_that_fails_leaves_the_cache_as_it_was():
+    """A tree of too many nodes, uniforms, rows or parents of another size, a
+    parameter out of range and too few blocks: the rows' lengths and blocks stay, and
+    a right call after them works."""
+    model = tiny64(1)
+    prompts = random_prompts(2, 256, 18)
+    cache = cache_for(model, blocks=8)
+    for s, p in enumerate(prompts):
+        cache.add(s)
+        forward(model, cache, [s], torch.tensor([p[:-1]]), [len(p) - 1])
+    lengths, used = [cache.length(s) for s in (0, 1)], cache.allocator.num_used
+    parents = tree_shape([2, 1])
+    tokens = torch.randint(0, 256, (2, 5), generator=torch.Generator().manual_seed(0))
+    tokens[:, 0] = torch.tensor([p[-1] for p in prompts])
+    u = torch.rand(2, 5, generator=torch.Generator().manual_seed(1))
+    good = dict(target=model, cache=cache, seq_ids=[0, 1], contexts=prompts, tokens=tokens, parents=parents, u=u)
+    wide, chain = tree_shape([255]), tree_shape([1] * 200)
+    for kind, change in [
+            (ValueError, dict(tokens=torch.zeros(2, 257, dtype=torch.int64), parents=torch.cat([wide, wide[:, -1:]], 1), u=torch.rand(2, 257))),
+            (ValueError, dict(u=u[:, :4])), (ValueError, dict(u=u[:1])), (ValueError, dict(tokens=tokens[:1])),
+            (ValueError, dict(tokens=tokens[0])), (ValueError, dict(parents=parents[:, :4])), (ValueError, dict(parents=parents[0])),
+            (ValueError, dict(parents=parents.repeat(3, 1))), (ValueError, dict(top_p=1.5)), (ValueError, dict(temperature=-1.0)),
+            (Exception, dict(tokens=torch.zeros(2, 201, dtype=torch.int64), parents=chain, u=torch.rand(2, 201)))]:
+        with pytest.raises(kind):
+            verify_tree(**{**good, **change})
+        assert [cache.length(s) for s in (0, 1)] == lengths, change.keys()
+        assert cache.allocator.num_used == used, change.keys()
+    verdict = verify_tree(**good)
+    for b, p in enumerate(prompts):
+        alone = cache_for(model)
+        alone.add(0)
+        forward(model, alone, [0], torch.tensor([p[:-1]]), [len(p) - 1])
+        one = verify_tree(model, alone, [0], [p], tokens[b:b + 1], parents, u[b:b + 1])
+        assert verdict[:, b].tolist() == one[:, 0].tolist()
