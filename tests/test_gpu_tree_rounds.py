@@ -37,6 +37,71 @@ def test_logits_that_are_no_numbers_end_the_rounds(monkeypatch):
     torch.cuda.synchronize()
 
 
+def plain_logits(model, context):
+    """The logits after a context, by a forward over all of it."""
+    cache = cache_for(model)
+    cache.add(0)
+    return forward(model, cache, [0], torch.tensor([context]), [len(context)])[0, -1].float().cpu()
+
+
+@pytest.mark.parametrize("branching", [[2], [3, 2, 1], [1, 1, 1]])
+def test_each_token_is_drawn_with_its_node_s_uniform(branching):
+    """The generator replayed: the first tokens', then for each round a uniform a row
+    and node.  From node 0 the token is the draw from the target's restricted
+    distribution after the path, by a plain forward and a sort in 64 bits, with the
+    uniform of the path's node; where a child carries it the path goes on there.  The
+    tree's sums are ordered otherwise than a plain forward's (2e-4 of the logits), so
+    a u nearer to its token's border than 1e-3 of the mass tells nothing.  The same
+    with another node's uniforms has to disagree."""
+    target = tiny64(2)
+    prompts = random_prompts(3, 256, 14)
+    f32 = lambda v: float(torch.tensor(v, dtype=torch.float32))
+    kw = dict(temperature=0.9, top_k=20, top_p=0.95, min_p=0.01)
+    drafter = ModelTree(early_exit(target), cache_for(early_exit(target)), branching)
+    proposals = []
+    propose = drafter.propose
+
+    def recorded(seq_ids, contexts):
+        tokens, parents = propose(seq_ids, contexts)
+        proposals.append((list(seq_ids), [list(c) for c in contexts], tokens.cpu(), parents))
+        return tokens, parents
+
+    drafter.propose = recorded
+    out, stats = generate_tree(target, cache_for(target), drafter, prompts, 14,
+                               generator=torch.Generator().manual_seed(3), **kw)
+    final = [p + o for p, o in zip(prompts, out)]
+    assert stats.accepted > 0 and [len(o) for o in out] == [14] * 3
+
+    def drawn(context, u):
+        token, _, gap = tree_ref.draw(plain_logits(target, context), float(u), f32(0.9), 20, f32(0.95), f32(0.01))
+        return token, gap
+
+    replay = torch.Generator().manual_seed(3)
+    for p, f, u in zip(prompts, final, torch.rand(3, generator=replay)):
+        token, gap = drawn(p, u)
+        assert f[len(p)] == token or gap < 1e-3
+    told, other, deep = 0, 0, 0
+    for ids, contexts, tokens, parents in proposals:
+        u = torch.rand(*tokens.shape, generator=replay)
+        for row, (seq, context) in enumerate(zip(ids, contexts)):
+            node, at = 0, len(context)
+            assert context == final[seq][:at]
+            while at < len(final[seq]):
+                token, gap = drawn(final[seq][:at], u[row, node])
+                assert final[seq][at] == token or gap < 1e-3, (seq, at, node)
+                told += gap >= 1e-3
+                deep += node > 0
+                wrong, wrong_gap = drawn(final[seq][:at], u[row, (node + 1) % u.shape[1]])
+                other += wrong != final[seq][at] and wrong_gap >= 1e-3
+                token, at = final[seq][at], at + 1
+                child = [c for c in range(node + 1, tokens.shape[1])
+                         if int(parents[0, c]) == node and int(tokens[row, c]) == token]
+                if not child:
+                    break
+                node = child[0]
+    assert told > 20 and deep > 0 and other > 0
+
+
 def test_a_verify_that_fails_leaves_the_cache_as_it_was():
     """A tree of too many nodes, uniforms, rows or parents of another size, a
     parameter out of range and too few blocks: the rows' lengths and blocks stay, and
