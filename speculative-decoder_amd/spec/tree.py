@@ -75,6 +75,8 @@ class ModelTree:
     none of it enters the draft's cache, which holds the context alone."""
 
     def __init__(self, model, cache: KVCache, branching: list[int]) -> None:
+        if not branching:
+            raise ValueError("a tree to draft has a level at least (got none)")
         self.model, self.cache, self.branching = model, cache, list(branching)
         self.parents = tree_shape(self.branching)
         mask, depth = trees.plan(self.parents)

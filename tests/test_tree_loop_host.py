@@ -71,3 +71,11 @@ def test_a_round_without_a_token_ends_the_call(monkeypatch, bad):
     with pytest.raises(RuntimeError, match="seq 1.*no token"):
         go()
     assert drafter.proposed == 2  # the second round's, and none after it
+
+
+def test_a_drafter_has_a_level_at_least():
+    with pytest.raises(ValueError, match="level"):
+        rounds.ModelTree(None, SimpleNamespace(device=torch.device("cpu")), [])
+    with pytest.raises(ValueError, match="child"):
+        rounds.ModelTree(None, SimpleNamespace(device=torch.device("cpu")), [2, 0])
+    assert rounds.tree_shape([]).tolist() == [[-1]]  # a tree of node 0 alone can be verified
