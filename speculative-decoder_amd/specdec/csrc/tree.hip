@@ -240,6 +240,18 @@ __device__ __forceinline__ void tree_row_pieces(const TreeArgs &a, const T *row,
   }
 }
 
+// The scale of scores in log2 units, above 0 so that a hidden key's -inf stays that
+// and the largest score is the largest after it: a negative scale is taken into q's
+// sign (exact), and 0 is the least fp32 number, which leaves every finite score less
+// than 2^-20.
+__device__ __forceinline__ float tree_scale(float scale) {
+  const float sc = fabsf(scale) * 1.4426950408889634f;
+  return sc == 0.0f ? 0x1p-149f : sc;
+}
+template <typename T> __device__ __forceinline__ unsigned tree_sign(float scale) {
+  return scale < 0.0f ? (sizeof(T) == 2 ? 0x80008000u : 0x80000000u) : 0u;
+}
+
 // How a call is cut: tiles of a wave, groups of them over a kv head's query
 // rows, splits over the cached keys.
 struct TreeCut {
@@ -298,15 +310,18 @@ __global__ __launch_bounds__(kTreeWaves *kWave)
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int qr = min(row0 + 16 * t + c, nrows - 1), node = a.first + qr / G;
-    if (t < tiles)
+    if (t < tiles) {
       tree_row_pieces<T, D>(a, rows + node * a.token_stride + (int64_t)(hk * G + qr % G) * D, (int64_t)r.past + depth[node], g,
                             q[t]);
+#pragma unroll
+      for (int j = 0; j < NP; ++j) q[t][j] ^= tree_sign<T>(a.scale);
+    }
     m[t] = -INFINITY;
     l[t] = 0.0f;
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  const float sc = a.scale * 1.4426950408889634f;  // scores in log2 units
+  const float sc = tree_scale(a.scale);
 
   // the chunk's weights of tile t, in log2 units against the running maximum,
   // which is raised when a score passes it by 2^8 only: rarely after the first
@@ -609,12 +624,14 @@ tree_attention_shared_kernel(TreeArgs a, TreeCut cut, int shift, float *ws) {
     const int qr = min(first_row(t) + c, nrows - 1), node = a.first + qr / G;
     tree_row_pieces<T, D>(a, rows + node * a.token_stride + (int64_t)(hk * G + qr % G) * D, (int64_t)r.past + depth[node], g,
                           q[t]);
+#pragma unroll
+    for (int j = 0; j < NP; ++j) q[t][j] ^= tree_sign<T>(a.scale);
     m[t] = -INFINITY;
     l[t] = 0.0f;
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  const float sc = a.scale * 1.4426950408889634f;
+  const float sc = tree_scale(a.scale);
 
   // half a chunk (CK keys) of buffer `buf` against this wave's tiles; hide(t, s) puts
   // the scores of keys that a query does not see to -inf
