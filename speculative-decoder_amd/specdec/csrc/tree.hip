@@ -282,22 +282,13 @@ __global__ __launch_bounds__(kTreeWaves *kWave)
   __shared__ float s_o[NW][MT][16][D + 4];
   __shared__ float s_ml[NW][MT][16][2];
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, c = lane & 15, g = lane / 16;
-  // query groups that read the same keys run next to one another on one XCD,
-  // whose L2 then serves all but the first (workgroups go to the XCDs in turn)
-  const int units = a.batch * a.Hkv * cut.splits;
-  int unit = blockIdx.x, qg = 0;
-  if (cut.groups > 1) {
-    const int rest = unit / 8;
-    qg = rest % cut.groups;
-    unit = rest / cut.groups * 8 + unit % 8;
-    if (unit >= units) return;
-  }
+  const int units = a.batch * a.Hkv * cut.splits, unit = blockIdx.x;
   const int split = unit % cut.splits, bh = unit / cut.splits, hk = bh % a.Hkv, b = bh / a.Hkv;
   const int G = a.H / a.Hkv;
   const TreeRow r = tree_row(a, b);
-  const int row0 = qg * NT * 16, nrows = (r.live - a.first) * G;
-  if (row0 >= nrows) return;
-  const int tiles = min(NT, (nrows - row0 + 15) / 16);
+  const int nrows = (r.live - a.first) * G;
+  if (nrows <= 0) return;
+  const int tiles = min(NT, (nrows + 15) / 16);
   bool bad = !r.fits;
   const int past = r.fits ? r.past : 0, live = r.live;
   const T *rows = (const T *)a.qkv + b * a.batch_stride;
@@ -309,7 +300,7 @@ __global__ __launch_bounds__(kTreeWaves *kWave)
   float m[NT], l[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    const int qr = min(row0 + 16 * t + c, nrows - 1), node = a.first + qr / G;
+    const int qr = min(16 * t + c, nrows - 1), node = a.first + qr / G;
     if (t < tiles) {
       tree_row_pieces<T, D>(a, rows + node * a.token_stride + (int64_t)(hk * G + qr % G) * D, (int64_t)r.past + depth[node], g,
                             q[t]);
@@ -386,7 +377,7 @@ __global__ __launch_bounds__(kTreeWaves *kWave)
       if (t >= tiles) break;
       float s[EPL];
       scores(t, k, s);
-      const int qr = min(row0 + 16 * t + c, nrows - 1);
+      const int qr = min(16 * t + c, nrows - 1);
       const uint64_t word = a.mask[b * a.mask_batch_stride + qr / G * a.mask_row_stride + n0 / 64];
       const unsigned seen = (unsigned)(word >> (n0 % 64 + EPL * g));
 #pragma unroll
@@ -529,7 +520,7 @@ __global__ __launch_bounds__(kTreeWaves *kWave)
     __syncthreads();
     for (int x = tid; x < MT * 16 * (D / 4); x += NW * kWave) {
       const int u = x / (4 * D), rr = x / (D / 4) % 16, d = x % (D / 4) * 4;
-      const int qr = row0 + 16 * (t0 + u) + rr;
+      const int qr = 16 * (t0 + u) + rr;
       if (qr >= nrows) continue;
       float top = -INFINITY, sum = 0.0f;
 #pragma unroll
@@ -595,8 +586,10 @@ tree_attention_shared_kernel(TreeArgs a, TreeCut cut, int shift, float *ws) {
   __shared__ S sh;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, c = lane & 15, g = lane / 16;
   const int units = a.batch * a.Hkv * cut.splits;
+  // query groups that read the same keys run next to one another on one XCD,
+  // whose L2 then serves all but the first (workgroups go to the XCDs in turn)
   int unit = blockIdx.x, qg = 0;
-  if (cut.groups > 1) {  // as above: query groups of one unit on one XCD
+  if (cut.groups > 1) {
     const int rest = unit / 8;
     qg = rest % cut.groups;
     unit = rest / cut.groups * 8 + unit % 8;

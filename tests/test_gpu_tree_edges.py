@@ -30,3 +30,16 @@ def test_scales_that_are_not_positive(heads, kv, nodes, bs, dtype, scale):
     scale of 0 is the mean of what is seen.  One or two tiles of query rows, many that
     share their keys, and blocks that the tiles do not take."""
     check_scaled(Case(nodes, [70, 0, 700], nodes, heads, kv, bs=bs, dtype=dtype), scale)
+
+
+@pytest.mark.parametrize("room", [1, 2, 4, 31, 32, 33, 100])
+def test_commit_goes_on_to_its_room_and_no_further(room):
+    """Chains of 40 nodes whose tokens are all as sampled: the path takes every slot
+    that it may, and every node where there are more."""
+    case = Commit(room, [3, 30, 7], 40, room=room, vocab=1)
+    case.parents = (torch.arange(40, dtype=torch.int32) - 1).expand(3, 40).contiguous()
+    verdict, path, _, _ = case.call()
+    n = min(room, 40)
+    assert verdict[0].tolist() == [n - 1] * 3
+    assert path.cpu().tolist() == [list(range(n)) + [-1] * (40 - n)] * 3
+    case.check()
