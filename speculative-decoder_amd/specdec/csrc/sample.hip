@@ -1096,8 +1096,10 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
     for (int k = 0; k < AT; ++k) mine += w[k];
   }
   double at = run + block.scan(mine);
-  // the threads whose ids the sum passes the goal in, or nearly
-  if (goal == INFINITY || (at <= goal * (1.0 + 1e-12) && (at + mine) * (1.0 + 1e-12) >= goal)) {
+  // the threads whose ids the sum passes the goal in, or nearly: the range was chosen by
+  // a sum in another order, off by up to n 2^-53 for the n <= 2^15 ids of a lane
+  constexpr double near = 0x1p-36;
+  if (goal == INFINITY || (at <= goal * (1.0 + near) && (at + mine) * (1.0 + near) >= goal)) {
     for (int i = i0; i < i1; i += AT) {
       if (each > AT) ids(i, w);
 #pragma unroll

@@ -130,3 +130,16 @@ def test_temperatures_at_the_ends_of_fp32(temperature, kw, vocab):
     x[3] = torch.tensor([-MOST, 0.0, MOST])[torch.randint(0, 3, (vocab,), generator=g)]
     x[4] = (torch.randint(-3, 1, (vocab,), generator=g).double() * min(temperature, 1e38)).float()
     check_near(x, torch.rand(5, generator=g), temperature, **kw)
+
+
+@pytest.mark.parametrize("kw", [{}, dict(top_p=0.9), dict(top_k=50, top_p=0.95), dict(top_k=100000, top_p=0.5), dict(min_p=0.01)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_widest_rows(dtype, kw):
+    """2^24 ids, and a few fewer from an address that is not aligned."""
+    g = torch.Generator().manual_seed(5)
+    x = (torch.randn(1, 1 << 24, generator=g) * 1.5).to(dtype)
+    u = torch.rand(1, generator=g)
+    check(x, u, **kw)
+    if not kw:
+        got = ops.sample(x.cuda()[:, 3:-2], u.cuda())
+        assert int(got) == int(check(x[:, 3:-2].contiguous(), u))
