@@ -637,10 +637,11 @@ int specdec_tree_attention_workspace(int32_t batch, int32_t nodes, int32_t first
  * out_token_stride apart, apart from the inputs) receives the softmax-weighted
  * values, zeros for a query that sees nothing; queries that are not live are
  * not written.  The cache is read only.  head_dim 64 or 128.  Softmax in fp32 with
- * `scale`.  max_kv_len is the cached length that the launch is laid out for;
- * longer rows are right too, and slower.  Without the whole of
- * specdec_tree_attention_workspace's floats the call runs without any; calls
- * sharing a workspace must be ordered. */
+ * `scale`, of any sign; in BF16 its weights are rounded to BF16 for the product with
+ * the values (each by 2^-8 of itself at most), their sum takes them unrounded.
+ * max_kv_len is the cached length that the launch is laid out for; longer rows are
+ * right too, and slower.  Without the whole of specdec_tree_attention_workspace's
+ * floats the call runs without any; calls sharing a workspace must be ordered. */
 int specdec_tree_attention(const void *qkv, int dtype, int64_t batch_stride, int64_t token_stride,
                            const float *cos_table, const float *sin_table, int64_t max_positions,
                            const void *k_pool, const void *v_pool, int64_t num_blocks,

@@ -29,14 +29,18 @@
 // Sums that atomics make are of integers, so their order does not matter: weights
 // in units of 2^-52, or of 2^-45 of the largest that a range can hold.
 //
-// What bounds it: many greedy rows of 49152 fp32 logits the memory (512 rows 20.2
-// us, a copy's rate; one row 6.4).  Otherwise a compute unit's vector instructions:
-// by their issue rate each one an id of such a row is 0.32 us.  One row and 512 of
-// them, us: the whole softmax 22 and 44, top-k 50 21 and 37, min-p 0.05 13 and 30, a
-// nucleus of some ten ids 26 and 58, of some 16000 58 and 103.  Slower are rows that
-// the first sample is off for (512 copies of one of 433 ids 138), and bf16 rows with
-// wide nuclei, which spill (65 and 116).  A call of few rows leaves most compute
-// units idle.
+// What bounds it: many greedy rows of 49152 fp32 logits the memory (512 rows 20.3
+// us, a copy's rate; one row 6.4).  Otherwise one row a compute unit's vector
+// instructions: the whole softmax is 37 k of them, 15 of its 22 us by their issue rate
+// (4 cycles at 2.4 GHz), each one an id 0.32 us; a call of few rows leaves most
+// compute units idle.  512 rows of mixed nuclei wait more than they issue (39 of 104
+// us): two rows a unit, and barriers between the steps.  One row and 512 of them, us:
+// the whole softmax 22 and 45, top-k 50 20 and 36, min-p 0.05 13 and 29, a nucleus of
+// some ten ids 25 and 58, of some 16000 58 and 103.  Slower are rows that the first
+// sample is off for (512 copies of one of 433 ids 138), bf16 rows with wide nuclei,
+// which spill (66 and 114), and cuts inside thousands of equal logits, which a search
+// over ids reads the row some 17 times for (one bf16 row of 128001, the cut inside
+// 2000: top-k 313, a nucleus 482).
 #include "common.h"
 #include "sample_ranges.h"
 
@@ -51,7 +55,11 @@ namespace specdec {
 
 constexpr int kSamplePieces = 6;    // pieces of 16 bytes of a part; the next part's are in flight
 constexpr int kSampleShare = 512;   // logits that a wave collects
-constexpr int kSampleTopK = 400;    // the largest top_k that is bounded by the threads' maxima
+// The largest top_k that is bounded by the threads' maxima; larger ones go by
+// histograms.  One row of 49152 at 400 and 401: 27.8 and 56.6 us, 64 rows 30.7 and 58.5.
+// Of 512 rows, whose workgroups have half of the maxima, 39 at 200, 109 at 300, 142 at
+// 400 and 120 at 401: there histograms are the faster ones from some 330 on.
+constexpr int kSampleTopK = 400;
 constexpr double kSampleOff = 1.0 / (1 << 17);
 constexpr int kSampleGuess = 128;   // reach the bound in the first part, for a nucleus of unknown size
 
@@ -870,7 +878,8 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
     double run = above + block.scan(sum);
 #pragma unroll
     for (int q = 0; q < N; ++q) {
-      // the first bin that the sum passes the goal in, by more than the units round
+      // the first bin that the sum reaches the goal in; weights in whole units are short
+      // by less than 2^-32 of the range's largest together
       if (run < goal && run + in_bin[q] >= goal) {
         s.token = N * tid + q;
         s.above = run;
@@ -1027,9 +1036,6 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4, 4)))
   Cut cut = all_ids;
   bool summed = weigh && !by_p;  // `mass` is that of the cut
   if (by_p && k_row == 0) {
-    // four times what a sum over some half of the sample's ids is off by; where few ids
-    // hold much of the rest it is off by more, and few are near the cut, so there is
-    // room for a range that is wider
     // four times what a sum over some half of the sample's ids is off by.  Where few ids
     // hold much of the rest it is off by more, and few are near the cut: once more with
     // room for that, before the histograms (512 rows of 49152, 142 -> 102 us; as a loop

@@ -163,9 +163,14 @@ __global__ __launch_bounds__(kWave) void tree_attention_any_kernel(TreeArgs a) {
 // end, where the workgroup's waves fold their (m, l, O).
 // A lane's row of K holds pieces j and j + NP / 2 of a rotated pair of dims, so the
 // tree's own keys are rotated in the registers that they arrive in.
+// In bf16 the second product takes P in bf16, as the other attention kernels here do:
+// each weight is off by 2^-8 of itself at most, while l sums them in fp32 as they
+// were.  Two halves of P would double that product's instructions.  Against 64 bits the
+// outputs are off by 0.0021 to 0.0022 of their size where one rounding at the end
+// leaves 0.0016 to 0.0017 (the bf16 cases of perf/more_operators.py).
 // Bound by memory: 8 rows of 32 nodes at 4096 keys, 32 heads of 64, 55 us for 241 MB
 // (85% of a copy's rate); by the dependent round trips of metadata, tables, nodes
-// and keys where these are few (one row of 16 nodes at 300 keys 7.1 us).
+// and keys where these are few (one row of 16 nodes at 300 keys 7.3 us).
 constexpr int kTreeWaves = 4;
 
 template <typename T, int D> struct TreeTile {
@@ -557,8 +562,8 @@ __global__ __launch_bounds__(kTreeWaves *kWave)
 // nodes at 4096 keys, one query head a kv head, 85 -> 65 us (73% of the bytes at a
 // copy's rate); 4 rows of 64 nodes at 8000 keys, four query heads a kv head of 64,
 // 72 -> 46, and of 128, where that grid has room for two tiles, 116 -> 76.  There it
-// is bound by its instructions: 11.5 k vector and 1.8 k matrix instructions a SIMD
-// are some 31 of the 60 us, with two waves a SIMD to hide the rest; the splits'
+// is bound by its instructions: 11.6 k vector and 1.8 k matrix instructions a SIMD
+// are some 31 of the 63 us, with two waves a SIMD to hide the rest; the splits'
 // partials (34 MB) and their fold are most of the others.
 // K is kept in the order of the score tiles' rows, rows of 4 NP pieces; V as in the
 // cache, rows of 8 pieces; a piece's place in its row is its number xor the row's
@@ -956,8 +961,8 @@ constexpr int kCommitHeads = 8;  // kv heads of a workgroup
 // VEC: a thread takes 16 bytes of each half of a head's k and v.  The path's nodes
 // are its threads' fastest index, so that neighbours write neighbouring slots of a
 // V row, whose elements lie a block apart from dim to dim: those 2-byte stores are
-// what it is bound by (one element of one head a thread at a time took 86 us where
-// this takes 41: 32 rows, 24 layers of 32 heads of 64).
+// what it is bound by: some 28 MB of 32 rows, 24 layers of 32 heads of 64, leave as 79
+// MB, 41 us (one element of one head a thread at a time took 86).
 template <typename T, bool VEC> __global__ __launch_bounds__(kCommitThreads) void tree_commit_kernel(CommitArgs a) {
   const int b = blockIdx.x, layer = blockIdx.y, tid = threadIdx.x, lane = tid & (kWave - 1);
   __shared__ int64_t tokens[kTreeMaxNodes], sampled[kTreeMaxNodes];
