@@ -143,3 +143,24 @@ def test_the_widest_rows(dtype, kw):
     if not kw:
         got = ops.sample(x.cuda()[:, 3:-2], u.cuda())
         assert int(got) == int(check(x[:, 3:-2].contiguous(), u))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kw", [{}, dict(top_p=0.9), dict(top_k=50, top_p=0.95), dict(top_k=1000), dict(min_p=0.05), dict(temperature=0.0),
+                                dict(top_p=0.999, min_p=0.0001)])
+def test_vocabularies_that_a_mask_leaves_little_of(kw, dtype):
+    """Rows whose first half, all but a few ids, all but the last or all but a stretch are
+    -inf, and rows with NaN or the type's lowest value in their place."""
+    v = 49152
+    g = torch.Generator().manual_seed(4)
+    x = (torch.randn(10, v, generator=g) * 2).to(dtype)
+    keep = torch.zeros(10, v, dtype=torch.bool)
+    keep[0, v // 2:] = keep[6, v // 2:] = keep[8, v // 2:] = True
+    keep[1, torch.randperm(v, generator=g)[:40]] = True
+    keep[2, -1] = True
+    keep[3, 30000:30700] = keep[7, 30000:30700] = keep[9, 30000:30700] = True
+    keep[4] = torch.arange(v) % 3072 >= 1536  # nothing in the part that is read first
+    keep[5, torch.randperm(v, generator=g)[:3000]] = True
+    fill = torch.tensor([float("-inf")] * 6 + [float("nan")] * 2 + [torch.finfo(dtype).min] * 2).to(dtype)
+    x = torch.where(keep, x, fill[:, None])
+    check(x, torch.rand(10, generator=g), **kw)
