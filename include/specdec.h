@@ -667,9 +667,9 @@ int specdec_tree_attention(const void *qkv, int dtype, int64_t batch_stride, int
  * and its v, from qkv [layers, batch, nodes, (H + 2 Hkv) * head_dim], are written
  * to slot past + j of k_pool [layers, num_blocks, Hkv, block_size, head_dim] and
  * v_pool [layers, num_blocks, Hkv, head_dim, block_size]; the row's table must
- * hold the blocks of `room` slots, and the path ends before a slot outside the
- * tables, the pool or the positions.  A row with no live node or no slot gets n =
- * -1 and token -1.  head_dim even. */
+ * hold the blocks of `room` slots, of which no two rows may share one, and the path
+ * ends before a slot outside the tables, the pool or the positions.  A row with no
+ * live node or no slot gets n = -1 and token -1.  head_dim even. */
 int specdec_tree_commit(const int64_t *tokens, int64_t tokens_stride, const int32_t *parents,
                         int64_t parents_stride, const int64_t *sampled, int64_t sampled_stride,
                         const int32_t *meta, int32_t batch, int32_t nodes, int32_t room,

@@ -142,6 +142,8 @@ def verify_tree(target, cache: KVCache, seq_ids: list[int], contexts: list[list[
         raise ValueError(f"tokens must be [{b}, N] of at most {ops.TREE_NODES} nodes for {len(contexts)} contexts "
                          f"(got {list(tokens.shape)})")
     n = tokens.shape[1]
+    if len(set(seq_ids)) != b:
+        raise ValueError(f"each sequence is verified once a call (got {list(seq_ids)})")
     if parents.dim() != 2 or parents.shape[0] not in (1, b) or parents.shape[1] != n:
         raise ValueError(f"parents must be [{b} or 1, {n}] (got {list(parents.shape)})")
     if u.numel() != b * n:

@@ -1402,9 +1402,9 @@ def tree_commit(tokens: torch.Tensor, parents: torch.Tensor, sampled: torch.Tens
     qkv [layers, B, N, (H + 2 Hkv) * head_dim] are the projections that the
     layers' tree_attention read; path node j's k, rotated at position past + j, and
     v go to slot past + j of the pools [layers, blocks, ..], whose tables hold the
-    blocks of `room` slots past each row's cached length.  The path has at most
-    `room` nodes (N where not given).  A row without a live node or a slot gets n =
-    -1 and token -1."""
+    blocks of `room` slots past each row's cached length; no two rows of a call may
+    write the same slots.  The path has at most `room` nodes (N where not given).  A
+    row without a live node or a slot gets n = -1 and token -1."""
     index = tokens.get_device()
     if index < 0:
         gpu(tokens, "tokens")

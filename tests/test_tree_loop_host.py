@@ -79,3 +79,10 @@ def test_a_drafter_has_a_level_at_least():
     with pytest.raises(ValueError, match="child"):
         rounds.ModelTree(None, SimpleNamespace(device=torch.device("cpu")), [2, 0])
     assert rounds.tree_shape([]).tolist() == [[-1]]  # a tree of node 0 alone can be verified
+
+
+def test_a_sequence_has_one_row_of_a_verify():
+    cache = SimpleNamespace(length=lambda s: 1, device=torch.device("cpu"))
+    with pytest.raises(ValueError, match="once"):
+        rounds.verify_tree(None, cache, [3, 3], [[1, 2], [1, 2]], torch.tensor([[2, 5], [2, 6]]), torch.tensor([[-1, 0]]),
+                           torch.zeros(2, 2))
