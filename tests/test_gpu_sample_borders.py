@@ -48,9 +48,10 @@ def test_close_values_in_more_rows_than_compute_units(cut):
 
 def late_rows(count):
     """(x [2 count, 49152], u, temperatures): two equal logits hold all the weight,
-    some 95 powers of two above what a thread of each wave reads first (wave w's ids
-    are 3072 w .. and its first part half of them); temperatures at which a power in
-    32 bits is off by most, short of it and past it."""
+    some 95 powers of two above what each wave reads first (of 16 waves a 16th of the
+    ids each, its first part half of them); temperatures at which a power in 32 bits is
+    off by most, short of it and past it."""
+    wave = 49152 // 16
     rng = np.random.default_rng(0)
     f = np.float32
     t = rng.uniform(0.2, 1.5, 200000).astype(f)
@@ -63,8 +64,8 @@ def late_rows(count):
     g = torch.Generator().manual_seed(1)
     x = torch.randn(2 * count, 49152, generator=g) * 0.3 - 5
     for r, i in enumerate(pick):
-        x[r, 3072 * 2 + 40 + r] = float(low[i])
-        x[r, 3072 * 3 + 1900] = x[r, 3072 * 9 + 1700 + r] = float(high[i])
+        x[r, wave * 2 + 40 + r] = float(low[i])
+        x[r, wave * 3 + 1900] = x[r, wave * 9 + 1700 + r] = float(high[i])
     return x, torch.rand(2 * count, generator=g), torch.from_numpy(t[pick])
 
 
@@ -159,7 +160,7 @@ def test_vocabularies_that_a_mask_leaves_little_of(kw, dtype):
     keep[1, torch.randperm(v, generator=g)[:40]] = True
     keep[2, -1] = True
     keep[3, 30000:30700] = keep[7, 30000:30700] = keep[9, 30000:30700] = True
-    keep[4] = torch.arange(v) % 3072 >= 1536  # nothing in the part that is read first
+    keep[4] = torch.arange(v) % (v // 16) >= v // 32  # nothing in the part that is read first
     keep[5, torch.randperm(v, generator=g)[:3000]] = True
     fill = torch.tensor([float("-inf")] * 6 + [float("nan")] * 2 + [torch.finfo(dtype).min] * 2).to(dtype)
     x = torch.where(keep, x, fill[:, None])
